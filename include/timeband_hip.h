@@ -128,6 +128,62 @@ int tb_head_fwd(const float* x, const float* w, const float* b, float* out, long
 int tb_head_bwd(const float* dy, const float* out, const float* x, const float* w, float* dx, float* dw, float* db,
                 long M, int K, int act, int accumulate, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- state space layer: short causal convolution, selective scan, linear with residual -------------------------------------
+ * A recurrent layer beside the LSTM whose steps need not wait for each other (no counterpart in the reference, whose only
+ * recurrence is nn.LSTM, source/utils/lstm_layer.py:31-33,75).  Element types: dtype 0 fp32, 1 bf16, 2 fp16, one for all the
+ * tensors of a call unless they are typed float here; sums and states are fp32, an output is rounded once.  Strides count
+ * elements; the last axis is always dense.  act: 0 none, 1 tanh, 2 sigmoid, 3 relu, 4 silu, 5 gelu (error-function form).
+ *
+ * Convolution: y[b,t,d] = act(bias[d] + sum_k w[d,k] x[b,t-K+1+k,d]), act none or silu, K = 1 .. 8.
+ *   x (B,T,D), w (D,K), bias (D) nullable; w_f32 != 0: w and bias (and dw, db) are fp32 whatever dtype.
+ *   state (B,K-1,D) nullable: the inputs before step 0 (zero without).  lengths (B) int32 nullable: steps at or behind a
+ *   sequence's length are not read, their outputs and gradients are zero.  state_out (B,K-1,D) nullable: the last K-1 inputs of each
+ *   sequence; it must not be `state`.
+ *   backward: dx (B,T,D) dense, dw / db nullable; dy dense.
+ *   step: x (B,D) with rows x_batch_stride apart, state rows (K-1,D) dense and state_batch_stride apart, shifted IN PLACE. */
+int tb_conv_fwd(const void* x, long x_batch_stride, long x_step_stride, const void* w, const void* bias, int w_f32,
+                const void* state, const int* lengths, void* y, void* state_out, int B, int T, int D, int K, int act, int dtype,
+                void* stream);
+size_t tb_conv_bwd_workspace_bytes(int B, int T, int D, int K, int dtype);
+int tb_conv_bwd(const void* dy, const void* x, long x_batch_stride, long x_step_stride, const void* w, const void* bias, int w_f32,
+                const void* state, const int* lengths, void* dx, void* dw, void* db, int B, int T, int D, int K, int act, int dtype,
+                void* ws, size_t ws_bytes, void* stream);
+int tb_conv_step(const void* x, long x_batch_stride, void* state, long state_batch_stride, const void* w, const void* bias, int w_f32,
+                 void* y, int B, int D, int K, int act, int dtype, void* stream);
+
+/* Selective scan, N = 1 .. 64 states a channel, G groups of D / G channels:
+ *   delta = softplus(dt + dt_bias) (softplus == 0: dt + dt_bias); h = exp(delta A) h + delta u B; out = (C.h + Dp u) silu(z)
+ *   u, dt, z (B,T,D), z nullable; Bm, Cm (B,T,G,N); A (D,N), Dp (D), dt_bias (D) fp32, the last two nullable;
+ *   h0, hT (B,D,N) fp32, nullable; lengths as above (a step that does not count leaves the state as it is).
+ *   strides: HOST array {u batch, u step, dt batch, dt step, z batch, z step, B batch, B step, B group, C batch, C step, C group}
+ *   and, for the backward pass, {dout batch, dout step}; for the step {u, dt, z, B batch, B group, C batch, C group}.
+ *   states: tb_scan_states_bytes, nullable; the forward pass leaves there what the backward pass starts its tiles from.
+ *   backward: dhT (B,D,N) nullable; du, ddt, dz (B,T,D), dB, dC (B,T,G,N) dense, dA, dD, dbias, dh0 fp32, each nullable.
+ *   step: u, dt, z, out (B,D), Bm, Cm (B,G,N); state rows (D,N) dense fp32, state_batch_stride apart, updated IN PLACE. */
+size_t tb_scan_workspace_bytes(int B, int T, int D, int N, int G, int backward);
+size_t tb_scan_states_bytes(int B, int T, int D, int N);
+int tb_scan_fwd(const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const long* strides, const float* A,
+                const float* Dp, const float* dt_bias, int softplus, const float* h0, const int* lengths, void* out, float* hT,
+                float* states, int B, int T, int D, int N, int G, int dtype, void* ws, size_t ws_bytes, void* stream);
+int tb_scan_bwd(const void* dout, const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const long* strides,
+                const float* A, const float* Dp, const float* dt_bias, int softplus, const int* lengths, const float* states,
+                const float* dhT, void* du, void* ddt, void* dz, void* dB, void* dC, float* dA, float* dD, float* dbias, float* dh0,
+                int B, int T, int D, int N, int G, int dtype, void* ws, size_t ws_bytes, void* stream);
+int tb_scan_step(float* state, long state_batch_stride, const void* u, const void* dt, const void* z, const void* Bm, const void* Cm,
+                 const long* strides, const float* A, const float* Dp, const float* dt_bias, int softplus, void* out, int B, int D, int N,
+                 int G, int dtype, void* stream);
+
+/* Linear with bias, activation and residual: y[M,N] = act(x[M,K].W[N,K]^T + b[N]) + residual[M,N]  (tb_linear_act_fwd beside it
+ * is fp32 through split bf16 products, without residual).  b, residual nullable.  z (M,N) fp32 nullable: the pre-activation,
+ * which the backward pass needs when act != 0.  backward: dz = dy act'(z), dx = dz.W, dW = dz^T.x, db = colsum(dz), each
+ * nullable and dense; the residual's gradient is dy itself. */
+size_t tb_linres_workspace_bytes(long M, int K, int N, int dtype, int backward);
+int tb_linres_fwd(const void* x, long x_row_stride, const void* W, long w_row_stride, const void* b, const void* residual,
+                  long residual_row_stride, void* y, float* z, long M, int K, int N, int act, int dtype, void* ws, size_t ws_bytes,
+                  void* stream);
+int tb_linres_bwd(const void* dy, long dy_row_stride, const void* x, long x_row_stride, const void* W, long w_row_stride, const float* z,
+                  int act, void* dx, void* dW, void* db, long M, int K, int N, int dtype, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- losses (source/loss.py) ---------------------------------------------------------------------
  * tb_loss_sums: one pass over whichever inputs are non-NULL into a device double[8]:
  *   [0] sum (Dy-0.9)^2  [1] sum (DGx-0.1)^2  [2] sum Dy  [3] sum DGx  [4] sum SmoothL1(pred-true)

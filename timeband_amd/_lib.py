@@ -50,6 +50,18 @@ SIGNATURES = {
     "tb_head_workspace_bytes": (Z, [L, I]),
     "tb_head_fwd": (I, [P, P, P, P, L, I, I, P]),
     "tb_head_bwd": (I, [P, P, P, P, P, P, P, L, I, I, I, P, Z, P]),
+    "tb_conv_fwd": (I, [P, L, L, P, P, I, P, P, P, P, I, I, I, I, I, I, P]),
+    "tb_conv_bwd_workspace_bytes": (Z, [I, I, I, I, I]),
+    "tb_conv_bwd": (I, [P, P, L, L, P, P, I, P, P, P, P, P, I, I, I, I, I, I, P, Z, P]),
+    "tb_conv_step": (I, [P, L, P, L, P, P, I, P, I, I, I, I, I, P]),
+    "tb_scan_workspace_bytes": (Z, [I, I, I, I, I, I]),
+    "tb_scan_states_bytes": (Z, [I, I, I, I]),
+    "tb_scan_fwd": (I, [P, P, P, P, P, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, P, Z, P]),
+    "tb_scan_bwd": (I, [P, P, P, P, P, P, P, P, P, P, I, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, P, Z, P]),
+    "tb_scan_step": (I, [P, L, P, P, P, P, P, P, P, P, P, I, P, I, I, I, I, I, P]),
+    "tb_linres_workspace_bytes": (Z, [L, I, I, I, I]),
+    "tb_linres_fwd": (I, [P, L, P, L, P, P, L, P, P, L, I, I, I, I, P, Z, P]),
+    "tb_linres_bwd": (I, [P, L, P, L, P, L, P, I, P, P, P, L, I, I, I, P, Z, P]),
     "tb_loss_workspace_bytes": (Z, []),
     "tb_loss_sums": (I, [P, L, P, L, P, P, L, P, P, Z, P]),
     "tb_loss_finish": (I, [P, I, D, D, D, D, F, F, F, P, P, P, P]),

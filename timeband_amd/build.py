@@ -15,7 +15,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtimeband_hip.so")
-SOURCES = ["capi.hip", "gemm.hip", "lstm.hip", "losses.hip", "postproc.hip", "head.hip"]
+SOURCES = ["capi.hip", "gemm.hip", "lstm.hip", "losses.hip", "postproc.hip", "head.hip", "conv.hip", "scan.hip", "linres.hip"]
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (some of their forms have given wrong results on this part now and then); the
 # host pass does not know the feature and says so, which is harmless.
 FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",

@@ -1,0 +1,414 @@
+// Short causal depthwise convolution over (B, T, D), channels last, with bias and SiLU: forward, backward, one step.
+//
+//   pre[b,t,c] = bias[c] + sum_k w[c,k] x[b, t-K+1+k, c]        y = act(pre)
+// with x before step 0 taken from `state` (B, K-1, D) or 0, and steps at or behind lengths[b] left out (y = 0 there).
+//   dpre = dy act'(pre)    dx[t] = sum_j w[j] dpre[t+K-1-j]    dw[j] = sum_{b,t} dpre[t] x[t-K+1+j]    db = sum dpre
+//
+// Bound by memory: 2 K operations an element against 2 elements moved (forward), 4 moved backward.  A thread owns VEC channels
+// (16 bytes) and walks a run of steps with the K-1 last inputs in registers, so that each element is read once, plus K-1 of
+// its neighbour's a run; lanes are neighbours in the channels, so a wave reads whole lines.  Backward recomputes pre from x
+// instead of keeping it (K multiplications against 2 or 4 bytes an element written and read).
+#include "elem.h"
+
+namespace {
+
+constexpr int KMAX = 8;
+
+struct ConvArgs {
+  const void *x, *w, *bias, *state, *dy;
+  const int* lengths;
+  void *y, *state_out, *dx;
+  float* slab;               // backward: [blocks along the runs][K + 1][D] sums of dw and db
+  long sxb, sxt;             // strides of x in elements; y, dy, dx, state are dense
+  int B, T, D, run, runs;    // runs of `run` steps each, `runs` of them a sequence
+  int act, wf32;
+};
+
+template <typename T, int VEC>
+__device__ __forceinline__ void load_x(const ConvArgs& a, int b, long t, int len, int K, int c, float (&r)[VEC]) {
+  if (t >= 0 && t < len) {
+    tb_load_n(static_cast<const T*>(a.x) + b * a.sxb + t * a.sxt + c, r);
+  } else if (t < 0 && a.state && t >= 1 - K) {
+    tb_load_n(static_cast<const T*>(a.state) + ((long)b * (K - 1) + (K - 1 + t)) * a.D + c, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) r[i] = 0.f;
+  }
+}
+
+// block: blockDim.x channel groups of VEC by blockDim.y runs
+template <typename T, int K, int VEC>
+__global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
+  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * VEC;
+  const long r = (long)blockIdx.y * blockDim.y + threadIdx.y;
+  if (c >= a.D || r >= (long)a.B * a.runs) return;
+  const int b = (int)(r / a.runs), q = (int)(r % a.runs);
+  const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+  const int t0 = q * a.run, t1 = min(t0 + a.run, a.T);
+  float w[K][VEC], bias[VEC], win[K][VEC];
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) w[k][i] = tb_load_par<T>(a.w, (long)(c + i) * K + k, a.wf32);
+    bias[i] = a.bias ? tb_load_par<T>(a.bias, c + i, a.wf32) : 0.f;
+  }
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
+  T* y = static_cast<T*>(a.y) + ((long)b * a.T) * a.D + c;
+  for (int t = t0; t < t1; ++t) {
+    load_x<T, VEC>(a, b, t, len, K, c, win[K - 1]);
+    float o[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      float s = bias[i];
+#pragma unroll
+      for (int k = 0; k < K; ++k) s = fmaf(w[k][i], win[k][i], s);
+      if (a.act == TB_ACT_SILU) s = tb_silu(s);
+      o[i] = t < len ? s : 0.f;
+    }
+    tb_store_n(y + (long)t * a.D, o);
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) win[k][i] = win[k + 1][i];
+  }
+  if (a.state_out && q == 0) {
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) {
+      float s[VEC];
+      load_x<T, VEC>(a, b, (long)len - (K - 1) + k, len, K, c, s);
+      tb_store_n(static_cast<T*>(a.state_out) + ((long)b * (K - 1) + k) * a.D + c, s);
+    }
+  }
+}
+
+template <typename T, int K, int VEC>
+__global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
+  __shared__ float red[256];
+  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * VEC;
+  const long r = (long)blockIdx.y * blockDim.y + threadIdx.y;
+  const bool on = c < a.D && r < (long)a.B * a.runs;
+  float dw[K + 1][VEC];
+#pragma unroll
+  for (int k = 0; k <= K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) dw[k][i] = 0.f;
+  if (on) {
+    const int b = (int)(r / a.runs), q = (int)(r % a.runs);
+    const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
+    const int t0 = q * a.run, t1 = min(t0 + a.run, a.T);
+    float w[K][VEC], bias[VEC], win[K][VEC], dp[K][VEC];   // win: x[s-K+1 .. s]; dp: dpre[s-K+1 .. s]
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        w[k][i] = tb_load_par<T>(a.w, (long)(c + i) * K + k, a.wf32);
+        dp[k][i] = 0.f;
+      }
+      bias[i] = a.bias ? tb_load_par<T>(a.bias, c + i, a.wf32) : 0.f;
+    }
+#pragma unroll
+    for (int k = 0; k < K - 1; ++k) load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
+    const T* dy = static_cast<const T*>(a.dy) + (long)b * a.T * a.D + c;
+    T* dx = static_cast<T*>(a.dx) + (long)b * a.T * a.D + c;
+    for (int s = t0; s < t1 + K - 1; ++s) {
+      load_x<T, VEC>(a, b, s, len, K, c, win[K - 1]);
+      float g[VEC];
+      if (s < len) {
+        tb_load_n(dy + (long)s * a.D, g);
+        if (a.act == TB_ACT_SILU) {
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            float p = bias[i];
+#pragma unroll
+            for (int k = 0; k < K; ++k) p = fmaf(w[k][i], win[k][i], p);
+            const float sg = tb_sig(p);
+            g[i] *= sg * (1.f + p * (1.f - sg));
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) g[i] = 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dp[K - 1][i] = g[i];
+      if (s < t1) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+          for (int k = 0; k < K; ++k) dw[k][i] = fmaf(g[i], win[k][i], dw[k][i]);
+          dw[K][i] += g[i];
+        }
+      }
+      const int t = s - (K - 1);                   // dx[t] needs dpre[t .. t+K-1] = dp[0 .. K-1]
+      if (t >= t0) {
+        float o[VEC];
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          float v = 0.f;
+#pragma unroll
+          for (int k = 0; k < K; ++k) v = fmaf(w[K - 1 - k][i], dp[k][i], v);
+          o[i] = t < len ? v : 0.f;
+        }
+        tb_store_n(dx + (long)t * a.D, o);
+      }
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          win[k][i] = win[k + 1][i];
+          dp[k][i] = dp[k + 1][i];
+        }
+    }
+  }
+  // sums of the block's runs, in the order of the runs
+#pragma unroll
+  for (int k = 0; k <= K; ++k)
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+      red[threadIdx.y * blockDim.x + threadIdx.x] = dw[k][i];
+      __syncthreads();
+      if (threadIdx.y == 0 && c < a.D) {
+        float s = 0.f;
+        for (int j = 0; j < (int)blockDim.y; ++j) s += red[j * blockDim.x + threadIdx.x];
+        a.slab[((long)blockIdx.y * (K + 1) + k) * a.D + c + i] = s;
+      }
+      __syncthreads();
+    }
+}
+
+// dw (D, K), db (D) from the slab's rows, summed in their order by sixteen threads a column
+template <typename T>
+__global__ void __launch_bounds__(1024) conv_finish(const float* slab, long rows, int K, int D, void* dw, void* db, int wf32) {
+  __shared__ float red[16][65];
+  const long cols = (long)(K + 1) * D;
+  const long col = (long)blockIdx.x * 64 + threadIdx.x;
+  float s = 0.f;
+  if (col < cols) {
+    const long per = (rows + 15) / 16;
+    const long r1 = min(rows, (threadIdx.y + 1) * per);
+#pragma unroll 4
+    for (long r = threadIdx.y * per; r < r1; ++r) s += slab[r * cols + col];
+  }
+  red[threadIdx.y][threadIdx.x] = s;
+  __syncthreads();
+  if (threadIdx.y == 0 && col < cols) {
+    s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s += red[j][threadIdx.x];
+    const int k = (int)(col / D), d = (int)(col % D);
+    if (k < K) {
+      if (dw) tb_store_par<T>(dw, (long)d * K + k, s, wf32);
+    } else if (db) {
+      tb_store_par<T>(db, d, s, wf32);
+    }
+  }
+}
+
+struct ConvStepArgs {
+  const void *x, *w, *bias;
+  void *state, *y;
+  long sxb, ssb;     // strides of a row of x and of a row of state
+  int B, D, act, wf32;
+};
+
+// state (K-1, D) of a row: shifted by one, x appended, in place; a thread reads and writes its own channels only
+template <typename T, int K, int VEC>
+__global__ void __launch_bounds__(256) conv_step(ConvStepArgs a) {
+  const int groups = a.D / VEC;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (long)a.B * groups) return;
+  const int b = (int)(id / groups), c = (int)(id % groups) * VEC;
+  T* st = static_cast<T*>(a.state) + b * a.ssb + c;
+  float win[K][VEC], o[VEC];
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) tb_load_n(st + (long)k * a.D, win[k]);
+  tb_load_n(static_cast<const T*>(a.x) + b * a.sxb + c, win[K - 1]);
+#pragma unroll
+  for (int i = 0; i < VEC; ++i) {
+    float s = a.bias ? tb_load_par<T>(a.bias, c + i, a.wf32) : 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) s = fmaf(tb_load_par<T>(a.w, (long)(c + i) * K + k, a.wf32), win[k][i], s);
+    o[i] = a.act == TB_ACT_SILU ? tb_silu(s) : s;
+  }
+#pragma unroll
+  for (int k = 0; k < K - 1; ++k) tb_store_n(st + (long)k * a.D, win[k + 1]);
+  tb_store_n(static_cast<T*>(a.y) + (long)b * a.D + c, o);
+}
+
+// one instantiation per (type, taps, vector width): F is called with the kernel's template arguments
+template <typename F>
+int by_shape(int dtype, int K, bool vec, F&& f) {
+#define TB_K(T, V)                                                          \
+  switch (K) {                                                              \
+    case 1: return f.template operator()<T, 1, V>();                        \
+    case 2: return f.template operator()<T, 2, V>();                        \
+    case 3: return f.template operator()<T, 3, V>();                        \
+    case 4: return f.template operator()<T, 4, V>();                        \
+    case 5: return f.template operator()<T, 5, V>();                        \
+    case 6: return f.template operator()<T, 6, V>();                        \
+    case 7: return f.template operator()<T, 7, V>();                        \
+    default: return f.template operator()<T, 8, V>();                       \
+  }
+  if (dtype == TB_F32) {
+    if (vec) TB_K(float, 4) else TB_K(float, 1)
+  } else if (dtype == TB_BF16) {
+    if (vec) TB_K(__bf16, 8) else TB_K(__bf16, 1)
+  } else {
+    if (vec) TB_K(_Float16, 8) else TB_K(_Float16, 1)
+  }
+#undef TB_K
+}
+
+struct FwdLaunch {
+  ConvArgs a;
+  dim3 grid, block;
+  hipStream_t s;
+  template <typename T, int K, int V>
+  int operator()() {
+    conv_fwd<T, K, V><<<grid, block, 0, s>>>(a);
+    return 0;
+  }
+};
+struct BwdLaunch {
+  ConvArgs a;
+  dim3 grid, block;
+  hipStream_t s;
+  template <typename T, int K, int V>
+  int operator()() {
+    conv_bwd<T, K, V><<<grid, block, 0, s>>>(a);
+    return 0;
+  }
+};
+struct StepLaunch {
+  ConvStepArgs a;
+  hipStream_t s;
+  template <typename T, int K, int V>
+  int operator()() {
+    const long n = (long)a.B * (a.D / V);
+    conv_step<T, K, V><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    return 0;
+  }
+};
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct Plan {
+  int vec, bx, by, run, runs;
+  long gx, gy;
+};
+
+// Steps a run: enough runs to fill the chip (about 2^18 threads), but no fewer than 8 steps (each run reads K-1 steps of its
+// neighbour's again) and no more than 64.
+Plan plan(int B, int T, int D, int vec) {
+  Plan p;
+  p.vec = vec;
+  const int groups = (D + vec - 1) / vec;
+  p.bx = 64;
+  while (p.bx > 1 && p.bx / 2 >= groups) p.bx /= 2;
+  p.by = 256 / p.bx;
+  const long want = ((long)B * T * groups) >> 18;
+  p.run = (int)(want < 8 ? 8 : want > 64 ? 64 : want);
+  p.runs = (T + p.run - 1) / p.run;
+  p.gx = (groups + p.bx - 1) / p.bx;
+  p.gy = ((long)B * p.runs + p.by - 1) / p.by;
+  return p;
+}
+
+int check_common(const char* what, int B, long T, int D, int K, int act, int dtype) {
+  if (B < 0 || T < 0 || D < 1) return tb_set_error(TB_ERR_ARG, "%s: bad sizes B=%d T=%ld D=%d", what, B, T, D);
+  if (K < 1 || K > KMAX) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: %d taps are not supported (1 to %d)", what, K, KMAX);
+  if (act != 0 && act != TB_ACT_SILU) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: activation %d is not supported (none, silu)", what, act);
+  if (!tb_dtype_ok(dtype)) return tb_set_error(TB_ERR_ARG, "%s: bad element type %d", what, dtype);
+  return TB_OK;
+}
+
+bool can_vec(int dtype, int D, long sb, long st, const void* const* p, int n) {
+  const int v = dtype == TB_F32 ? 4 : 8;
+  if (D % v || sb % v || st % v) return false;
+  for (int i = 0; i < n; ++i)
+    if (!aligned(p[i])) return false;
+  return true;
+}
+
+// grid.y is 16 bits wide in some launch paths; the runs' blocks stay far below that
+int check_grid(const char* what, const Plan& p) {
+  if (p.gy > 65535 || p.gx > 0x7fffffffL) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: too many sequences in one call", what);
+  return TB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int tb_conv_fwd(const void* x, long x_batch_stride, long x_step_stride, const void* w, const void* bias, int w_f32,
+                const void* state, const int* lengths, void* y, void* state_out, int B, int T, int D, int K, int act, int dtype,
+                void* stream) {
+  int rc = check_common("conv_fwd", B, T, D, K, act, dtype);
+  if (rc) return rc;
+  if (B == 0 || (T == 0 && !state_out)) return TB_OK;
+  if (!w || (T > 0 && (!x || !y))) return tb_set_error(TB_ERR_ARG, "conv_fwd: null pointer");
+  const void* ptrs[] = {x, y, state, state_out};
+  const bool vec = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 4);
+  const Plan p = plan(B, T > 0 ? T : 1, D, vec ? (dtype == TB_F32 ? 4 : 8) : 1);
+  rc = check_grid("conv_fwd", p);
+  if (rc) return rc;
+  ConvArgs a{x, w, bias, state, nullptr, lengths, y, state_out, nullptr, nullptr, x_batch_stride, x_step_stride, B, T, D, p.run,
+             p.runs, act, w_f32};
+  by_shape(dtype, K, vec, FwdLaunch{a, dim3((unsigned)p.gx, (unsigned)p.gy), dim3(p.bx, p.by), static_cast<hipStream_t>(stream)});
+  TB_LAUNCH_CHECK("conv_fwd");
+  return TB_OK;
+}
+
+size_t tb_conv_bwd_workspace_bytes(int B, int T, int D, int K, int dtype) {
+  if (B < 1 || T < 1 || D < 1 || K < 1) return 256;
+  // the widest of the two layouts
+  const Plan p = plan(B, T, D, 1), q = plan(B, T, D, dtype == TB_F32 ? 4 : 8);
+  return tb_align_up((size_t)(p.gy > q.gy ? p.gy : q.gy) * (K + 1) * D * 4, 256);
+}
+
+int tb_conv_bwd(const void* dy, const void* x, long x_batch_stride, long x_step_stride, const void* w, const void* bias, int w_f32,
+                const void* state, const int* lengths, void* dx, void* dw, void* db, int B, int T, int D, int K, int act, int dtype,
+                void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_common("conv_bwd", B, T, D, K, act, dtype);
+  if (rc) return rc;
+  if (B < 1 || T < 1) return tb_set_error(TB_ERR_ARG, "conv_bwd: an empty batch has no gradients to form here");
+  if (!dy || !x || !w || !dx || !ws) return tb_set_error(TB_ERR_ARG, "conv_bwd: null pointer");
+  if (ws_bytes < tb_conv_bwd_workspace_bytes(B, T, D, K, dtype)) return tb_set_error(TB_ERR_WORKSPACE, "conv_bwd: workspace too small");
+  const void* ptrs[] = {x, dy, dx, state};
+  const bool vec = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 4);
+  const Plan p = plan(B, T, D, vec ? (dtype == TB_F32 ? 4 : 8) : 1);
+  rc = check_grid("conv_bwd", p);
+  if (rc) return rc;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  ConvArgs a{x, w, bias, state, dy, lengths, nullptr, nullptr, dx, static_cast<float*>(ws), x_batch_stride, x_step_stride, B, T, D,
+             p.run, p.runs, act, w_f32};
+  by_shape(dtype, K, vec, BwdLaunch{a, dim3((unsigned)p.gx, (unsigned)p.gy), dim3(p.bx, p.by), s});
+  TB_LAUNCH_CHECK("conv_bwd");
+  if (dw || db) {
+    const long cols = (long)(K + 1) * D;
+    const dim3 grid((unsigned)((cols + 63) / 64)), block(64, 16);
+    const float* slab = static_cast<const float*>(ws);
+    if (dtype == TB_F32) conv_finish<float><<<grid, block, 0, s>>>(slab, p.gy, K, D, dw, db, w_f32);
+    else if (dtype == TB_BF16) conv_finish<__bf16><<<grid, block, 0, s>>>(slab, p.gy, K, D, dw, db, w_f32);
+    else conv_finish<_Float16><<<grid, block, 0, s>>>(slab, p.gy, K, D, dw, db, w_f32);
+    TB_LAUNCH_CHECK("conv_finish");
+  }
+  return TB_OK;
+}
+
+int tb_conv_step(const void* x, long x_batch_stride, void* state, long state_batch_stride, const void* w, const void* bias, int w_f32,
+                 void* y, int B, int D, int K, int act, int dtype, void* stream) {
+  int rc = check_common("conv_step", B, 1, D, K, act, dtype);
+  if (rc) return rc;
+  if (B == 0) return TB_OK;
+  if (!x || !w || !y || (K > 1 && !state)) return tb_set_error(TB_ERR_ARG, "conv_step: null pointer");
+  const void* ptrs[] = {x, y, state};
+  const bool vec = can_vec(dtype, D, x_batch_stride, state_batch_stride, ptrs, 3);
+  ConvStepArgs a{x, w, bias, state, y, x_batch_stride, state_batch_stride, B, D, act, w_f32};
+  by_shape(dtype, K, vec, StepLaunch{a, static_cast<hipStream_t>(stream)});
+  TB_LAUNCH_CHECK("conv_step");
+  return TB_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,60 @@
+// Element types of the state space layer's operators (convolution, selective scan, linear with residual): fp32, bf16 and fp16
+// in memory, fp32 in registers.  A store rounds once, to nearest even.
+#pragma once
+#include "common.h"
+
+#define TB_F32 0
+#define TB_BF16 1
+#define TB_F16 2
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+static inline size_t tb_dtype_size(int dt) { return dt == TB_F32 ? 4 : 2; }
+static inline bool tb_dtype_ok(int dt) { return dt >= TB_F32 && dt <= TB_F16; }
+
+// N consecutive elements as one access where the address allows it (the caller knows), element by element otherwise
+template <typename T, int N>
+struct alignas(sizeof(T) * N) TbVec {
+  T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void tb_load_n(const T* p, float (&r)[N]) {
+  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;   // at most 16 bytes an access
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    const TbVec<T, W> t = *reinterpret_cast<const TbVec<T, W>*>(p + i);
+#pragma unroll
+    for (int j = 0; j < W; ++j) r[i + j] = (float)t.v[j];
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void tb_store_n(T* p, const float (&r)[N]) {
+  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    TbVec<T, W> t;
+#pragma unroll
+    for (int j = 0; j < W; ++j) t.v[j] = (T)r[i + j];
+    *reinterpret_cast<TbVec<T, W>*>(p + i) = t;
+  }
+}
+
+// A parameter that is kept either in the operator's element type or in fp32 (f32 != 0): read / written once per thread
+template <typename T>
+__device__ __forceinline__ float tb_load_par(const void* p, long i, int f32) {
+  return f32 ? static_cast<const float*>(p)[i] : (float)static_cast<const T*>(p)[i];
+}
+template <typename T>
+__device__ __forceinline__ void tb_store_par(void* p, long i, float v, int f32) {
+  if (f32) static_cast<float*>(p)[i] = v;
+  else static_cast<T*>(p)[i] = (T)v;
+}
+
+// activations: 0 none, 1 tanh, 2 sigmoid, 3 relu, 4 silu, 5 gelu (the error-function form)
+#define TB_ACT_SILU 4
+#define TB_ACT_LAST 5
+
+// 1 / (1 + e^-x) on the hardware exp and reciprocal (1 ulp each): e^-x = inf gives 0, e^-x = 0 gives 1
+__device__ __forceinline__ float tb_sig(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
+__device__ __forceinline__ float tb_silu(float x) { return x * tb_sig(x); }

@@ -1,0 +1,628 @@
+// Linear with bias, activation and residual: y = act(x W^T + b) + r, its gradients, fp32 / bf16 / fp16.
+//
+//   z = x W^T + b,  y = act(z) + r        dz = dy act'(z),  dx = dz W,  dW = dz^T x,  db = colsum(dz),  dr = dy
+//
+// One matrix kernel serves all three products: C[m][n] = sum_k P[m][k] Q[n][k] with k running along the rows of both operands,
+// which is what a matrix instruction's lanes want (16 neighbouring bytes each).  For dx and dW the operands are written once
+// with their axes exchanged (W, x and dz: 2 bytes an element moved against K or M operations on it); the kernel that forms
+// dz = dy act'(z) writes both orders and the column sums of db in its one pass.
+// 16-bit operands go through v_mfma_f32_16x16x32, fp32 ones through v_mfma_f32_16x16x4 (exact fp32 products: no splitting
+// into 16-bit parts, so infinities and the type's whole range pass).  Sums are fp32, z is kept in fp32 for the gradient (kept in 16 bits it
+// would add a second rounding to act'), and dz is rounded to the operands' type because it enters the matrix instructions.
+// Rows of 128 bytes of both operands are copied straight to LDS (16 bytes a lane), the next tile's while the present one is
+// multiplied; the 16-byte pieces of a row are exchanged by the row's low bits, so that the sixteen rows a fragment reads fall
+// on different banks.
+// Few rows (a batch of single tokens) are bound by reading W once: a kernel without LDS staging whose waves split K.
+#include "elem.h"
+
+namespace {
+
+typedef __attribute__((address_space(1))) const void gvoid;
+typedef __attribute__((address_space(3))) void lvoid;
+
+__device__ const f32x4 g_zeros[16] = {};     // what pieces behind the end of K are read from
+
+// tanh to a relative error of 2^-21: below 1/8 its series, where 1 - 2 / (1 + e^2x) cancels
+__device__ __forceinline__ float tanh_rel(float x) {
+  const float q = x * x;
+  const float p = x * (1.f + q * (-0.333333333f + q * (0.133333333f + q * (-0.0539682540f + q * 0.0218694885f))));
+  return fabsf(x) < 0.125f ? p : tb_tanh(x);
+}
+__device__ __forceinline__ float act_of(float z, int act) {
+  switch (act) {
+    case 1: return tanh_rel(z);
+    case 2: return tb_sig(z);
+    case 3: return z < 0.f ? 0.f : z;
+    case 4: return tb_silu(z);
+    case 5: return 0.5f * z * (1.f + erff(z * 0.70710678f));
+    default: return z;
+  }
+}
+__device__ __forceinline__ float act_grad(float z, int act) {
+  switch (act) {
+    case 1: { const float y = tanh_rel(z); return 1.f - y * y; }
+    case 2: { const float y = tb_sig(z); return y * (1.f - y); }
+    case 3: return z > 0.f ? 1.f : 0.f;
+    case 4: { const float y = tb_sig(z); return y * (1.f + z * (1.f - y)); }
+    case 5: return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+    default: return 1.f;
+  }
+}
+
+// 16 bytes of k for each of the sixteen rows of a fragment: lane l holds row l & 15, piece l >> 4 of four
+template <typename T>
+struct Mfma;
+template <>
+struct Mfma<__bf16> {
+  static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mfma<_Float16> {
+  static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct Mfma<float> {
+  // the four k of a lane's piece in four instructions: the order of k is free as long as both operands keep the same one
+  static __device__ __forceinline__ f32x4 mul(u32x4 a, u32x4 b, f32x4 c) {
+    const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+struct Epi {
+  const void *bias, *res;   // element type T, each nullable
+  void* y;                  // M x N dense
+  float* z;                 // M x N dense, nullable: the pre-activation
+  float* slab;              // split k: partial sums [split][M][N] instead of everything above
+  long ldr;
+  int act;
+};
+
+// four neighbouring columns n .. n+3 of row m
+template <typename T>
+__device__ __forceinline__ void finish4(const Epi& e, long M, int N, long m, int n, f32x4 v, bool four) {
+  if (m >= M || n >= N) return;
+  const long at = m * N + n;
+  float o[4] = {v[0], v[1], v[2], v[3]};
+  if (four) {
+    if (e.bias) {
+      float b[4];
+      tb_load_n(static_cast<const T*>(e.bias) + n, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += b[i];
+    }
+    if (e.z) tb_store_n(e.z + at, o);
+    if (e.act)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] = act_of(o[i], e.act);
+    if (e.res) {
+      float r[4];
+      tb_load_n(static_cast<const T*>(e.res) + m * e.ldr + n, r);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[i] += r[i];
+    }
+    tb_store_n(static_cast<T*>(e.y) + at, o);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (n + i >= N) break;
+      float w = o[i];
+      if (e.bias) w += (float)static_cast<const T*>(e.bias)[n + i];
+      if (e.z) e.z[at + i] = w;
+      if (e.act) w = act_of(w, e.act);
+      if (e.res) w += (float)static_cast<const T*>(e.res)[m * e.ldr + n + i];
+      static_cast<T*>(e.y)[at + i] = (T)w;
+    }
+  }
+}
+
+struct GemmArgs {
+  const void *P, *Q;        // P: M rows, Q: N rows; rows start on 16 bytes, K a multiple of 16 bytes
+  long ldp, ldq;
+  long M;
+  int N, K;
+  int tm, tn, splits, per;  // tiles; k tiles a split
+  int four;                 // rows of y, z, the residual and the bias allow four columns at once
+  Epi e;
+};
+
+// Tiles of the output in an order that keeps each of the eight dies on neighbouring tiles (consecutive workgroups go to
+// different dies, each with its own L2): die x takes the x-th eighth of the tiles, which run down eight rows of tiles at a time.
+__device__ __forceinline__ void tile_of(int id, int tm, int tn, int& im, int& in) {
+  const int n = tm * tn, q = n / 8, r = n % 8, x = id % 8, i = id / 8;
+  const int at = x < r ? x * (q + 1) + i : r * (q + 1) + (x - r) * q + i;
+  const int band = at / (8 * tn), rows = min(8, tm - band * 8), in_band = at - band * 8 * tn;
+  im = band * 8 + in_band % rows;
+  in = in_band / rows;
+}
+
+template <typename T, int BM, int BN, int WM, int WN>
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) gemm_nt(GemmArgs a) {
+  constexpr int WAVES = (BM / WM) * (BN / WN), CE = 16 / sizeof(T), BK = 8 * CE;
+  constexpr int MF = WM / 16, NF = WN / 16, LP = BM / 8 / WAVES, LQ = BN / 8 / WAVES;
+  __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * 128];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int im, in;
+  tile_of(blockIdx.x, a.tm, a.tn, im, in);
+  const long m0 = (long)im * BM;
+  const int n0 = in * BN;
+  const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
+  const int kt0 = blockIdx.y * a.per, kt1 = min(kt0 + a.per, (a.K + BK - 1) / BK);
+
+  // what this lane copies: row 8 i + lane / 8 of each of its pieces, and of that row's eight 16-byte pieces the one whose
+  // place in LDS is lane % 8
+  const int lr = lane >> 3, piece = ((lane & 7) ^ lr) * CE;
+  const T* pp[LP];
+  const T* qp[LQ];
+#pragma unroll
+  for (int i = 0; i < LP; ++i) {
+    long r = m0 + (wave * LP + i) * 8 + lr;
+    r = r < a.M ? r : a.M - 1;                  // rows behind the last: any row, never stored
+    pp[i] = static_cast<const T*>(a.P) + r * a.ldp + piece;
+  }
+#pragma unroll
+  for (int i = 0; i < LQ; ++i) {
+    int r = n0 + (wave * LQ + i) * 8 + lr;
+    r = r < a.N ? r : a.N - 1;
+    qp[i] = static_cast<const T*>(a.Q) + (long)r * a.ldq + piece;
+  }
+  auto copy = [&](int kt, int buf) {
+    const long k = (long)kt * BK;
+    if (k + BK <= a.K) {
+#pragma unroll
+      for (int i = 0; i < LP; ++i)
+        __builtin_amdgcn_global_load_lds((gvoid*)(pp[i] + k), (lvoid*)&lds[buf][(wave * LP + i) * 1024], 16, 0, 0);
+#pragma unroll
+      for (int i = 0; i < LQ; ++i)
+        __builtin_amdgcn_global_load_lds((gvoid*)(qp[i] + k), (lvoid*)&lds[buf][BM * 128 + (wave * LQ + i) * 1024], 16, 0, 0);
+    } else {       // the last tile: pieces behind K come from a row of zeros
+      const bool in_k = k + piece < a.K;
+      const uintptr_t zero = reinterpret_cast<uintptr_t>(g_zeros);
+#pragma unroll
+      for (int i = 0; i < LP; ++i)
+        __builtin_amdgcn_global_load_lds((gvoid*)(in_k ? reinterpret_cast<uintptr_t>(pp[i] + k) : zero),
+                                         (lvoid*)&lds[buf][(wave * LP + i) * 1024], 16, 0, 0);
+#pragma unroll
+      for (int i = 0; i < LQ; ++i)
+        __builtin_amdgcn_global_load_lds((gvoid*)(in_k ? reinterpret_cast<uintptr_t>(qp[i] + k) : zero),
+                                         (lvoid*)&lds[buf][BM * 128 + (wave * LQ + i) * 1024], 16, 0, 0);
+    }
+  };
+
+  f32x4 acc[MF][NF];
+#pragma unroll
+  for (int i = 0; i < MF; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+
+  if (kt0 < kt1) copy(kt0, 0);
+  __syncthreads();
+  for (int kt = kt0; kt < kt1; ++kt) {
+    const int buf = (kt - kt0) & 1;
+    if (kt + 1 < kt1) copy(kt + 1, buf ^ 1);
+    const char* sp = &lds[buf][(wm + (lane & 15)) * 128];
+    const char* sq = &lds[buf][BM * 128 + (wn + (lane & 15)) * 128];
+#pragma unroll
+    for (int kk = 0; kk < 2; ++kk) {
+      const int off = ((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 16;
+      u32x4 fp[MF], fq[NF];
+#pragma unroll
+      for (int j = 0; j < NF; ++j) fq[j] = *reinterpret_cast<const u32x4*>(sq + j * 2048 + off);
+#pragma unroll
+      for (int i = 0; i < MF; ++i) fp[i] = *reinterpret_cast<const u32x4*>(sp + i * 2048 + off);
+#pragma unroll
+      for (int i = 0; i < MF; ++i)
+#pragma unroll
+        for (int j = 0; j < NF; ++j) acc[i][j] = Mfma<T>::mul(fq[j], fp[i], acc[i][j]);
+    }
+    __syncthreads();
+  }
+  // a lane holds row lane & 15 and four neighbouring columns of each 16 x 16 piece (Q is the left operand)
+#pragma unroll
+  for (int i = 0; i < MF; ++i)
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {
+      const long m = m0 + wm + i * 16 + (lane & 15);
+      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
+      if (a.e.slab) {
+        if (m < a.M && n < a.N) {
+          float* s = a.e.slab + ((long)blockIdx.y * a.M + m) * a.N + n;
+          if (a.four) *reinterpret_cast<f32x4*>(s) = acc[i][j];
+          else
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              if (n + q < a.N) s[q] = acc[i][j][q];
+        }
+      } else {
+        finish4<T>(a.e, a.M, a.N, m, n, acc[i][j], a.four);
+      }
+    }
+}
+
+// the splits' sums, in their order, and the epilogue
+template <typename T>
+__global__ void __launch_bounds__(256) split_finish(Epi e, long M, int N, int splits, int four) {
+  const int nq = (N + 3) / 4;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= M * nq) return;
+  const long m = id / nq;
+  const int n = (int)(id % nq) * 4;
+  f32x4 s = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int k = 0; k < splits; ++k) {
+    const float* p = e.slab + ((long)k * M + m) * N + n;
+    if (four) s += *reinterpret_cast<const f32x4*>(p);
+    else
+      for (int q = 0; q < 4; ++q)
+        if (n + q < N) s[q] += p[q];
+  }
+  finish4<T>(e, M, N, m, n, s, four);
+}
+
+struct FewArgs {
+  const void *x, *W;
+  long ldx, ldw, M;
+  int N, K, vec, four;
+  Epi e;
+};
+
+template <typename T>
+__device__ __forceinline__ u32x4 load_piece(const T* row, long k, int K, bool vec, bool on) {
+  constexpr int CE = 16 / sizeof(T);
+  u32x4 r = (u32x4){0u, 0u, 0u, 0u};
+  if (vec) {
+    if (on && k < K) r = *reinterpret_cast<const u32x4*>(row + k);
+  } else {
+    TbVec<T, CE> v;
+#pragma unroll
+    for (int i = 0; i < CE; ++i) v.v[i] = on && k + i < K ? row[k + i] : (T)0.f;
+    r = __builtin_bit_cast(u32x4, v);
+  }
+  return r;
+}
+
+// up to 16 MT rows: a block owns sixteen columns, its waves take turns along K and are summed at the end
+template <typename T, int MT, int WAVES>
+__global__ void __launch_bounds__(WAVES * 64) gemm_few(FewArgs a) {
+  constexpr int CE = 16 / sizeof(T), U = 4, STEP = 4 * CE * U;
+  __shared__ f32x4 red[WAVES][MT][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, piece = (lane >> 4) * CE;
+  const int n0 = blockIdx.x * 16;
+  const int wr = min(n0 + row, a.N - 1);
+  const T* W = static_cast<const T*>(a.W) + (long)wr * a.ldw;
+  const T* x[MT];
+  bool on[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) {
+    const long m = i * 16 + row;
+    on[i] = m < a.M;
+    x[i] = static_cast<const T*>(a.x) + (on[i] ? m : 0) * a.ldx;
+  }
+  f32x4 acc[MT];
+#pragma unroll
+  for (int i = 0; i < MT; ++i) acc[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (long k0 = (long)wave * STEP; k0 < a.K; k0 += WAVES * STEP) {
+    u32x4 w[U], v[MT][U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) w[u] = load_piece(W, k0 + u * 4 * CE + piece, a.K, a.vec, true);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int u = 0; u < U; ++u) v[i][u] = load_piece(x[i], k0 + u * 4 * CE + piece, a.K, a.vec, on[i]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < MT; ++i) acc[i] = Mfma<T>::mul(w[u], v[i][u], acc[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < MT; ++i) red[wave][i][lane] = acc[i];
+  __syncthreads();
+  if (wave < MT) {
+    f32x4 s = red[0][wave][lane];
+#pragma unroll
+    for (int k = 1; k < WAVES; ++k) s += red[k][wave][lane];
+    finish4<T>(a.e, a.M, a.N, wave * 16 + row, n0 + (lane >> 4) * 4, s, a.four);
+  }
+}
+
+// rows copied with their k padded by zeros to whole 16-byte pieces (rows that do not start on 16 bytes)
+template <typename T>
+__global__ void __launch_bounds__(256) pack_rows(const T* src, long ld, long R, int C, T* dst, int Cp) {
+  constexpr int CE = 16 / sizeof(T);
+  const int per = Cp / CE;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= R * per) return;
+  const long r = id / per;
+  const int c = (int)(id % per) * CE;
+  TbVec<T, CE> v;
+#pragma unroll
+  for (int i = 0; i < CE; ++i) v.v[i] = c + i < C ? src[r * ld + c + i] : (T)0.f;
+  *reinterpret_cast<TbVec<T, CE>*>(dst + r * Cp + c) = v;
+}
+
+// dst[c][r] = src[r][c]; dst's rows are padded by zeros to Rp
+template <typename T>
+__global__ void __launch_bounds__(256) transpose(const T* src, long ld, long R, int C, T* dst, long Rp) {
+  __shared__ float t[64][65];
+  const long r0 = (long)blockIdx.x * 64;
+  const int c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const long r = r0 + y + i * 4;
+    t[y + i * 4][x] = r < R && c0 + x < C ? (float)src[r * ld + c0 + x] : 0.f;
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int c = c0 + y + i * 4;
+    if (c < C && r0 + x < Rp) dst[c * Rp + r0 + x] = (T)t[x][y + i * 4];
+  }
+}
+
+// dz = dy act'(z) in both orders, each nullable, and the column sums of each 64 rows (fp32, before dz is rounded)
+template <typename T>
+__global__ void __launch_bounds__(256) form_dz(const T* dy, long ldy, const float* z, int act, long M, int N, T* dz, int Np, T* dzT, long Mp,
+                                               float* part) {
+  __shared__ float t[64][65];
+  const long r0 = (long)blockIdx.x * 64;
+  const int c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+#pragma unroll 4
+  for (int i = 0; i < 16; ++i) {
+    const long r = r0 + y + i * 4;
+    float v = 0.f;
+    if (r < M && c0 + x < N) {
+      v = (float)dy[r * ldy + c0 + x];
+      if (z) v *= act_grad(z[r * N + c0 + x], act);
+    }
+    if (dz && r < M && c0 + x < Np) dz[r * Np + c0 + x] = (T)v;
+    t[y + i * 4][x] = v;
+  }
+  __syncthreads();
+  if (dzT) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      const int c = c0 + y + i * 4;
+      if (c < N && r0 + x < Mp) dzT[c * Mp + r0 + x] = (T)t[x][y + i * 4];
+    }
+  }
+  if (part && y == 0 && c0 + x < N) {
+    float s = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < 64; ++i) s += t[i][x];
+    part[(long)blockIdx.x * N + c0 + x] = s;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024) colsum_finish(const float* part, long rows, int N, T* db) {
+  __shared__ float red[16][65];
+  const int x = threadIdx.x & 63, y = threadIdx.x >> 6, c = blockIdx.x * 64 + x;
+  float s = 0.f;
+  if (c < N) {
+    const long per = (rows + 15) / 16, r1 = min(rows, (y + 1) * per);
+#pragma unroll 4
+    for (long r = y * per; r < r1; ++r) s += part[r * N + c];
+  }
+  red[y][x] = s;
+  __syncthreads();
+  if (y == 0 && c < N) {
+    s = 0.f;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s += red[j][x];
+    db[c] = (T)s;
+  }
+}
+
+constexpr int FEW = 32;     // rows up to which the kernel for few rows is taken
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+struct Plan {
+  bool big;
+  int tm, tn, splits, per;
+};
+// 256 x 256 tiles where they fill the chip, 128 x 128 otherwise (two blocks a unit); k is split where even those leave units
+// idle, into parts of eight k tiles at least.
+Plan plan(long M, int N, long K, int esize) {
+  Plan p;
+  const long cus = tb_num_cus(), kt = (K * esize + 127) / 128;
+  const long big = ((M + 255) / 256) * ((N + 255) / 256);
+  p.big = big >= cus;
+  const int b = p.big ? 256 : 128;
+  p.tm = (int)((M + b - 1) / b);
+  p.tn = (N + b - 1) / b;
+  const long tiles = (long)p.tm * p.tn;
+  long s = 1;
+  if (!p.big && tiles < 2 * cus) {
+    s = 2 * cus / tiles;
+    if (s > kt / 8) s = kt / 8;
+    if (s > 64) s = 64;
+    if (s < 1) s = 1;
+  }
+  p.per = (int)((kt + s - 1) / s);
+  p.splits = (int)((kt + p.per - 1) / p.per);
+  return p;
+}
+size_t slab_bytes(long M, int N, long K, int esize) {
+  const Plan p = plan(M, N, K, esize);
+  return p.splits > 1 ? tb_align_up((size_t)p.splits * M * N * 4, 256) : 0;
+}
+
+template <typename T>
+int launch_gemm(const T* P, long ldp, const T* Q, long ldq, long M, int N, long K, Epi e, float* slab, hipStream_t s) {
+  const Plan p = plan(M, N, K, sizeof(T));
+  constexpr int CE = 16 / sizeof(T);
+  GemmArgs a{P, Q, ldp, ldq, M, N, (int)K, p.tm, p.tn, p.splits, p.per, 0, e};
+  a.four = N % 4 == 0 && aligned(e.y) && aligned(e.z) && aligned(e.bias) && aligned(e.res) && (!e.res || e.ldr % CE == 0);
+  a.e.slab = p.splits > 1 ? slab : nullptr;
+  const dim3 grid(p.tm * p.tn, p.splits);
+  if (p.big) gemm_nt<T, 256, 256, 128, 64><<<grid, 512, 0, s>>>(a);
+  else gemm_nt<T, 128, 128, 64, 64><<<grid, 256, 0, s>>>(a);
+  TB_LAUNCH_CHECK("linres gemm");
+  if (p.splits > 1) {
+    split_finish<T><<<(unsigned)((M * ((N + 3) / 4) + 255) / 256), 256, 0, s>>>(a.e, M, N, p.splits, a.four);
+    TB_LAUNCH_CHECK("linres split_finish");
+  }
+  return TB_OK;
+}
+
+// an operand the matrix kernel can copy: rows on 16 bytes, whole 16-byte pieces of k
+template <typename T>
+bool direct(const void* p, long ld, long K) { return aligned(p) && ld % (16 / (long)sizeof(T)) == 0 && K % (16 / (long)sizeof(T)) == 0; }
+
+long up(long x, int esize) { return (x + 16 / esize - 1) / (16 / esize) * (16 / esize); }
+
+template <typename T>
+int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, int N, char* ws, hipStream_t s) {
+  constexpr int CE = 16 / sizeof(T);
+  if (M <= FEW) {
+    FewArgs a{x, W, ldx, ldw, M, N, K, 0, 0, e};
+    a.vec = direct<T>(x, ldx, K) && direct<T>(W, ldw, K);
+    a.four = N % 4 == 0 && aligned(e.y) && aligned(e.z) && aligned(e.bias) && aligned(e.res) && (!e.res || e.ldr % CE == 0);
+    const unsigned grid = (N + 15) / 16;
+    if (M <= 16) gemm_few<T, 1, 4><<<grid, 256, 0, s>>>(a);
+    else gemm_few<T, 2, 4><<<grid, 256, 0, s>>>(a);
+    TB_LAUNCH_CHECK("linres gemm_few");
+    return TB_OK;
+  }
+  const long Kp = up(K, sizeof(T));
+  const bool dxr = direct<T>(x, ldx, K), dwr = direct<T>(W, ldw, K);
+  char* p = ws;
+  if (!dxr) {
+    pack_rows<T><<<(unsigned)((M * (Kp / CE) + 255) / 256), 256, 0, s>>>(x, ldx, M, K, reinterpret_cast<T*>(p), (int)Kp);
+    TB_LAUNCH_CHECK("linres pack");
+    x = reinterpret_cast<T*>(p);
+    ldx = Kp;
+  }
+  p += tb_align_up((size_t)M * Kp * sizeof(T), 256);
+  if (!dwr) {
+    pack_rows<T><<<(unsigned)(((long)N * (Kp / CE) + 255) / 256), 256, 0, s>>>(W, ldw, N, K, reinterpret_cast<T*>(p), (int)Kp);
+    TB_LAUNCH_CHECK("linres pack");
+    W = reinterpret_cast<T*>(p);
+    ldw = Kp;
+  }
+  p += tb_align_up((size_t)N * Kp * sizeof(T), 256);
+  return launch_gemm<T>(x, ldx, W, ldw, M, N, Kp, e, reinterpret_cast<float*>(p), s);
+}
+
+struct BwdSizes {
+  size_t dz, dzT, WT, xT, part, slab, total;
+  long Np, Mp;
+};
+BwdSizes bwd_sizes(long M, int K, int N, int es) {
+  BwdSizes b;
+  b.Np = up(N, es);
+  b.Mp = up(M, es);
+  b.dz = tb_align_up((size_t)M * b.Np * es, 256);
+  b.dzT = tb_align_up((size_t)N * b.Mp * es, 256);
+  b.WT = tb_align_up((size_t)K * b.Np * es, 256);
+  b.xT = tb_align_up((size_t)K * b.Mp * es, 256);
+  b.part = tb_align_up((size_t)((M + 63) / 64) * N * 4, 256);
+  const size_t s1 = slab_bytes(M, K, b.Np, es), s2 = slab_bytes(N, K, b.Mp, es);
+  b.slab = s1 > s2 ? s1 : s2;
+  b.total = b.dz + b.dzT + b.WT + b.xT + b.part + b.slab + 256;
+  return b;
+}
+
+template <typename T>
+int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, const float* z, int act, T* dx, T* dW, T* db, long M, int K,
+             int N, char* ws, hipStream_t s) {
+  const BwdSizes b = bwd_sizes(M, K, N, sizeof(T));
+  T* dz = reinterpret_cast<T*>(ws);
+  T* dzT = reinterpret_cast<T*>(ws + b.dz);
+  T* WT = reinterpret_cast<T*>(ws + b.dz + b.dzT);
+  T* xT = reinterpret_cast<T*>(ws + b.dz + b.dzT + b.WT);
+  float* part = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT);
+  float* slab = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT + b.part);
+  const bool as_is = !z && direct<T>(dy, ldy, N);      // dz = dy, and its rows can be copied as they are
+  const T* dzr = as_is ? dy : dz;
+  const long ldz = as_is ? ldy : b.Np;
+  if (!as_is || dW || db) {
+    form_dz<T><<<dim3((unsigned)((M + 63) / 64), (unsigned)((b.Np + 63) / 64)), 256, 0, s>>>(
+        dy, ldy, z, act, M, N, as_is || !dx ? nullptr : dz, (int)b.Np, dW ? dzT : nullptr, b.Mp, db ? part : nullptr);
+    TB_LAUNCH_CHECK("linres form_dz");
+  }
+  if (db) {
+    colsum_finish<T><<<(unsigned)((N + 63) / 64), 1024, 0, s>>>(part, (M + 63) / 64, N, db);
+    TB_LAUNCH_CHECK("linres colsum_finish");
+  }
+  Epi e{};
+  if (dx) {
+    transpose<T><<<dim3((unsigned)((b.Np + 63) / 64), (unsigned)((K + 63) / 64)), 256, 0, s>>>(W, ldw, N, K, WT, b.Np);
+    TB_LAUNCH_CHECK("linres transpose");
+    e.y = dx;
+    const int rc = launch_gemm<T>(dzr, ldz, WT, b.Np, M, K, b.Np, e, slab, s);
+    if (rc) return rc;
+  }
+  if (dW) {
+    transpose<T><<<dim3((unsigned)((b.Mp + 63) / 64), (unsigned)((K + 63) / 64)), 256, 0, s>>>(x, ldx, M, K, xT, b.Mp);
+    TB_LAUNCH_CHECK("linres transpose");
+    e.y = dW;
+    const int rc = launch_gemm<T>(dzT, b.Mp, xT, b.Mp, N, K, b.Mp, e, slab, s);
+    if (rc) return rc;
+  }
+  return TB_OK;
+}
+
+int check_common(const char* what, long M, int K, int N, int act, int dtype) {
+  // the tile counts and the transposes' grids are 32 and 16 bits wide
+  if (M < 0 || K < 1 || N < 1 || K > 4000000 || N > 4000000 || M > (1L << 31)) return tb_set_error(TB_ERR_ARG, "%s: bad sizes M=%ld K=%d N=%d", what, M, K, N);
+  if (act < 0 || act > TB_ACT_LAST) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: activation %d is not supported", what, act);
+  if (!tb_dtype_ok(dtype)) return tb_set_error(TB_ERR_ARG, "%s: bad element type %d", what, dtype);
+  return TB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tb_linres_workspace_bytes(long M, int K, int N, int dtype, int backward) {
+  if (M < 1 || K < 1 || N < 1 || !tb_dtype_ok(dtype)) return 256;
+  const int es = (int)tb_dtype_size(dtype);
+  if (backward) return bwd_sizes(M, K, N, es).total;
+  if (M <= FEW) return 256;
+  const long Kp = up(K, es);
+  return tb_align_up((size_t)M * Kp * es, 256) + tb_align_up((size_t)N * Kp * es, 256) + slab_bytes(M, N, Kp, es) + 256;
+}
+
+int tb_linres_fwd(const void* x, long x_row_stride, const void* W, long w_row_stride, const void* b, const void* residual,
+                  long residual_row_stride, void* y, float* z, long M, int K, int N, int act, int dtype, void* ws, size_t ws_bytes,
+                  void* stream) {
+  int rc = check_common("linres_fwd", M, K, N, act, dtype);
+  if (rc) return rc;
+  if (M == 0) return TB_OK;
+  if (!x || !W || !y || !ws) return tb_set_error(TB_ERR_ARG, "linres_fwd: null pointer");
+  if (ws_bytes < tb_linres_workspace_bytes(M, K, N, dtype, 0)) return tb_set_error(TB_ERR_WORKSPACE, "linres_fwd: workspace too small");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* w = static_cast<char*>(ws);
+  Epi e{b, residual, y, z, nullptr, residual_row_stride, act};
+  if (dtype == TB_F32) return forward<float>((const float*)x, x_row_stride, (const float*)W, w_row_stride, e, M, K, N, w, s);
+  if (dtype == TB_BF16) return forward<__bf16>((const __bf16*)x, x_row_stride, (const __bf16*)W, w_row_stride, e, M, K, N, w, s);
+  return forward<_Float16>((const _Float16*)x, x_row_stride, (const _Float16*)W, w_row_stride, e, M, K, N, w, s);
+}
+
+int tb_linres_bwd(const void* dy, long dy_row_stride, const void* x, long x_row_stride, const void* W, long w_row_stride, const float* z,
+                  int act, void* dx, void* dW, void* db, long M, int K, int N, int dtype, void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_common("linres_bwd", M, K, N, act, dtype);
+  if (rc) return rc;
+  if (M < 1) return tb_set_error(TB_ERR_ARG, "linres_bwd: no rows have no gradients to form here");
+  if (!dy || (dx && !W) || (dW && !x) || (act && !z) || !ws) return tb_set_error(TB_ERR_ARG, "linres_bwd: null pointer");
+  if (ws_bytes < tb_linres_workspace_bytes(M, K, N, dtype, 1)) return tb_set_error(TB_ERR_WORKSPACE, "linres_bwd: workspace too small");
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  char* w = static_cast<char*>(ws);
+  const float* zz = act ? z : nullptr;
+#define TB_BWD(T) \
+  return backward<T>((const T*)dy, dy_row_stride, (const T*)x, x_row_stride, (const T*)W, w_row_stride, zz, act, (T*)dx, (T*)dW, (T*)db, M, K, N, w, s)
+  if (dtype == TB_F32) TB_BWD(float);
+  if (dtype == TB_BF16) TB_BWD(__bf16);
+  TB_BWD(_Float16);
+#undef TB_BWD
+}
+
+}  // extern "C"

@@ -1,0 +1,818 @@
+// Selective state space scan over (B, T, D) with N states a channel: prompts, gradients, one step.
+//
+//   delta = softplus(dt + bias)   (or dt + bias)          per step and channel
+//   h_t   = exp(delta A) h_{t-1} + delta u B_t            per state; A (D, N), B_t / C_t (N) shared by the channels of a group
+//   y     = C_t . h_t + D u,   out = y silu(z)
+// Backward, with dy = dout silu(z):
+//   g_t = C_t dy_t + a_{t+1} g_{t+1},  q = g_t a_t h_{t-1}
+//   ddelta = sum_n q A + u sum_n g B,  du = delta sum_n g B + D dy,  dA = sum q delta,  dB_t = sum_c g delta u,
+//   dC_t = sum_c dy h,  dD = sum dy u,  dz = dout y silu'(z),  ddt = ddelta sigmoid(dt + bias)
+//
+// Bound by arithmetic: an exponential (a quarter of the vector rate) and four other operations a state and step forward, two
+// exponentials and about fourteen backward, against two bytes an element and tensor.  Layout: a lane owns one channel and S = N/4 of
+// its states, four neighbouring lanes a channel, so that the sum over the states is two quad permutes and a block of four
+// waves owns 64 neighbouring channels (whole lines of every tensor).  Steps go in tiles: a tile's rows are fetched into
+// registers one tile ahead, what does not depend on the state (softplus, the gate's derivative) is computed once per element
+// by all lanes and left in LDS in fp32, then each wave walks the tile's steps with its states in registers.
+// Where the batch has too few channel blocks for the chip, the steps are cut into chunks: a first pass finds each chunk's own
+// end state from zero and the sum of its delta, a small kernel chains them (exp(A sum delta) is the chunk's decay), and the
+// main pass starts every chunk from its true state.
+// States, sums and gradients of parameters are fp32; every output is rounded once.  No atomics: partial sums are added in a
+// fixed order.
+#include "elem.h"
+
+namespace {
+
+constexpr int CB = 64;          // channels a block
+constexpr int NMAX = 64;
+constexpr float LOG2E = 1.4426950408889634f;
+
+// steps a tile of the backward pass: the states of a tile stay in registers, TT * S = 128 of them at most
+template <int S>
+struct Tile {
+  static constexpr int BWD = S <= 4 ? 32 : S == 8 ? 16 : 8;
+};
+int bwd_tile(int S) { return S <= 4 ? 32 : S == 8 ? 16 : 8; }
+
+struct ScanArgs {
+  const void *u, *dt, *z, *Bm, *Cm, *dout;
+  const float *A, *Dp, *bias, *h0, *dhT;
+  const int* lengths;
+  void *out, *du, *ddt, *dz;
+  float *hT, *dh0;
+  float* ck;               // states at the start of every backward tile: [B][tiles][D][4 S]
+  float* cstate;           // chunks: [B][chunks][D][4 S]
+  float* csum;             // chunks: [B][chunks][D]
+  float* bc;               // backward: [B][G][cblk][T][2][4 S] sums over a block's channels of dB and dC
+  float* par;              // backward: [B][chunks][D][4 S + 2] sums over a chunk's steps of dA, dD, dbias
+  long sub, sut, sdb, sdt, szb, szt, sob, sot, sBb, sBt, sBg, sCb, sCt, sCg;
+  int B, T, D, N, G, Dg;   // Dg channels a group
+  int cblk;                // blocks of 64 channels a group
+  int chunk, chunks;       // steps a chunk (a multiple of 32), chunks
+  int ckt, cktiles;        // steps between kept states (0: none)
+  int softplus, vec;
+};
+
+// log(1 + e^x).  With w = 1 + e rounded, log(w) e / (w - 1) repairs what the rounding of w lost (w - 1 is exact);
+// above 20 the result is x to fp32.
+__device__ __forceinline__ float softplus(float x) {
+  const float e = __expf(x), w = 1.f + e, m = w - 1.f;
+  const float l = __logf(w) * e * __builtin_amdgcn_rcpf(m);
+  return x > 20.f ? x : m > 0.f ? l : e;
+}
+
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+  v += dpp<0xB1>(v);       // lanes 1 0 3 2
+  return v + dpp<0x4E>(v); // lanes 2 3 0 1
+}
+
+// EPT neighbouring channels of a row; channels behind the group's last and rows that are off read as 0
+template <typename T, int EPT>
+__device__ __forceinline__ void fetch(const void* base, long off, int c0, int Dg, bool vec, bool on, float (&r)[EPT]) {
+  const T* p = static_cast<const T*>(base) + off;
+  if (on && vec && c0 + EPT <= Dg) {
+    tb_load_n(p + c0, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) r[i] = on && c0 + i < Dg ? (float)p[c0 + i] : 0.f;
+  }
+}
+template <typename T, int EPT>
+__device__ __forceinline__ void put(void* base, long off, int c0, int Dg, bool vec, const float (&r)[EPT]) {
+  T* p = static_cast<T*>(base) + off;
+  if (vec && c0 + EPT <= Dg) {
+    tb_store_n(p + c0, r);
+  } else {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i)
+      if (c0 + i < Dg) p[c0 + i] = (T)r[i];
+  }
+}
+
+struct Where {
+  int b, g, cb, chunk, c0, d0, len;   // c0: the block's first channel of its group, d0: of all
+};
+__device__ __forceinline__ Where where(const ScanArgs& a, int chunks) {
+  Where w;
+  int id = blockIdx.x;
+  w.cb = id % a.cblk; id /= a.cblk;
+  w.g = id % a.G; id /= a.G;
+  w.chunk = id % chunks;
+  w.b = id / chunks;
+  w.c0 = w.cb * CB;
+  w.d0 = w.g * a.Dg + w.c0;
+  w.len = a.lengths ? min(max(a.lengths[w.b], 0), a.T) : a.T;
+  return w;
+}
+
+// S states of channel d: [d][N] of the caller (count: N), zero behind N
+template <int S>
+__device__ __forceinline__ void load_state(const float* p, long row, int n0, int N, bool on, float (&h)[S]) {
+#pragma unroll
+  for (int s = 0; s < S; ++s) h[s] = on && p && n0 + s < N ? p[row * N + n0 + s] : 0.f;
+}
+template <int S>
+__device__ __forceinline__ void store_state(float* p, long row, int n0, int N, bool on, const float (&h)[S]) {
+#pragma unroll
+  for (int s = 0; s < S; ++s)
+    if (on && n0 + s < N) p[row * N + n0 + s] = h[s];
+}
+// S floats of a row of 4 S
+template <int S>
+__device__ __forceinline__ void load_row(const float* p, float (&v)[S]) { tb_load_n(p, v); }
+template <int S>
+__device__ __forceinline__ void store_row(float* p, const float (&v)[S]) { tb_store_n(p, v); }
+
+// rows of B or C of a tile into LDS as fp32, [TT][4 S], zero behind N and where the step is off
+template <typename T, int S, int TT>
+__device__ __forceinline__ void stage_bc(const void* base, long off, long st, int t0, int t1, int N, float* lds) {
+  constexpr int NP = 4 * S;
+  for (int i = threadIdx.x; i < TT * NP; i += 256) {
+    const int t = i / NP, n = i % NP;
+    lds[i] = t0 + t < t1 && n < N ? (float)static_cast<const T*>(base)[off + (long)(t0 + t) * st + n] : 0.f;
+  }
+}
+
+// forward.  STATE: only the chunk's end state from zero and its sum of delta (first pass over chunks).
+template <typename T, int S, bool STATE>
+__global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
+  constexpr int TT = 32, EPT = 8, NP = 4 * S;
+  __shared__ float sD[TT][CB][2];            // delta, delta u
+  __shared__ float sB[TT * NP], sC[STATE ? 1 : TT * NP];
+  __shared__ float sY[STATE ? 1 : TT][CB];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Where w = where(a, STATE ? a.chunks - 1 : a.chunks);
+  // the coop part: one step, eight channels a thread
+  const int ct = tid / (CB / EPT), cc = (tid % (CB / EPT)) * EPT;
+  // the recurrence: channel rc of the block, states n0 .. n0 + S
+  const int rc = wave * 16 + (lane >> 2), n0 = (lane & 3) * S;
+  const bool ron = w.c0 + rc < a.Dg;
+  const long rd = w.d0 + rc;
+  const int ts = w.chunk * a.chunk, te = min(ts + a.chunk, a.T);
+  const int tv = min(te, w.len);              // steps that count end here
+
+  float A2[S], h[S];
+  load_state<S>(a.A, rd, n0, a.N, ron, A2);
+#pragma unroll
+  for (int s = 0; s < S; ++s) A2[s] *= LOG2E;
+  if (STATE) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) h[s] = 0.f;
+  } else if (a.chunks > 1) {
+    if (ron) load_row<S>(a.cstate + (((long)w.b * a.chunks + w.chunk) * a.D + rd) * NP + n0, h);
+    else
+#pragma unroll
+      for (int s = 0; s < S; ++s) h[s] = 0.f;
+  } else {
+    load_state<S>(a.h0, (long)w.b * a.D + rd, n0, a.N, ron, h);
+  }
+  float bias[EPT], Dp[EPT];
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) {
+    const bool on = w.c0 + cc + i < a.Dg;
+    bias[i] = on && a.bias ? a.bias[w.d0 + cc + i] : 0.f;
+    Dp[i] = !STATE && on && a.Dp ? a.Dp[w.d0 + cc + i] : 0.f;
+  }
+  const long uo = (long)w.b * a.sub + (long)w.g * a.Dg, dof = (long)w.b * a.sdb + (long)w.g * a.Dg,
+             zo = (long)w.b * a.szb + (long)w.g * a.Dg, oo = (long)w.b * a.T * a.D + (long)w.g * a.Dg;
+  const int ch = w.c0 + cc;
+  float sum = 0.f;
+
+  for (int t0 = ts; t0 < te; t0 += TT) {
+    const int t = t0 + ct;
+    const bool on = t < tv;
+    float u[EPT], dl[EPT], z[EPT];
+    fetch<T, EPT>(a.u, uo + (long)t * a.sut, ch, a.Dg, a.vec, on, u);
+    fetch<T, EPT>(a.dt, dof + (long)t * a.sdt, ch, a.Dg, a.vec, on, dl);
+    if (!STATE && a.z) fetch<T, EPT>(a.z, zo + (long)t * a.szt, ch, a.Dg, a.vec, on, z);
+    stage_bc<T, S, TT>(a.Bm, (long)w.b * a.sBb + (long)w.g * a.sBg, a.sBt, t0, tv, a.N, sB);
+    if (!STATE) stage_bc<T, S, TT>(a.Cm, (long)w.b * a.sCb + (long)w.g * a.sCg, a.sCt, t0, tv, a.N, sC);
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) {
+      float d = dl[i] + bias[i];
+      if (a.softplus) d = softplus(d);
+      d = on && ch + i < a.Dg ? d : 0.f;       // a step that does not count leaves the state as it is
+      sD[ct][cc + i][0] = d;
+      sD[ct][cc + i][1] = d * u[i];
+    }
+    __syncthreads();
+    if (!STATE && a.ckt && ron) store_row<S>(a.ck + (((long)w.b * a.cktiles + t0 / a.ckt) * a.D + rd) * NP + n0, h);
+#pragma unroll 4
+    for (int k = 0; k < TT; ++k) {
+      if (!STATE && Tile<S>::BWD < TT) {          // a backward tile is shorter than this one: its start lies inside
+        if (k && a.ckt && k % Tile<S>::BWD == 0 && ron && t0 + k < a.T)
+          store_row<S>(a.ck + (((long)w.b * a.cktiles + (t0 + k) / a.ckt) * a.D + rd) * NP + n0, h);
+      }
+      const float d = sD[k][rc][0], x = sD[k][rc][1];
+      float bv[S], cv[S], y = 0.f;
+      load_row<S>(sB + k * NP + n0, bv);
+      if (!STATE) load_row<S>(sC + k * NP + n0, cv);
+#pragma unroll
+      for (int s = 0; s < S; ++s) {
+        const float e = __builtin_amdgcn_exp2f(d * A2[s]);
+        h[s] = fmaf(e, h[s], x * bv[s]);
+        if (!STATE) y = fmaf(h[s], cv[s], y);
+      }
+      if (STATE) sum += d;
+      else {
+        y = quad_sum(y);
+        if ((lane & 3) == 0) sY[k][rc] = y;
+      }
+    }
+    __syncthreads();
+    if (!STATE && t < te) {
+      float o[EPT];
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) {
+        float y = fmaf(Dp[i], u[i], sY[ct][cc + i]);
+        if (a.z) y *= tb_silu(z[i]);
+        o[i] = on ? y : 0.f;
+      }
+      put<T, EPT>(a.out, oo + (long)t * a.D, ch, a.Dg, a.vec, o);
+    }
+  }
+  if (STATE) {
+    const long row = ((long)w.b * a.chunks + w.chunk) * a.D + rd;
+    if (ron) store_row<S>(a.cstate + row * NP + n0, h);
+    if (ron && (lane & 3) == 0) a.csum[row] = sum;
+  } else if (a.hT && w.chunk == a.chunks - 1) {
+    store_state<S>(a.hT, (long)w.b * a.D + rd, n0, a.N, ron, h);
+  }
+}
+
+// chunks' own end states -> their start states (forward: from h0 on; REV: from the last chunk's dhT back)
+template <int S, bool REV>
+__global__ void __launch_bounds__(256) scan_chain(ScanArgs a) {
+  constexpr int NP = 4 * S;
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  if (id >= (long)a.B * a.D * NP) return;
+  const int n = (int)(id % NP);
+  const long d = id / NP % a.D, b = id / NP / a.D;
+  const float A2 = n < a.N ? a.A[d * a.N + n] * LOG2E : 0.f;
+  const float* first = REV ? a.dhT : a.h0;
+  float h = first && n < a.N ? first[(b * a.D + d) * a.N + n] : 0.f;
+  const int last = a.chunks - 1;
+  for (int i = 0; i < last; ++i) {
+    const int c = REV ? last - i : i;
+    const long row = (b * a.chunks + c) * a.D + d;
+    const float own = a.cstate[row * NP + n], s = a.csum[row];
+    a.cstate[row * NP + n] = h;
+    h = fmaf(__builtin_amdgcn_exp2f(A2 * s), h, own);
+  }
+  a.cstate[((b * a.chunks + (REV ? 0 : last)) * a.D + d) * NP + n] = h;
+}
+
+// v[0..2S) of the wave's sixteen channels (lane bits 2..5) summed: halves are exchanged so that each step adds what is left,
+// and the lanes with bits 2 and 3 clear end with S/2 sums each (S = 1: one), of v[0..S) in the lower half of the wave and of
+// v[S..2S) in the upper; bit 4 says which half of the S.
+template <int S>
+__device__ __forceinline__ void channel_sum(float (&v)[2 * S]) {
+#pragma unroll
+  for (int i = 0; i < S; ++i) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v[i]), __float_as_uint(v[i + S]), false, false);
+    v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  constexpr int H = S > 1 ? S / 2 : 1;
+#pragma unroll
+  for (int i = 0; i < H; ++i) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v[i]), __float_as_uint(v[S > 1 ? i + H : i]), false, false);
+    v[i] = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+#pragma unroll
+  for (int i = 0; i < H; ++i) {
+    v[i] += dpp<0x128>(v[i]);     // rotate the row of sixteen by eight
+    v[i] += dpp<0x124>(v[i]);     // and by four
+  }
+}
+
+// what a lane needs of a step: delta, delta u, dy, and its states' B and C
+template <int S>
+struct Row {
+  float d, x, y, b[S], c[S];
+  __device__ __forceinline__ void load(const float* dx, float dy, const float* B, const float* C) {
+    d = dx[0];
+    x = dx[1];
+    y = dy;
+    load_row<S>(B, b);
+    load_row<S>(C, c);
+  }
+};
+
+// backward.  STATE: only g in front of the chunk's first step from zero behind its last, and its sum of delta.
+template <typename T, int S, bool STATE>
+__global__ void __launch_bounds__(256, 2) scan_bwd(ScanArgs a) {
+  constexpr int TT = Tile<S>::BWD, EPT = TT / 4, NP = 4 * S;
+  __shared__ float sD[TT][CB][2], sG[TT][CB];           // delta, delta u; dy
+  __shared__ float sB[STATE ? 1 : TT * NP], sC[TT * NP];
+  __shared__ float sY[STATE ? 1 : TT][CB], sGB[STATE ? 1 : TT][CB], sGA[STATE ? 1 : TT][CB];
+  __shared__ float sP[STATE ? 1 : 4][STATE ? 1 : TT][2 * NP];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  Where w = where(a, STATE ? a.chunks - 1 : a.chunks);
+  if (STATE) ++w.chunk;
+  const int ct = tid / (CB / EPT), cc = (tid % (CB / EPT)) * EPT;
+  const int rc = wave * 16 + (lane >> 2), n0 = (lane & 3) * S;
+  const bool ron = w.c0 + rc < a.Dg;
+  const long rd = w.d0 + rc;
+  const int ts = w.chunk * a.chunk, te = min(ts + a.chunk, a.T), tv = min(te, w.len);
+
+  float A2[S], Ar[S], g[S], dA[S];
+  load_state<S>(a.A, rd, n0, a.N, ron, Ar);
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    A2[s] = Ar[s] * LOG2E;
+    dA[s] = 0.f;
+    g[s] = 0.f;
+  }
+  if (!STATE) {
+    if (a.chunks > 1) {
+      if (ron) load_row<S>(a.cstate + (((long)w.b * a.chunks + w.chunk) * a.D + rd) * NP + n0, g);
+    } else {
+      load_state<S>(a.dhT, (long)w.b * a.D + rd, n0, a.N, ron, g);
+    }
+  }
+  float dD[EPT], dbias[EPT];
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) dD[i] = dbias[i] = 0.f;
+  const long gof = (long)w.g * a.Dg;
+  const long uo = (long)w.b * a.sub + gof, dof = (long)w.b * a.sdb + gof, zo = (long)w.b * a.szb + gof,
+             go = (long)w.b * a.sob + gof, oo = (long)w.b * a.T * a.D + gof;
+  const int ch = w.c0 + cc;
+  float sum = 0.f;
+
+  for (int t0 = ts + (te - ts - 1) / TT * TT; t0 >= ts; t0 -= TT) {
+    const int t = t0 + ct;
+    const bool on = t < tv;
+    // what the tile's elements give by themselves.  Nothing of it is kept over the walk (its registers hold the tile's
+    // states): what is needed again behind it is fetched again, from the caches
+    {
+      float u[EPT], dl[EPT], z[EPT], go_[EPT], bias[EPT];
+      if (!STATE) fetch<T, EPT>(a.u, uo + (long)t * a.sut, ch, a.Dg, a.vec, on, u);
+      fetch<T, EPT>(a.dt, dof + (long)t * a.sdt, ch, a.Dg, a.vec, on, dl);
+      fetch<T, EPT>(a.dout, go + (long)t * a.sot, ch, a.Dg, a.vec, on, go_);
+      if (a.z) fetch<T, EPT>(a.z, zo + (long)t * a.szt, ch, a.Dg, a.vec, on, z);
+      fetch<float, EPT>(a.bias, w.g * a.Dg, ch, a.Dg, false, a.bias != nullptr, bias);
+      if (!STATE) stage_bc<T, S, TT>(a.Bm, (long)w.b * a.sBb + (long)w.g * a.sBg, a.sBt, t0, tv, a.N, sB);
+      stage_bc<T, S, TT>(a.Cm, (long)w.b * a.sCb + (long)w.g * a.sCg, a.sCt, t0, tv, a.N, sC);
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) {
+        float d = dl[i] + bias[i];
+        if (a.softplus) d = softplus(d);
+        d = on && ch + i < a.Dg ? d : 0.f;
+        sD[ct][cc + i][0] = d;
+        if (!STATE) sD[ct][cc + i][1] = d * u[i];
+        sG[ct][cc + i] = a.z ? go_[i] * tb_silu(z[i]) : go_[i];
+      }
+    }
+    __syncthreads();
+    if (STATE) {
+#pragma unroll 4
+      for (int k = TT - 1; k >= 0; --k) {
+        const float d = sD[k][rc][0], y = sG[k][rc];
+        float cv[S];
+        load_row<S>(sC + k * NP + n0, cv);
+        sum += d;
+#pragma unroll
+        for (int s = 0; s < S; ++s) g[s] = fmaf(cv[s], y, g[s]) * __builtin_amdgcn_exp2f(d * A2[s]);
+      }
+    } else {
+      float h[TT + 1][S];      // h[k]: the state in front of step k
+      if (ron) load_row<S>(a.ck + (((long)w.b * a.cktiles + t0 / TT) * a.D + rd) * NP + n0, h[0]);
+      else
+#pragma unroll
+        for (int s = 0; s < S; ++s) h[0][s] = 0.f;
+      // one step ahead of the arithmetic, and no further: left alone, the compiler keeps all of a tile's rows in registers
+      Row<S> r;
+      r.load(sD[0][rc], sG[0][rc], sB + n0, sC + n0);
+#pragma unroll
+      for (int k = 0; k < TT; ++k) {
+        const Row<S> c = r;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        if (k + 1 < TT) r.load(sD[k + 1][rc], sG[k + 1][rc], sB + (k + 1) * NP + n0, sC + (k + 1) * NP + n0);
+        float y = 0.f;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          h[k + 1][s] = fmaf(__builtin_amdgcn_exp2f(c.d * A2[s]), h[k][s], c.x * c.b[s]);
+          y = fmaf(h[k + 1][s], c.c[s], y);
+        }
+        y = quad_sum(y);
+        if ((lane & 3) == 0) sY[k][rc] = y;
+      }
+#pragma unroll
+      for (int k = TT - 1; k >= 0; --k) {
+        const Row<S> c = r;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        if (k > 0) r.load(sD[k - 1][rc], sG[k - 1][rc], sB + (k - 1) * NP + n0, sC + (k - 1) * NP + n0);
+        float v[2 * S], gB = 0.f, gA = 0.f;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          g[s] = fmaf(c.c[s], c.y, g[s]);
+          v[s] = g[s] * c.x;                       // dB
+          v[S + s] = h[k + 1][s] * c.y;            // dC
+          gB = fmaf(g[s], c.b[s], gB);
+          g[s] *= __builtin_amdgcn_exp2f(c.d * A2[s]);
+          const float q = g[s] * h[k][s];
+          gA = fmaf(q, Ar[s], gA);
+          dA[s] = fmaf(q, c.d, dA[s]);
+        }
+        gB = quad_sum(gB);
+        gA = quad_sum(gA);
+        if ((lane & 3) == 0) {
+          sGB[k][rc] = gB;
+          sGA[k][rc] = gA;
+        }
+        channel_sum<S>(v);
+        constexpr int H = S > 1 ? S / 2 : 1;
+        if ((lane & 12) == 0 && (S > 1 || (lane & 16) == 0)) {
+          float* p = &sP[wave][k][(lane >> 5) * NP + n0 + (S > 1 && (lane & 16) ? H : 0)];
+#pragma unroll
+          for (int i = 0; i < H; ++i) p[i] = v[i];
+        }
+      }
+    }
+    __syncthreads();
+    if (!STATE) {
+      for (int i = tid; i < TT * 2 * NP; i += 256) {
+        const int k = i / (2 * NP), n = i % (2 * NP);
+        if (t0 + k < te)
+          a.bc[((((long)w.b * a.G + w.g) * a.cblk + w.cb) * a.T + t0 + k) * (2 * NP) + n] =
+              t0 + k < tv ? (sP[0][k][n] + sP[1][k][n]) + (sP[2][k][n] + sP[3][k][n]) : 0.f;
+      }
+      if (t < te) {
+        float o[EPT], u[EPT], dl[EPT], par[EPT];
+        fetch<T, EPT>(a.u, uo + (long)t * a.sut, ch, a.Dg, a.vec, on, u);
+        fetch<T, EPT>(a.dt, dof + (long)t * a.sdt, ch, a.Dg, a.vec, on, dl);
+        fetch<float, EPT>(a.bias, gof, ch, a.Dg, false, a.bias != nullptr, par);
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+          o[i] = on ? fmaf(u[i], sGB[ct][cc + i], sGA[ct][cc + i]) : 0.f;
+          if (a.softplus && on) o[i] *= tb_sig(dl[i] + par[i]);      // d delta / d raw
+          dbias[i] += o[i];
+        }
+        if (a.ddt) put<T, EPT>(a.ddt, oo + (long)t * a.D, ch, a.Dg, a.vec, o);
+        fetch<float, EPT>(a.Dp, gof, ch, a.Dg, false, a.Dp != nullptr, par);
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+          const float dy = sG[ct][cc + i];
+          o[i] = on ? fmaf(sD[ct][cc + i][0], sGB[ct][cc + i], par[i] * dy) : 0.f;
+          dD[i] = fmaf(dy, u[i], dD[i]);
+        }
+        if (a.du) put<T, EPT>(a.du, oo + (long)t * a.D, ch, a.Dg, a.vec, o);
+        if (a.dz) {
+          float z[EPT];
+          fetch<T, EPT>(a.dout, go + (long)t * a.sot, ch, a.Dg, a.vec, on, o);
+          fetch<T, EPT>(a.z, zo + (long)t * a.szt, ch, a.Dg, a.vec, on, z);
+#pragma unroll
+          for (int i = 0; i < EPT; ++i) {
+            const float q = tb_sig(z[i]), y = fmaf(par[i], u[i], sY[ct][cc + i]);
+            o[i] = on ? o[i] * y * (q * (1.f + z[i] * (1.f - q))) : 0.f;
+          }
+          put<T, EPT>(a.dz, oo + (long)t * a.D, ch, a.Dg, a.vec, o);
+        }
+      }
+      __syncthreads();
+    }
+  }
+  const long row = ((long)w.b * a.chunks + w.chunk) * a.D + rd;
+  if (STATE) {
+    if (ron) store_row<S>(a.cstate + row * NP + n0, g);
+    if (ron && (lane & 3) == 0) a.csum[row] = sum;
+    return;
+  }
+  if (ron) {
+#pragma unroll
+    for (int s = 0; s < S; ++s) a.par[row * (NP + 2) + n0 + s] = dA[s];
+  }
+  if (a.dh0 && w.chunk == 0) store_state<S>(a.dh0, (long)w.b * a.D + rd, n0, a.N, ron, g);
+  // dD and dbias: over the block's steps, in their order
+  float* f = &sD[0][0][0];
+#pragma unroll
+  for (int i = 0; i < EPT; ++i) {
+    f[(ct * CB + cc + i) * 2] = dD[i];
+    f[(ct * CB + cc + i) * 2 + 1] = dbias[i];
+  }
+  __syncthreads();
+  if (tid < 2 * CB && w.c0 + tid / 2 < a.Dg) {
+    float s = 0.f;
+    for (int k = 0; k < TT; ++k) s += f[k * CB * 2 + tid];
+    a.par[(((long)w.b * a.chunks + w.chunk) * a.D + w.d0 + tid / 2) * (NP + 2) + NP + (tid & 1)] = s;
+  }
+}
+
+// dA (D, N), dD (D), dbias (D) from the rows of (sequence, chunk), in their order by four threads a value
+__global__ void __launch_bounds__(256) scan_finish_par(const float* par, int rows, int D, int N, int NP, float* dA, float* dD, float* dbias) {
+  __shared__ float red[4][64];
+  const long cols = (long)D * (NP + 2), col = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+  const int q = threadIdx.x >> 6, per = (rows + 3) / 4;
+  float s = 0.f;
+  if (col < cols) {
+    const int r1 = min(rows, (q + 1) * per);
+#pragma unroll 4
+    for (int r = q * per; r < r1; ++r) s += par[r * cols + col];
+  }
+  red[q][threadIdx.x & 63] = s;
+  __syncthreads();
+  if (q == 0 && col < cols) {
+    const int l = threadIdx.x;
+    s = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
+    const long d = col / (NP + 2);
+    const int n = (int)(col % (NP + 2));
+    if (n < N) {
+      if (dA) dA[d * N + n] = s;
+    } else if (n == NP) {
+      if (dD) dD[d] = s;
+    } else if (n == NP + 1) {
+      if (dbias) dbias[d] = s;
+    }
+  }
+}
+
+// dB, dC (B, T, G, N) from the channel blocks' sums
+template <typename T>
+__global__ void __launch_bounds__(256) scan_finish_bc(const float* bc, int B, int Tn, int G, int N, int NP, int cblk, void* dB, void* dC) {
+  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  const long per = (long)Tn * 2 * NP;
+  if (id >= (long)B * G * per) return;
+  const long bg = id / per, r = id % per;
+  const int n = (int)(r % (2 * NP)), t = (int)(r / (2 * NP));
+  const int half = n >= NP, k = n - half * NP;
+  if (k >= N) return;
+  float s = 0.f;
+#pragma unroll 4
+  for (int c = 0; c < cblk; ++c) s += bc[(bg * cblk + c) * per + r];
+  void* o = half ? dC : dB;
+  if (o) static_cast<T*>(o)[(((bg / G) * Tn + t) * G + bg % G) * N + k] = (T)s;
+}
+
+struct StepArgs {
+  float* state;
+  const void *u, *dt, *z, *Bm, *Cm;
+  const float *A, *Dp, *bias;
+  void* out;
+  long sub, sdb, szb, sBb, sBg, sCb, sCg, ssb;
+  int B, D, N, G, Dg, softplus;
+};
+
+// one step: reads and writes each state once.  Lanes as above: four a channel.
+template <typename T, int S>
+__global__ void __launch_bounds__(256) scan_step(StepArgs a) {
+  const int lane = threadIdx.x & 3, n0 = lane * S;
+  const long id = (long)blockIdx.x * 64 + (threadIdx.x >> 2);
+  const bool on = id < (long)a.B * a.D;
+  const int b = on ? (int)(id / a.D) : 0, d = on ? (int)(id % a.D) : 0, g = d / a.Dg;
+  float* st = a.state + b * a.ssb + (long)d * a.N;
+  float h[S], A[S], bv[S], cv[S];
+  const bool whole = a.N == 4 * S && (a.ssb & 3) == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.A) & 15) == 0;
+  if (whole) {
+    tb_load_n(st + n0, h);
+    tb_load_n(a.A + (long)d * a.N + n0, A);
+  }
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    const bool in = n0 + s < a.N;
+    if (!whole) {
+      h[s] = in ? st[n0 + s] : 0.f;
+      A[s] = in ? a.A[(long)d * a.N + n0 + s] : 0.f;
+    }
+    bv[s] = in ? (float)static_cast<const T*>(a.Bm)[b * a.sBb + g * a.sBg + n0 + s] : 0.f;
+    cv[s] = in ? (float)static_cast<const T*>(a.Cm)[b * a.sCb + g * a.sCg + n0 + s] : 0.f;
+  }
+  const float u = (float)static_cast<const T*>(a.u)[b * a.sub + d];
+  float dl = (float)static_cast<const T*>(a.dt)[b * a.sdb + d] + (a.bias ? a.bias[d] : 0.f);
+  if (a.softplus) dl = softplus(dl);
+  float y = 0.f;
+#pragma unroll
+  for (int s = 0; s < S; ++s) {
+    h[s] = fmaf(__builtin_amdgcn_exp2f(dl * (A[s] * LOG2E)), h[s], dl * u * bv[s]);
+    y = fmaf(h[s], cv[s], y);
+  }
+  y = quad_sum(y);
+  if (!on) return;
+  if (whole) tb_store_n(st + n0, h);
+  else
+#pragma unroll
+    for (int s = 0; s < S; ++s)
+      if (n0 + s < a.N) st[n0 + s] = h[s];
+  if (lane == 0) {
+    if (a.Dp) y = fmaf(a.Dp[d], u, y);
+    if (a.z) y *= tb_silu((float)static_cast<const T*>(a.z)[b * a.szb + d]);
+    static_cast<T*>(a.out)[(long)b * a.D + d] = (T)y;
+  }
+}
+
+int states_per_lane(int N) { return N <= 4 ? 1 : N <= 8 ? 2 : N <= 16 ? 4 : N <= 32 ? 8 : 16; }
+
+template <typename F>
+int by_shape(int dtype, int S, F&& f) {
+#define TB_S(T)                                                  \
+  switch (S) {                                                   \
+    case 1: return f.template operator()<T, 1>();                \
+    case 2: return f.template operator()<T, 2>();                \
+    case 4: return f.template operator()<T, 4>();                \
+    case 8: return f.template operator()<T, 8>();                \
+    default: return f.template operator()<T, 16>();              \
+  }
+  if (dtype == TB_F32) TB_S(float)
+  if (dtype == TB_BF16) TB_S(__bf16)
+  TB_S(_Float16)
+#undef TB_S
+}
+
+struct FwdLaunch {
+  ScanArgs a;
+  long blocks;       // channel blocks of the batch
+  hipStream_t s;
+  template <typename T, int S>
+  int operator()() {
+    if (a.chunks > 1) {
+      scan_fwd<T, S, true><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
+      scan_chain<S, false><<<(unsigned)(((long)a.B * a.D * 4 * S + 255) / 256), 256, 0, s>>>(a);
+    }
+    scan_fwd<T, S, false><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
+    return 0;
+  }
+};
+struct BwdLaunch {
+  ScanArgs a;
+  long blocks;
+  float *dA, *dD, *dbias;
+  void *dB, *dC;
+  hipStream_t s;
+  template <typename T, int S>
+  int operator()() {
+    if (a.chunks > 1) {
+      scan_bwd<T, S, true><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
+      scan_chain<S, true><<<(unsigned)(((long)a.B * a.D * 4 * S + 255) / 256), 256, 0, s>>>(a);
+    }
+    scan_bwd<T, S, false><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
+    if (dA || dD || dbias)
+      scan_finish_par<<<(unsigned)(((long)a.D * (4 * S + 2) + 63) / 64), 256, 0, s>>>(a.par, a.B * a.chunks, a.D, a.N, 4 * S, dA, dD, dbias);
+    if (dB || dC)
+      scan_finish_bc<T><<<(unsigned)(((long)a.B * a.G * a.T * 8 * S + 255) / 256), 256, 0, s>>>(a.bc, a.B, a.T, a.G, a.N, 4 * S, a.cblk, dB, dC);
+    return 0;
+  }
+};
+struct StepLaunch {
+  StepArgs a;
+  hipStream_t s;
+  template <typename T, int S>
+  int operator()() {
+    scan_step<T, S><<<(unsigned)(((long)a.B * a.D + 63) / 64), 256, 0, s>>>(a);
+    return 0;
+  }
+};
+
+// chunks of the steps: none where the channel blocks alone give the chip a block per compute unit (cutting the steps costs
+// a second walk over them), else as many as bring it to four blocks a unit, of 128 steps at least
+void plan(int B, int T, int G, int Dg, int* cblk, int* chunk, int* chunks) {
+  *cblk = (Dg + CB - 1) / CB;
+  const long blocks = (long)B * G * *cblk;
+  const long cus = tb_num_cus();
+  long n = 1;
+  if (blocks < cus * 3 / 4) n = (4 * cus + blocks - 1) / blocks;
+  long len = (T + n - 1) / n;
+  if (len < 128) len = 128;
+  len = (len + 31) / 32 * 32;
+  *chunk = (int)len;
+  *chunks = T > 0 ? (int)((T + len - 1) / len) : 1;
+}
+
+int check_common(const char* what, int B, long T, int D, int N, int G, int dtype) {
+  if (B < 0 || T < 0 || D < 1 || N < 1 || G < 1 || D % G) return tb_set_error(TB_ERR_ARG, "%s: bad sizes B=%d T=%ld D=%d N=%d G=%d", what, B, T, D, N, G);
+  if (N > NMAX) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: %d states a channel are not supported (1 to %d)", what, N, NMAX);
+  if (!tb_dtype_ok(dtype)) return tb_set_error(TB_ERR_ARG, "%s: bad element type %d", what, dtype);
+  return TB_OK;
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+// 16-byte accesses: every row of every tensor starts on 16 bytes, and so does every group
+bool can_vec(const ScanArgs& a, int dtype) {
+  const int v = dtype == TB_F32 ? 4 : 8;
+  if (a.D % v || a.Dg % v || a.sub % v || a.sut % v || a.sdb % v || a.sdt % v) return false;
+  if (a.z && (a.szb % v || a.szt % v)) return false;
+  if (a.dout && (a.sob % v || a.sot % v)) return false;
+  const void* p[] = {a.u, a.dt, a.z, a.dout, a.out, a.du, a.ddt, a.dz};
+  for (const void* q : p)
+    if (!aligned(q)) return false;
+  return true;
+}
+
+struct Sizes {
+  size_t cstate, csum, bc, par, total;
+};
+Sizes sizes(int B, int T, int D, int N, int G, int backward) {
+  int cblk, chunk, chunks;
+  plan(B, T, G, D / G, &cblk, &chunk, &chunks);
+  const size_t NP = 4 * states_per_lane(N);
+  Sizes z;
+  z.cstate = chunks > 1 ? tb_align_up((size_t)B * chunks * D * NP * 4, 256) : 0;
+  z.csum = chunks > 1 ? tb_align_up((size_t)B * chunks * D * 4, 256) : 0;
+  z.bc = backward ? tb_align_up((size_t)B * G * cblk * T * 2 * NP * 4, 256) : 0;
+  z.par = backward ? tb_align_up((size_t)B * chunks * D * (NP + 2) * 4, 256) : 0;
+  z.total = z.cstate + z.csum + z.bc + z.par + 256;
+  return z;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t tb_scan_workspace_bytes(int B, int T, int D, int N, int G, int backward) {
+  if (B < 1 || T < 1 || D < 1 || N < 1 || N > NMAX || G < 1 || D % G) return 256;
+  return sizes(B, T, D, N, G, backward).total;
+}
+
+size_t tb_scan_states_bytes(int B, int T, int D, int N) {
+  if (B < 1 || T < 1 || D < 1 || N < 1 || N > NMAX) return 0;
+  const int S = states_per_lane(N), tt = bwd_tile(S);
+  return (size_t)B * ((T + tt - 1) / tt) * D * 4 * S * 4;
+}
+
+int tb_scan_fwd(const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const long* strides, const float* A,
+                const float* Dp, const float* dt_bias, int softplus, const float* h0, const int* lengths, void* out, float* hT,
+                float* states, int B, int T, int D, int N, int G, int dtype, void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_common("scan_fwd", B, T, D, N, G, dtype);
+  if (rc) return rc;
+  if (B < 1 || T < 1) return tb_set_error(TB_ERR_ARG, "scan_fwd: an empty batch has nothing to scan");
+  if (!u || !dt || !Bm || !Cm || !strides || !A || !out || !ws) return tb_set_error(TB_ERR_ARG, "scan_fwd: null pointer");
+  const Sizes sz = sizes(B, T, D, N, G, 0);
+  if (ws_bytes < sz.total) return tb_set_error(TB_ERR_WORKSPACE, "scan_fwd: workspace too small");
+  const int S = states_per_lane(N);
+  ScanArgs a{};
+  a.u = u; a.dt = dt; a.z = z; a.Bm = Bm; a.Cm = Cm;
+  a.A = A; a.Dp = Dp; a.bias = dt_bias; a.h0 = h0; a.lengths = lengths;
+  a.out = out; a.hT = hT; a.ck = states;
+  const long* q = strides;
+  a.sub = q[0]; a.sut = q[1]; a.sdb = q[2]; a.sdt = q[3]; a.szb = q[4]; a.szt = q[5];
+  a.sBb = q[6]; a.sBt = q[7]; a.sBg = q[8]; a.sCb = q[9]; a.sCt = q[10]; a.sCg = q[11];
+  a.B = B; a.T = T; a.D = D; a.N = N; a.G = G; a.Dg = D / G;
+  plan(B, T, G, a.Dg, &a.cblk, &a.chunk, &a.chunks);
+  a.softplus = softplus;
+  a.ckt = states ? bwd_tile(S) : 0;
+  a.cktiles = states ? (T + a.ckt - 1) / a.ckt : 0;
+  a.cstate = static_cast<float*>(ws);
+  a.csum = reinterpret_cast<float*>(static_cast<char*>(ws) + sz.cstate);
+  a.vec = can_vec(a, dtype);
+  by_shape(dtype, S, FwdLaunch{a, (long)B * G * a.cblk, static_cast<hipStream_t>(stream)});
+  TB_LAUNCH_CHECK("scan_fwd");
+  return TB_OK;
+}
+
+int tb_scan_bwd(const void* dout, const void* u, const void* dt, const void* z, const void* Bm, const void* Cm, const long* strides,
+                const float* A, const float* Dp, const float* dt_bias, int softplus, const int* lengths, const float* states,
+                const float* dhT, void* du, void* ddt, void* dz, void* dB, void* dC, float* dA, float* dD, float* dbias, float* dh0,
+                int B, int T, int D, int N, int G, int dtype, void* ws, size_t ws_bytes, void* stream) {
+  int rc = check_common("scan_bwd", B, T, D, N, G, dtype);
+  if (rc) return rc;
+  if (B < 1 || T < 1) return tb_set_error(TB_ERR_ARG, "scan_bwd: an empty batch has no gradients to form here");
+  if (!dout || !u || !dt || !Bm || !Cm || !strides || !A || !states || !ws) return tb_set_error(TB_ERR_ARG, "scan_bwd: null pointer");
+  const Sizes sz = sizes(B, T, D, N, G, 1);
+  if (ws_bytes < sz.total) return tb_set_error(TB_ERR_WORKSPACE, "scan_bwd: workspace too small");
+  const int S = states_per_lane(N);
+  ScanArgs a{};
+  a.u = u; a.dt = dt; a.z = z; a.Bm = Bm; a.Cm = Cm; a.dout = dout;
+  a.A = A; a.Dp = Dp; a.bias = dt_bias; a.dhT = dhT; a.lengths = lengths;
+  a.du = du; a.ddt = ddt; a.dz = z ? dz : nullptr; a.dh0 = dh0;
+  a.ck = const_cast<float*>(states);
+  const long* q = strides;
+  a.sub = q[0]; a.sut = q[1]; a.sdb = q[2]; a.sdt = q[3]; a.szb = q[4]; a.szt = q[5];
+  a.sBb = q[6]; a.sBt = q[7]; a.sBg = q[8]; a.sCb = q[9]; a.sCt = q[10]; a.sCg = q[11];
+  a.sob = q[12]; a.sot = q[13];
+  a.B = B; a.T = T; a.D = D; a.N = N; a.G = G; a.Dg = D / G;
+  plan(B, T, G, a.Dg, &a.cblk, &a.chunk, &a.chunks);
+  a.softplus = softplus;
+  a.ckt = bwd_tile(S);
+  a.cktiles = (T + a.ckt - 1) / a.ckt;
+  char* p = static_cast<char*>(ws);
+  a.cstate = reinterpret_cast<float*>(p);
+  a.csum = reinterpret_cast<float*>(p + sz.cstate);
+  a.bc = reinterpret_cast<float*>(p + sz.cstate + sz.csum);
+  a.par = reinterpret_cast<float*>(p + sz.cstate + sz.csum + sz.bc);
+  a.vec = can_vec(a, dtype);
+  by_shape(dtype, S, BwdLaunch{a, (long)B * G * a.cblk, dA, dD, dbias, dB, dC, static_cast<hipStream_t>(stream)});
+  TB_LAUNCH_CHECK("scan_bwd");
+  return TB_OK;
+}
+
+int tb_scan_step(float* state, long state_batch_stride, const void* u, const void* dt, const void* z, const void* Bm, const void* Cm,
+                 const long* strides, const float* A, const float* Dp, const float* dt_bias, int softplus, void* out, int B, int D, int N,
+                 int G, int dtype, void* stream) {
+  int rc = check_common("scan_step", B, 1, D, N, G, dtype);
+  if (rc) return rc;
+  if (B == 0) return TB_OK;
+  if (!state || !u || !dt || !Bm || !Cm || !strides || !A || !out) return tb_set_error(TB_ERR_ARG, "scan_step: null pointer");
+  const long* q = strides;
+  StepArgs a{state, u, dt, z, Bm, Cm, A, Dp, dt_bias, out, q[0], q[1], q[2], q[3], q[4], q[5], q[6], state_batch_stride,
+             B, D, N, G, D / G, softplus};
+  by_shape(dtype, states_per_lane(N), StepLaunch{a, static_cast<hipStream_t>(stream)});
+  TB_LAUNCH_CHECK("scan_step");
+  return TB_OK;
+}
+
+}  // extern "C"
