@@ -15,6 +15,8 @@
 // Few rows (a batch of single tokens) are bound by reading W once: a kernel without LDS staging whose waves split K.
 #include "elem.h"
 
+#include <type_traits>
+
 namespace {
 
 typedef __attribute__((address_space(1))) const void gvoid;
@@ -28,13 +30,28 @@ __device__ __forceinline__ float tanh_rel(float x) {
   const float p = x * (1.f + q * (-0.333333333f + q * (0.133333333f + q * (-0.0539682540f + q * 0.0218694885f))));
   return fabsf(x) < 0.125f ? p : tb_tanh(x);
 }
+// half of erfc(|z| / sqrt 2): t e^(-z^2/2 + P(t)), t = 1 / (1 + 0.4 x), with P a degree 8 least-maximum fit of
+// log(erfc(x) e^(x^2) / t) on 0 <= x < 9.5 (off by 9e-8): the lower tail keeps its relative precision, where 1 + erf cancels
+__device__ __forceinline__ float half_erfc(float z) {
+  const float x = fabsf(z) * 0.70710678f, t = __builtin_amdgcn_rcpf(fmaf(0.4f, x, 1.f));
+  float p = -0.2059148f;
+  p = fmaf(p, t, 0.91647777f);
+  p = fmaf(p, t, -1.46799367f);
+  p = fmaf(p, t, 0.97708137f);
+  p = fmaf(p, t, -0.42703877f);
+  p = fmaf(p, t, 0.29283921f);
+  p = fmaf(p, t, 0.40185486f);
+  p = fmaf(p, t, 1.00138551f);
+  p = fmaf(p, t, -1.48869157f);
+  return 0.5f * t * __expf(fmaf(-x, x, p));
+}
 __device__ __forceinline__ float act_of(float z, int act) {
   switch (act) {
     case 1: return tanh_rel(z);
     case 2: return tb_sig(z);
     case 3: return z < 0.f ? 0.f : z;
     case 4: return tb_silu(z);
-    case 5: return 0.5f * z * (1.f + erff(z * 0.70710678f));
+    case 5: { const float e = half_erfc(z); return z * (z > 0.f ? 1.f - e : e); }
     default: return z;
   }
 }
@@ -44,7 +61,7 @@ __device__ __forceinline__ float act_grad(float z, int act) {
     case 2: { const float y = tb_sig(z); return y * (1.f - y); }
     case 3: return z > 0.f ? 1.f : 0.f;
     case 4: { const float y = tb_sig(z); return y * (1.f + z * (1.f - y)); }
-    case 5: return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+    case 5: { const float e = half_erfc(z); return (z > 0.f ? 1.f - e : e) + z * 0.39894228f * __expf(-0.5f * z * z); }
     default: return 1.f;
   }
 }
@@ -128,7 +145,7 @@ struct GemmArgs {
   long M;
   int N, K;
   int tm, tn, splits, per;  // tiles; k tiles a split
-  int four;                 // rows of y, z, the residual and the bias allow four columns at once
+  int four;                 // rows of y, z, the residual and the bias allow 16-byte accesses
   Epi e;
 };
 
@@ -142,57 +159,132 @@ __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& im, int& in
   in = in_band / rows;
 }
 
+// 64 x 64 sums of a wave, in LDS as gemm_nt leaves them, through the epilogue to memory
+template <typename T>
+__device__ __forceinline__ void write_block(const GemmArgs& a, const float* own, long m0, int n0, int lane) {
+  const Epi& e = a.e;
+  auto piece = [&](int r, int c) { return *reinterpret_cast<const f32x4*>(own + r * 64 + ((c ^ (r & 15)) * 4)); };
+  if (!a.four) {                       // any width: a lane a column, element by element
+    const int n = n0 + lane;
+    if (n >= a.N) return;
+    const float b = e.bias && !e.slab ? (float)static_cast<const T*>(e.bias)[n] : 0.f;
+#pragma unroll 2
+    for (int r = 0; r < 64; ++r) {
+      const long m = m0 + r;
+      if (m >= a.M) break;
+      float v = own[r * 64 + (((lane >> 2) ^ (r & 15)) * 4) + (lane & 3)];
+      if (e.slab) {
+        e.slab[((long)blockIdx.y * a.M + m) * a.N + n] = v;
+        continue;
+      }
+      v += b;
+      if (e.z) e.z[m * a.N + n] = v;
+      v = act_of(v, e.act);
+      if (e.res) v += (float)static_cast<const T*>(e.res)[m * e.ldr + n];
+      static_cast<T*>(e.y)[m * a.N + n] = (T)v;
+    }
+    return;
+  }
+  if (e.slab) {
+    const int c = lane & 15, n = n0 + c * 4;
+    if (n >= a.N) return;
+#pragma unroll 2
+    for (int r = lane >> 4; r < 64; r += 4) {
+      const long m = m0 + r;
+      if (m >= a.M) break;
+      *reinterpret_cast<f32x4*>(e.slab + ((long)blockIdx.y * a.M + m) * a.N + n) = piece(r, c);
+    }
+    return;
+  }
+  constexpr int V = 16 / sizeof(T), L = 64 / V;       // columns a lane, lanes a row
+  const int c = lane % L, n = n0 + c * V;
+  if (n >= a.N) return;                                // four: N is a multiple of V
+  float b[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) b[i] = 0.f;
+  if (e.bias) tb_load_n(static_cast<const T*>(e.bias) + n, b);
+#pragma unroll 2
+  for (int r = lane / L; r < 64; r += V) {
+    const long m = m0 + r;
+    if (m >= a.M) break;
+    float o[V], q[V];
+    if (e.res) tb_load_n(static_cast<const T*>(e.res) + m * e.ldr + n, q);
+#pragma unroll
+    for (int k = 0; k < V / 4; ++k) {
+      const f32x4 v = piece(r, c * (V / 4) + k);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[k * 4 + i] = v[i] + b[k * 4 + i];
+    }
+    if (e.z) tb_store_n(e.z + m * a.N + n, o);
+    if (e.act)
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = act_of(o[i], e.act);
+    if (e.res)
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] += q[i];
+    tb_store_n(static_cast<T*>(e.y) + m * a.N + n, o);
+  }
+}
+
+// 64 bytes of k a tile, four tiles in LDS: while one tile is multiplied from registers, the next one's fragments are read
+// from LDS and the copies of the three behind it are under way.  One barrier a tile: behind it the tile that was just read into
+// registers by every wave is free for a new copy, and the next one has landed (the copies still under way are counted, not
+// drained).
 template <typename T, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) gemm_nt(GemmArgs a) {
-  constexpr int WAVES = (BM / WM) * (BN / WN), CE = 16 / sizeof(T), BK = 8 * CE;
-  constexpr int MF = WM / 16, NF = WN / 16, LP = BM / 8 / WAVES, LQ = BN / 8 / WAVES;
-  __shared__ __attribute__((aligned(16))) char lds[2][(BM + BN) * 128];
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm_nt(GemmArgs a) {
+  constexpr int WAVES = (BM / WM) * (BN / WN), CE = 16 / sizeof(T), BK = 4 * CE;
+  constexpr int MF = WM / 16, NF = WN / 16, LP = BM / 16 / WAVES, LQ = BN / 16 / WAVES;
+  constexpr int STAGE = (BM + BN) * 64;
+  static_assert(LP + LQ == 4, "the counted waits below are for four copies a wave and tile");
+  __shared__ __attribute__((aligned(16))) char lds[4 * STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int im, in;
   tile_of(blockIdx.x, a.tm, a.tn, im, in);
   const long m0 = (long)im * BM;
   const int n0 = in * BN;
   const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
-  const int kt0 = blockIdx.y * a.per, kt1 = min(kt0 + a.per, (a.K + BK - 1) / BK);
+  const int kt0 = blockIdx.y * a.per, nt = min(a.per, (a.K + BK - 1) / BK - kt0);
 
-  // what this lane copies: row 8 i + lane / 8 of each of its pieces, and of that row's eight 16-byte pieces the one whose
-  // place in LDS is lane % 8
-  const int lr = lane >> 3, piece = ((lane & 7) ^ lr) * CE;
+  // what this lane copies: row 16 i + lane / 4 of each of its pieces, and of that row's four 16-byte pieces the one whose place
+  // in LDS is lane % 4: piece p of row r lies at p ^ (r / 2 % 4), so that eight neighbouring rows fill all banks
+  const int lr = lane >> 2, piece = ((lane & 3) ^ ((lr >> 1) & 3)) * CE;
   const T* pp[LP];
   const T* qp[LQ];
 #pragma unroll
   for (int i = 0; i < LP; ++i) {
-    long r = m0 + (wave * LP + i) * 8 + lr;
+    long r = m0 + (wave * LP + i) * 16 + lr;
     r = r < a.M ? r : a.M - 1;                  // rows behind the last: any row, never stored
     pp[i] = static_cast<const T*>(a.P) + r * a.ldp + piece;
   }
 #pragma unroll
   for (int i = 0; i < LQ; ++i) {
-    int r = n0 + (wave * LQ + i) * 8 + lr;
+    int r = n0 + (wave * LQ + i) * 16 + lr;
     r = r < a.N ? r : a.N - 1;
     qp[i] = static_cast<const T*>(a.Q) + (long)r * a.ldq + piece;
   }
-  auto copy = [&](int kt, int buf) {
-    const long k = (long)kt * BK;
-    if (k + BK <= a.K) {
+  // TAIL: the tile may reach behind the end of K, whose pieces come from a row of zeros
+  auto copy = [&](int t, auto tail) {
+    char* to = lds + (t & 3) * STAGE;
+    const long k = (long)(kt0 + t) * BK;
+    const bool in_k = !tail || k + piece < a.K;
+    const uintptr_t zero = reinterpret_cast<uintptr_t>(g_zeros);
 #pragma unroll
-      for (int i = 0; i < LP; ++i)
-        __builtin_amdgcn_global_load_lds((gvoid*)(pp[i] + k), (lvoid*)&lds[buf][(wave * LP + i) * 1024], 16, 0, 0);
+    for (int i = 0; i < LP; ++i)
+      __builtin_amdgcn_global_load_lds((gvoid*)(in_k ? reinterpret_cast<uintptr_t>(pp[i] + k) : zero),
+                                       (lvoid*)(to + (wave * LP + i) * 1024), 16, 0, 0);
 #pragma unroll
-      for (int i = 0; i < LQ; ++i)
-        __builtin_amdgcn_global_load_lds((gvoid*)(qp[i] + k), (lvoid*)&lds[buf][BM * 128 + (wave * LQ + i) * 1024], 16, 0, 0);
-    } else {       // the last tile: pieces behind K come from a row of zeros
-      const bool in_k = k + piece < a.K;
-      const uintptr_t zero = reinterpret_cast<uintptr_t>(g_zeros);
+    for (int i = 0; i < LQ; ++i)
+      __builtin_amdgcn_global_load_lds((gvoid*)(in_k ? reinterpret_cast<uintptr_t>(qp[i] + k) : zero),
+                                       (lvoid*)(to + BM * 64 + (wave * LQ + i) * 1024), 16, 0, 0);
+  };
+  const int place = ((lane >> 4) ^ ((lane >> 1) & 3)) * 16;
+  const int po = (wm + (lane & 15)) * 64 + place, qo = BM * 64 + (wn + (lane & 15)) * 64 + place;
+  auto read = [&](int t, u32x4 (&fp)[MF], u32x4 (&fq)[NF]) {
+    const char* from = lds + (t & 3) * STAGE;
 #pragma unroll
-      for (int i = 0; i < LP; ++i)
-        __builtin_amdgcn_global_load_lds((gvoid*)(in_k ? reinterpret_cast<uintptr_t>(pp[i] + k) : zero),
-                                         (lvoid*)&lds[buf][(wave * LP + i) * 1024], 16, 0, 0);
+    for (int j = 0; j < NF; ++j) fq[j] = *reinterpret_cast<const u32x4*>(from + qo + j * 1024);
 #pragma unroll
-      for (int i = 0; i < LQ; ++i)
-        __builtin_amdgcn_global_load_lds((gvoid*)(in_k ? reinterpret_cast<uintptr_t>(qp[i] + k) : zero),
-                                         (lvoid*)&lds[buf][BM * 128 + (wave * LQ + i) * 1024], 16, 0, 0);
-    }
+    for (int i = 0; i < MF; ++i) fp[i] = *reinterpret_cast<const u32x4*>(from + po + i * 1024);
   };
 
   f32x4 acc[MF][NF];
@@ -200,49 +292,80 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64) gemm_nt(GemmArgs a
   for (int i = 0; i < MF; ++i)
 #pragma unroll
     for (int j = 0; j < NF; ++j) acc[i][j] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  u32x4 fp[2][MF], fq[2][NF];
 
-  if (kt0 < kt1) copy(kt0, 0);
-  __syncthreads();
-  for (int kt = kt0; kt < kt1; ++kt) {
-    const int buf = (kt - kt0) & 1;
-    if (kt + 1 < kt1) copy(kt + 1, buf ^ 1);
-    const char* sp = &lds[buf][(wm + (lane & 15)) * 128];
-    const char* sq = &lds[buf][BM * 128 + (wn + (lane & 15)) * 128];
+  // in front of a barrier: this wave has read tile t into registers, and its copies of tile t + 1 have landed
+  auto meet = [&](auto drain) {
+    if constexpr (drain) __builtin_amdgcn_s_waitcnt(0x0070);       // vmcnt(0) lgkmcnt(0)
+    else __builtin_amdgcn_s_waitcnt(0x0078);                       // vmcnt(8) lgkmcnt(0): two tiles' copies under way
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto multiply = [&](const u32x4 (&p)[MF], const u32x4 (&q)[NF]) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk) {
-      const int off = ((kk * 4 + (lane >> 4)) ^ (lane & 7)) * 16;
-      u32x4 fp[MF], fq[NF];
+    for (int i = 0; i < MF; ++i)
 #pragma unroll
-      for (int j = 0; j < NF; ++j) fq[j] = *reinterpret_cast<const u32x4*>(sq + j * 2048 + off);
+      for (int j = 0; j < NF; ++j) acc[i][j] = Mfma<T>::mul(q[j], p[i], acc[i][j]);
+    // keeps the products in front of the next barrier (an empty statement; without it they are moved behind it, where
+    // they no longer cover the copies and reads)
 #pragma unroll
-      for (int i = 0; i < MF; ++i) fp[i] = *reinterpret_cast<const u32x4*>(sp + i * 2048 + off);
+    for (int i = 0; i < MF; ++i)
 #pragma unroll
-      for (int i = 0; i < MF; ++i)
-#pragma unroll
-        for (int j = 0; j < NF; ++j) acc[i][j] = Mfma<T>::mul(fq[j], fp[i], acc[i][j]);
+      for (int j = 0; j < NF; ++j) asm volatile("" : "+v"(acc[i][j]));
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  constexpr std::true_type yes{};
+  constexpr std::false_type no{};
+  if (nt > 0) {
+    for (int t = 0; t < 4 && t < nt; ++t) copy(t, yes);
+    meet(yes);
+    read(0, fp[0], fq[0]);
+    int t = 0;
+    for (; t + 6 < nt; t += 2) {        // the copies here are of whole tiles
+      meet(no);
+      copy(t + 4, no);
+      read(t + 1, fp[1], fq[1]);
+      multiply(fp[0], fq[0]);
+      meet(no);
+      copy(t + 5, no);
+      read(t + 2, fp[0], fq[0]);
+      multiply(fp[1], fq[1]);
     }
-    __syncthreads();
-  }
-  // a lane holds row lane & 15 and four neighbouring columns of each 16 x 16 piece (Q is the left operand)
-#pragma unroll
-  for (int i = 0; i < MF; ++i)
-#pragma unroll
-    for (int j = 0; j < NF; ++j) {
-      const long m = m0 + wm + i * 16 + (lane & 15);
-      const int n = n0 + wn + j * 16 + (lane >> 4) * 4;
-      if (a.e.slab) {
-        if (m < a.M && n < a.N) {
-          float* s = a.e.slab + ((long)blockIdx.y * a.M + m) * a.N + n;
-          if (a.four) *reinterpret_cast<f32x4*>(s) = acc[i][j];
-          else
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (n + q < a.N) s[q] = acc[i][j][q];
-        }
-      } else {
-        finish4<T>(a.e, a.M, a.N, m, n, acc[i][j], a.four);
+    for (; t < nt; t += 2) {
+      meet(yes);
+      if (t + 4 < nt) copy(t + 4, yes);
+      if (t + 1 < nt) read(t + 1, fp[1], fq[1]);
+      multiply(fp[0], fq[0]);
+      if (t + 1 < nt) {
+        meet(yes);
+        if (t + 5 < nt) copy(t + 5, yes);
+        if (t + 2 < nt) read(t + 2, fp[0], fq[0]);
+        multiply(fp[1], fq[1]);
       }
     }
+  }
+  // A lane holds row lane & 15 and four neighbouring columns of each 16 x 16 piece (Q is the left operand).  They change
+  // places through LDS, 64 rows at a time in each wave's own 16 KB, so that every access to memory is of whole rows of
+  // the wave's 64 columns; and the epilogue is a short loop: unrolled over the accumulators it was 300 KB of code, whose fetching
+  // took longer than the products (K = 2048: 326 of 726 us).
+  __syncthreads();
+  float* own = reinterpret_cast<float*>(lds + wave * 16384);
+  static_assert(WN == 64 && WAVES * 16384 <= 4 * STAGE, "a wave's 64 x 64 block of sums in LDS");
+#pragma unroll
+  for (int h = 0; h < MF / 4; ++h) {
+    asm volatile("" ::: "memory");
+    // 16-byte piece c of row r lies at c ^ (r & 15): the sixteen rows of a store fall on different banks
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < NF; ++j)
+        *reinterpret_cast<f32x4*>(own + (i * 16 + (lane & 15)) * 64 + (((j * 4 + (lane >> 4)) ^ (lane & 15)) * 4)) = acc[h * 4 + i][j];
+    __builtin_amdgcn_s_waitcnt(0xC07F);        // lgkmcnt(0): the block is this wave's own, no barrier
+    asm volatile("" ::: "memory");
+    write_block<T>(a, own, m0 + wm + h * 64, n0 + wn, lane);
+  }
 }
 
 // the splits' sums, in their order, and the epilogue
@@ -428,10 +551,10 @@ struct Plan {
   int tm, tn, splits, per;
 };
 // 256 x 256 tiles where they fill the chip, 128 x 128 otherwise (two blocks a unit); k is split where even those leave units
-// idle, into parts of eight k tiles at least.
+// idle, into parts of sixteen k tiles (1 KB of a row) at least.
 Plan plan(long M, int N, long K, int esize) {
   Plan p;
-  const long cus = tb_num_cus(), kt = (K * esize + 127) / 128;
+  const long cus = tb_num_cus(), kt = (K * esize + 63) / 64;
   const long big = ((M + 255) / 256) * ((N + 255) / 256);
   p.big = big >= cus;
   const int b = p.big ? 256 : 128;
@@ -441,7 +564,7 @@ Plan plan(long M, int N, long K, int esize) {
   long s = 1;
   if (!p.big && tiles < 2 * cus) {
     s = 2 * cus / tiles;
-    if (s > kt / 8) s = kt / 8;
+    if (s > kt / 16) s = kt / 16;
     if (s > 64) s = 64;
     if (s < 1) s = 1;
   }
@@ -459,7 +582,7 @@ int launch_gemm(const T* P, long ldp, const T* Q, long ldq, long M, int N, long 
   const Plan p = plan(M, N, K, sizeof(T));
   constexpr int CE = 16 / sizeof(T);
   GemmArgs a{P, Q, ldp, ldq, M, N, (int)K, p.tm, p.tn, p.splits, p.per, 0, e};
-  a.four = N % 4 == 0 && aligned(e.y) && aligned(e.z) && aligned(e.bias) && aligned(e.res) && (!e.res || e.ldr % CE == 0);
+  a.four = N % CE == 0 && aligned(e.y) && aligned(e.z) && aligned(e.bias) && aligned(e.res) && (!e.res || e.ldr % CE == 0);
   a.e.slab = p.splits > 1 ? slab : nullptr;
   const dim3 grid(p.tm * p.tn, p.splits);
   if (p.big) gemm_nt<T, 256, 256, 128, 64><<<grid, 512, 0, s>>>(a);
