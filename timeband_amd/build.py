@@ -70,7 +70,7 @@ def _build(objdir, LIB, FLAGS, verbose, jobs):
 
 
 EXT = os.path.join(HERE, "_tbext.so")
-EXT_SRC = os.path.join(CSRC, "ext.cpp")
+EXT_SRC = [os.path.join(CSRC, f) for f in ("ext.cpp", "ext_ssm.cpp")]
 
 
 def ext_needs_build():
@@ -78,11 +78,11 @@ def ext_needs_build():
         return True
     t = os.path.getmtime(EXT)
     hdr = os.path.join(os.path.dirname(HERE), "include", "timeband_hip.h")
-    return any(os.path.getmtime(d) > t for d in (EXT_SRC, hdr))
+    return any(os.path.getmtime(d) > t for d in (*EXT_SRC, hdr))
 
 
 def build_ext(force=False, verbose=True):
-    """The thin PyTorch-ROCm C++ extension (csrc/ext.cpp: torch::autograd::Functions over the C-ABI) -> timeband_amd/_tbext.so.
+    """The thin PyTorch-ROCm C++ extension (csrc/ext.cpp, csrc/ext_ssm.cpp: torch::autograd::Functions over the C-ABI) -> timeband_amd/_tbext.so.
     Host C++ only (g++): it contains no kernels and links against libtimeband_hip.so next to it."""
     if not force and not ext_needs_build():
         return EXT
@@ -95,7 +95,7 @@ def build_ext(force=False, verbose=True):
     cxx = shutil.which("g++") or "g++"
     cmd = [cxx, "-O2", "-fPIC", "-shared", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-sign-compare",
            "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_tbext", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, EXT_SRC, "-o", EXT,
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, *EXT_SRC, "-o", EXT,
            f"-L{tlib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
            f"-L{HERE}", "-l:libtimeband_hip.so", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"]
     if verbose:

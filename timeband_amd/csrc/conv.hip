@@ -36,6 +36,30 @@ __device__ __forceinline__ void load_x(const ConvArgs& a, int b, long t, int len
   }
 }
 
+// the taps of VEC channels: K VEC neighbouring values, fetched whole where the channels are (the caller has seen to the
+// alignment of w and bias then)
+template <typename T, int K, int VEC>
+__device__ __forceinline__ void load_par(const void* w, const void* bias, int f32, int c, float (&r)[K][VEC], float (&b)[VEC]) {
+  float flat[K * VEC];
+  if constexpr (VEC == 1) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) flat[k] = tb_load_par<T>(w, (long)c * K + k, f32);
+    b[0] = bias ? tb_load_par<T>(bias, c, f32) : 0.f;
+  } else {
+    if (f32) tb_load_n(static_cast<const float*>(w) + (long)c * K, flat);
+    else tb_load_n(static_cast<const T*>(w) + (long)c * K, flat);
+    if (!bias) {
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) b[i] = 0.f;
+    } else if (f32) tb_load_n(static_cast<const float*>(bias) + c, b);
+    else tb_load_n(static_cast<const T*>(bias) + c, b);
+  }
+#pragma unroll
+  for (int i = 0; i < VEC; ++i)
+#pragma unroll
+    for (int k = 0; k < K; ++k) r[k][i] = flat[i * K + k];
+}
+
 // block: blockDim.x channel groups of VEC by blockDim.y runs
 template <typename T, int K, int VEC>
 __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
@@ -46,12 +70,7 @@ __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
   const int t0 = q * a.run, t1 = min(t0 + a.run, a.T);
   float w[K][VEC], bias[VEC], win[K][VEC];
-#pragma unroll
-  for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-    for (int k = 0; k < K; ++k) w[k][i] = tb_load_par<T>(a.w, (long)(c + i) * K + k, a.wf32);
-    bias[i] = a.bias ? tb_load_par<T>(a.bias, c + i, a.wf32) : 0.f;
-  }
+  load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
   T* y = static_cast<T*>(a.y) + ((long)b * a.T) * a.D + c;
@@ -98,15 +117,11 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
     const int t0 = q * a.run, t1 = min(t0 + a.run, a.T);
     float w[K][VEC], bias[VEC], win[K][VEC], dp[K][VEC];   // win: x[s-K+1 .. s]; dp: dpre[s-K+1 .. s]
+    load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
+    for (int i = 0; i < VEC; ++i)
 #pragma unroll
-      for (int k = 0; k < K; ++k) {
-        w[k][i] = tb_load_par<T>(a.w, (long)(c + i) * K + k, a.wf32);
-        dp[k][i] = 0.f;
-      }
-      bias[i] = a.bias ? tb_load_par<T>(a.bias, c + i, a.wf32) : 0.f;
-    }
+      for (int k = 0; k < K; ++k) dp[k][i] = 0.f;
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
     const T* dy = static_cast<const T*>(a.dy) + (long)b * a.T * a.D + c;
@@ -220,15 +235,16 @@ __global__ void __launch_bounds__(256) conv_step(ConvStepArgs a) {
   if (id >= (long)a.B * groups) return;
   const int b = (int)(id / groups), c = (int)(id % groups) * VEC;
   T* st = static_cast<T*>(a.state) + b * a.ssb + c;
-  float win[K][VEC], o[VEC];
+  float win[K][VEC], w[K][VEC], bias[VEC], o[VEC];
+  load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) tb_load_n(st + (long)k * a.D, win[k]);
   tb_load_n(static_cast<const T*>(a.x) + b * a.sxb + c, win[K - 1]);
 #pragma unroll
   for (int i = 0; i < VEC; ++i) {
-    float s = a.bias ? tb_load_par<T>(a.bias, c + i, a.wf32) : 0.f;
+    float s = bias[i];
 #pragma unroll
-    for (int k = 0; k < K; ++k) s = fmaf(tb_load_par<T>(a.w, (long)(c + i) * K + k, a.wf32), win[k][i], s);
+    for (int k = 0; k < K; ++k) s = fmaf(w[k][i], win[k][i], s);
     o[i] = a.act == TB_ACT_SILU ? tb_silu(s) : s;
   }
 #pragma unroll
@@ -348,8 +364,8 @@ int tb_conv_fwd(const void* x, long x_batch_stride, long x_step_stride, const vo
   if (rc) return rc;
   if (B == 0 || (T == 0 && !state_out)) return TB_OK;
   if (!w || (T > 0 && (!x || !y))) return tb_set_error(TB_ERR_ARG, "conv_fwd: null pointer");
-  const void* ptrs[] = {x, y, state, state_out};
-  const bool vec = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 4);
+  const void* ptrs[] = {x, y, state, state_out, w, bias};
+  const bool vec = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 6);
   const Plan p = plan(B, T > 0 ? T : 1, D, vec ? (dtype == TB_F32 ? 4 : 8) : 1);
   rc = check_grid("conv_fwd", p);
   if (rc) return rc;
@@ -375,8 +391,8 @@ int tb_conv_bwd(const void* dy, const void* x, long x_batch_stride, long x_step_
   if (B < 1 || T < 1) return tb_set_error(TB_ERR_ARG, "conv_bwd: an empty batch has no gradients to form here");
   if (!dy || !x || !w || !dx || !ws) return tb_set_error(TB_ERR_ARG, "conv_bwd: null pointer");
   if (ws_bytes < tb_conv_bwd_workspace_bytes(B, T, D, K, dtype)) return tb_set_error(TB_ERR_WORKSPACE, "conv_bwd: workspace too small");
-  const void* ptrs[] = {x, dy, dx, state};
-  const bool vec = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 4);
+  const void* ptrs[] = {x, dy, dx, state, w, bias};
+  const bool vec = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 6);
   const Plan p = plan(B, T, D, vec ? (dtype == TB_F32 ? 4 : 8) : 1);
   rc = check_grid("conv_bwd", p);
   if (rc) return rc;
@@ -403,8 +419,8 @@ int tb_conv_step(const void* x, long x_batch_stride, void* state, long state_bat
   if (rc) return rc;
   if (B == 0) return TB_OK;
   if (!x || !w || !y || (K > 1 && !state)) return tb_set_error(TB_ERR_ARG, "conv_step: null pointer");
-  const void* ptrs[] = {x, y, state};
-  const bool vec = can_vec(dtype, D, x_batch_stride, state_batch_stride, ptrs, 3);
+  const void* ptrs[] = {x, y, state, w, bias};
+  const bool vec = can_vec(dtype, D, x_batch_stride, state_batch_stride, ptrs, 5);
   ConvStepArgs a{x, w, bias, state, y, x_batch_stride, state_batch_stride, B, D, act, w_f32};
   by_shape(dtype, K, vec, StepLaunch{a, static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("conv_step");

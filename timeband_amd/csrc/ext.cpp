@@ -17,7 +17,6 @@
 #include <memory>
 #include <mutex>
 #include <unordered_map>
-#include <unordered_set>
 #include <vector>
 
 #include "timeband_hip.h"
@@ -415,49 +414,13 @@ Tensor linear_act(Tensor x, Tensor W, OptT b, int64_t act, OptT s_W, OptT s_b, O
 
 Tensor linear_act_raw_py(Tensor x, Tensor W, OptT b, int64_t act) { return linear_act_raw(x, W, opt(b), act); }
 
-// A backward pass ends by making its stream wait for the streams that its leaves' accumulation nodes were made on.  Under
-// capture such a node from outside (an eager graph of the same leaf that somebody still holds) ties the capture to work
-// that is not part of it, and the process ends inside the runtime when the capture does.  Refused here, before anything is
-// recorded: every accumulation node behind `inputs` has to be of the capturing stream.
-void check_capture(std::vector<OptT> inputs) {
-  hipStreamCaptureStatus status;
-  std::vector<torch::autograd::Node*> todo;
-  std::unordered_set<torch::autograd::Node*> seen;
-  std::vector<std::shared_ptr<torch::autograd::Node>> held;
-  c10::optional<c10::hip::HIPStream> cur;
-  for (const OptT& t : inputs) {
-    if (!t.has_value() || !t->defined() || !t->requires_grad()) continue;
-    if (!cur) {
-      cur = c10::hip::getCurrentHIPStream(t->get_device());
-      C10_HIP_CHECK(hipStreamIsCapturing(cur->stream(), &status));
-      if (status == hipStreamCaptureStatusNone) return;
-    }
-    auto n = t->is_leaf() ? torch::autograd::impl::try_get_grad_accumulator(*t) : t->grad_fn();
-    if (n && seen.insert(n.get()).second) {
-      todo.push_back(n.get());
-      held.push_back(std::move(n));
-    }
-  }
-  while (!todo.empty()) {
-    torch::autograd::Node* n = todo.back();
-    todo.pop_back();
-    if (n->next_edges().empty() && n->num_inputs() == 1 && n->name() == "torch::autograd::AccumulateGrad") {
-      const auto s = n->stream();
-      TORCH_CHECK(!s.has_value() || s->id() == cur->unwrap().id(),
-                  "timeband_amd: a backward pass cannot be captured while an autograd graph of the same leaf, made outside the "
-                  "capture, is alive: drop (or detach) what earlier calls returned");
-    }
-    for (const auto& e : n->next_edges())
-      if (e.function && seen.insert(e.function.get()).second) todo.push_back(e.function.get());
-  }
-}
-
 }  // namespace
+
+void tb_bind_ssm(py::module_& m);      // ext_ssm.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "timeband_amd: autograd Functions over libtimeband_hip.so (C-ABI include/timeband_hip.h)";
   m.def("set_runtime", &set_runtime);
-  m.def("check_capture", &check_capture);
   m.def("clustered_begin", &clustered_begin);
   m.def("clustered_end", &clustered_end);
   m.def("set_grads_hook", &set_grads_hook);
@@ -470,4 +433,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("linear_act", &linear_act, py::arg("x"), py::arg("W"), py::arg("b"), py::arg("act") = 0, py::arg("s_W") = py::none(),
         py::arg("s_b") = py::none(), py::arg("pre") = py::none());
   m.def("linear_act_raw", &linear_act_raw_py);
+  tb_bind_ssm(m);
 }

@@ -556,6 +556,7 @@ struct StepArgs {
   void* out;
   long sub, sdb, szb, sBb, sBg, sCb, sCg, ssb;
   int B, D, N, G, Dg, softplus;
+  int vec, vecbc;      // whole rows of 4 S states, and of B and C, on 16 bytes
 };
 
 // one step: reads and writes each state once.  Lanes as above: four a channel.
@@ -567,7 +568,7 @@ __global__ void __launch_bounds__(256) scan_step(StepArgs a) {
   const int b = on ? (int)(id / a.D) : 0, d = on ? (int)(id % a.D) : 0, g = d / a.Dg;
   float* st = a.state + b * a.ssb + (long)d * a.N;
   float h[S], A[S], bv[S], cv[S];
-  const bool whole = a.N == 4 * S && (a.ssb & 3) == 0 && (reinterpret_cast<uintptr_t>(a.state) & 15) == 0 && (reinterpret_cast<uintptr_t>(a.A) & 15) == 0;
+  const bool whole = a.vec;
   if (whole) {
     tb_load_n(st + n0, h);
     tb_load_n(a.A + (long)d * a.N + n0, A);
@@ -579,8 +580,14 @@ __global__ void __launch_bounds__(256) scan_step(StepArgs a) {
       h[s] = in ? st[n0 + s] : 0.f;
       A[s] = in ? a.A[(long)d * a.N + n0 + s] : 0.f;
     }
-    bv[s] = in ? (float)static_cast<const T*>(a.Bm)[b * a.sBb + g * a.sBg + n0 + s] : 0.f;
-    cv[s] = in ? (float)static_cast<const T*>(a.Cm)[b * a.sCb + g * a.sCg + n0 + s] : 0.f;
+    if (!a.vecbc) {
+      bv[s] = in ? (float)static_cast<const T*>(a.Bm)[b * a.sBb + g * a.sBg + n0 + s] : 0.f;
+      cv[s] = in ? (float)static_cast<const T*>(a.Cm)[b * a.sCb + g * a.sCg + n0 + s] : 0.f;
+    }
+  }
+  if (a.vecbc) {
+    tb_load_n(static_cast<const T*>(a.Bm) + b * a.sBb + g * a.sBg + n0, bv);
+    tb_load_n(static_cast<const T*>(a.Cm) + b * a.sCb + g * a.sCg + n0, cv);
   }
   const float u = (float)static_cast<const T*>(a.u)[b * a.sub + d];
   float dl = (float)static_cast<const T*>(a.dt)[b * a.sdb + d] + (a.bias ? a.bias[d] : 0.f);
@@ -809,8 +816,11 @@ int tb_scan_step(float* state, long state_batch_stride, const void* u, const voi
   if (!state || !u || !dt || !Bm || !Cm || !strides || !A || !out) return tb_set_error(TB_ERR_ARG, "scan_step: null pointer");
   const long* q = strides;
   StepArgs a{state, u, dt, z, Bm, Cm, A, Dp, dt_bias, out, q[0], q[1], q[2], q[3], q[4], q[5], q[6], state_batch_stride,
-             B, D, N, G, D / G, softplus};
-  by_shape(dtype, states_per_lane(N), StepLaunch{a, static_cast<hipStream_t>(stream)});
+             B, D, N, G, D / G, softplus, 0, 0};
+  const int S = states_per_lane(N), v = dtype == TB_F32 ? 4 : 8;
+  a.vec = N == 4 * S && state_batch_stride % 4 == 0 && aligned(state) && aligned(A);
+  a.vecbc = N == 4 * S && N % v == 0 && aligned(Bm) && aligned(Cm) && q[3] % v == 0 && q[4] % v == 0 && q[5] % v == 0 && q[6] % v == 0;
+  by_shape(dtype, S, StepLaunch{a, static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("scan_step");
   return TB_OK;
 }

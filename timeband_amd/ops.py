@@ -6,10 +6,7 @@ libtimeband_hip.so; there is no eager/CPU fallback -- a CPU tensor raises.
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib, dp
 
@@ -540,257 +537,36 @@ def linear_act(x2d, W, b, act=ACT_NONE, pre=None):
 
 # ----------------------------------------------------------------------------------------------
 # State space layer: causal convolution, selective scan, linear with residual.  fp32, bf16 or fp16 tensors (one type a call),
-# parameters of the scan fp32.  Workspaces come from torch's allocator call by call, not from Runtime.workspace: these
-# operators may be captured into a graph, and a captured address must not be handed to another call meanwhile.
+# parameters of the scan fp32.  Checks, workspaces and autograd Functions are the extension's (csrc/ext_ssm.cpp), whatever
+# TB_EXT says: that variable chooses between two forms of the operators above, and these have one.
 # ----------------------------------------------------------------------------------------------
-_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+_SSM = None
 
 
-def _ssm_check(what, lead, *others):
-    """Device and element type of a call: the code of the type; raises where a tensor is elsewhere or of another type."""
-    for t in (lead, *others):
-        if t is None:
-            continue
-        if not t.is_cuda:
-            _need_cuda(t)
-        if t.device != lead.device:
-            raise RuntimeError(f"{what}: tensors are on {lead.device} and {t.device}")
-        if t.dtype != lead.dtype:
-            raise RuntimeError(f"{what}: expected {lead.dtype} throughout, got {t.dtype}")
-    code = _DTYPES.get(lead.dtype)
-    if code is None:
-        raise RuntimeError(f"{what}: {lead.dtype} is not supported (float32, bfloat16, float16)")
-    Runtime.get(lead.device)         # loads the library and refuses other devices than gfx950, once
-    return code
-
-
-def _par32(what, t, shape, device):
-    """An fp32 parameter of the scan, dense."""
-    if t is None:
-        return None
-    if t.dtype != torch.float32 or tuple(t.shape) != tuple(shape) or t.device != device:
-        raise RuntimeError(f"{what}: expected float32 {tuple(shape)} on {device}, got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t if t.is_contiguous() else t.contiguous()
-
-
-def _shape(what, t, shape):
-    if t is not None and tuple(t.shape) != tuple(shape):
-        raise RuntimeError(f"{what}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-
-
-def _last_dense(t):
-    return t if t is None or t.shape[-1] <= 1 or t.stride(-1) == 1 else t.contiguous()
-
-
-def _lengths(what, lengths, B, device):
-    if lengths is None:
-        return None
-    if lengths.dtype != torch.int32 or tuple(lengths.shape) != (B,) or lengths.device != device:
-        raise RuntimeError(f"{what}: lengths must be int32 ({B},) on {device}")
-    return lengths if lengths.is_contiguous() else lengths.contiguous()
-
-
-class _on:
-    """The device of a call, made current while it launches (nothing to do where it is already)."""
-
-    def __init__(self, device):
-        self.want = device.index
-
-    def __enter__(self):
-        self.was = torch.cuda.current_device()
-        if self.was != self.want:
-            torch.cuda.set_device(self.want)
-
-    def __exit__(self, *exc):
-        if self.was != self.want:
-            torch.cuda.set_device(self.was)
-
-
-def _bytes(n, device):
-    return torch.empty(n, dtype=torch.uint8, device=device)
-
-
-def _grad_wanted(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
-
-
-def _graph_wanted(*ts):
-    """_grad_wanted for an operator about to make its autograd node: under capture, refuses what would end the process."""
-    if not _grad_wanted(*ts):
-        return False
-    if torch.cuda.is_current_stream_capturing():
-        ext = _load_ext()
-        if ext is not None:
-            ext.check_capture(list(ts))
-    return True
-
-
-def _no_grad_here(what, *ts):
-    if _grad_wanted(*ts):
-        raise RuntimeError(f"{what} updates its state in place and has no gradient: call it under torch.no_grad()")
-
-
-class _ConvFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias, act, state, lengths, want_state):
-        B, T, D = x.shape
-        K = weight.shape[1]
-        code = _DTYPES[x.dtype]
-        wf32 = int(weight.dtype == torch.float32)
-        with _on(x.device):
-            y = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
-            new = torch.empty(B, K - 1, D, dtype=x.dtype, device=x.device) if want_state else None
-            _lib.call("tb_conv_fwd", _ptr(x), x.stride(0), x.stride(1), _ptr(weight), _ptr(bias), wf32, _ptr(state), _ptr(lengths),
-                      _ptr(y), _ptr(new), B, T, D, K, act, code, _stream(x.device.index))
-        ctx.save_for_backward(x, weight, bias, state, lengths)
-        ctx.act = act
-        ctx.set_materialize_grads(False)
-        if new is not None:
-            ctx.mark_non_differentiable(new)
-        return y, new
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, _dnew):
-        if dy is None:
-            return (None,) * 7
-        x, weight, bias, state, lengths = ctx.saved_tensors
-        B, T, D = x.shape
-        K = weight.shape[1]
-        need = ctx.needs_input_grad
-        if B == 0 or T == 0:
-            return (torch.zeros_like(x) if need[0] else None, torch.zeros_like(weight) if need[1] else None,
-                    torch.zeros_like(bias) if need[2] else None, None, None, None, None)
-        code = _DTYPES[x.dtype]
-        dy = dy.contiguous()
-        with _on(x.device):
-            dx = torch.empty(B, T, D, dtype=x.dtype, device=x.device)
-            dw = torch.empty(D, K, dtype=weight.dtype, device=x.device) if need[1] else None
-            db = torch.empty(D, dtype=bias.dtype, device=x.device) if need[2] else None
-            ws = _bytes(_lib.load().tb_conv_bwd_workspace_bytes(B, T, D, K, code), x.device)
-            _lib.call("tb_conv_bwd", _ptr(dy), _ptr(x), x.stride(0), x.stride(1), _ptr(weight), _ptr(bias),
-                      int(weight.dtype == torch.float32), _ptr(state), _ptr(lengths), _ptr(dx), _ptr(dw), _ptr(db), B, T, D, K,
-                      ctx.act, code, _ptr(ws), ws.numel(), _stream(x.device.index))
-        return dx if need[0] else None, dw, db, None, None, None, None
-
-
-def _conv_params(what, weight, bias, D, x):
-    if weight.dim() != 2 or weight.shape[0] != D:
-        raise RuntimeError(f"{what}: weight must be ({D}, taps), got {tuple(weight.shape)}")
-    for t in (weight, bias):
-        if t is not None and (t.device != x.device or t.dtype not in (torch.float32, x.dtype) or t.dtype != weight.dtype):
-            raise RuntimeError(f"{what}: weight and bias must both be {x.dtype} or both float32, on {x.device}")
-    _shape(f"{what}: bias", bias, (D,))
-    return weight.contiguous(), None if bias is None else bias.contiguous()
+def _ssm():
+    global _SSM
+    if _SSM is None:
+        _lib.load()
+        try:
+            from . import _tbext
+        except ImportError as e:
+            raise RuntimeError("timeband_amd/_tbext.so is missing: build it with `python -m timeband_amd.build`") from e
+        _SSM = _tbext
+    return _SSM
 
 
 def causal_conv(x, weight, bias=None, act=ACT_NONE, state=None, lengths=None, return_state=False):
     """Depthwise causal convolution of x (B,T,D) along its steps: act(bias + sum_k weight[:,k] x[t-K+1+k]), weight (D,K) with
-    1 to 8 taps, act ACT_NONE or ACT_SILU.  state (B,K-1,D): the inputs before step 0 (zero without); lengths (B,) int32: steps
-    at or behind a sequence's length are not read and give zero.  return_state: also the last K-1 inputs of each sequence, for
-    the next call or causal_conv_step (no gradient runs through either state)."""
-    _ssm_check("causal_conv", x, state)
-    if x.dim() != 3:
-        raise RuntimeError("causal_conv: x must be (B, T, D)")
-    B, T, D = x.shape
-    weight, bias = _conv_params("causal_conv", weight, bias, D, x)
-    _shape("causal_conv: state", state, (B, weight.shape[1] - 1, D))
-    if _grad_wanted(state):
-        raise RuntimeError("causal_conv: no gradient runs through the state (detach it)")
-    lengths = _lengths("causal_conv", lengths, B, x.device)
-    _graph_wanted(x, weight, bias)
-    y, new = _ConvFn.apply(_last_dense(x), weight, bias, int(act), None if state is None else state.contiguous(), lengths,
-                           bool(return_state))
-    return (y, new) if return_state else y
+    1 to 8 taps, act ACT_NONE or ACT_SILU; weight and bias of x's type or float32.  state (B,K-1,D): the inputs before step 0
+    (zero without); lengths (B,) int32: steps at or behind a sequence's length are not read and give zero.  return_state: also
+    the last K-1 inputs of each sequence, for the next call or causal_conv_step (no gradient runs through either state)."""
+    return (_SSM or _ssm()).causal_conv(x, weight, bias, act, state, lengths, return_state)
 
 
 def causal_conv_step(x, state, weight, bias=None, act=ACT_NONE):
-    """causal_conv for one step: x (B,D) -> (B,D).  state (B,K-1,D), rows dense, is shifted and takes x, IN PLACE."""
-    code = _ssm_check("causal_conv_step", x, state)
-    if x.dim() != 2:
-        raise RuntimeError("causal_conv_step: x must be (B, D)")
-    B, D = x.shape
-    weight, bias = _conv_params("causal_conv_step", weight, bias, D, x)
-    K = weight.shape[1]
-    _shape("causal_conv_step: state", state, (B, K - 1, D))
-    _no_grad_here("causal_conv_step", x, state, weight, bias)
-    if K > 1 and not state[0:1].is_contiguous():
-        raise RuntimeError("causal_conv_step: the rows of state must be dense (it is updated in place)")
-    if B > 1 and state.stride(0) < (K - 1) * D:
-        raise RuntimeError("causal_conv_step: the rows of state overlap")
-    x = _last_dense(x)
-    with _on(x.device):
-        y = torch.empty(B, D, dtype=x.dtype, device=x.device)
-        _lib.call("tb_conv_step", _ptr(x), x.stride(0), _ptr(state), state.stride(0), _ptr(weight), _ptr(bias),
-                  int(weight.dtype == torch.float32), _ptr(y), B, D, K, int(act), code, _stream(x.device.index))
-    return y
-
-
-def _longs(*v):
-    return (ctypes.c_long * len(v))(*v)
-
-
-class _ScanFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, u, dt, A, Bm, Cm, D, z, dt_bias, h0, lengths, softplus, want_state, train):
-        B, T, Dn = u.shape
-        G, N = Bm.shape[2:]
-        code = _DTYPES[u.dtype]
-        lib = _lib.load()
-        dev = u.device
-        strides = (u.stride(0), u.stride(1), dt.stride(0), dt.stride(1), *((z.stride(0), z.stride(1)) if z is not None else (0, 0)),
-                   *Bm.stride()[:3], *Cm.stride()[:3])
-        states = None
-        with _on(dev):
-            out = torch.empty(B, T, Dn, dtype=u.dtype, device=dev)
-            hT = torch.empty(B, Dn, N, dtype=torch.float32, device=dev) if want_state else None
-            if B and T:
-                if train:
-                    states = _bytes(lib.tb_scan_states_bytes(B, T, Dn, N), dev)
-                ws = _bytes(lib.tb_scan_workspace_bytes(B, T, Dn, N, G, 0), dev)
-                _lib.call("tb_scan_fwd", _ptr(u), _ptr(dt), _ptr(z), _ptr(Bm), _ptr(Cm), _longs(*strides), _ptr(A), _ptr(D),
-                          _ptr(dt_bias), softplus, _ptr(h0), _ptr(lengths), _ptr(out), _ptr(hT), _ptr(states), B, T, Dn, N, G, code,
-                          _ptr(ws), ws.numel(), _stream(dev.index))
-            elif hT is not None:
-                hT.copy_(h0) if h0 is not None else hT.zero_()
-        if train:
-            ctx.save_for_backward(u, dt, A, Bm, Cm, D, z, dt_bias, lengths, states)
-            ctx.rest = (strides, softplus)
-        ctx.set_materialize_grads(False)
-        return out, hT
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dout, dhT):
-        if dout is None and dhT is None:
-            return (None,) * 13
-        u, dt, A, Bm, Cm, D, z, dt_bias, lengths, states = ctx.saved_tensors
-        strides, softplus = ctx.rest
-        B, T, Dn = u.shape
-        G, N = Bm.shape[2:]
-        need = ctx.needs_input_grad
-        dev = u.device
-        lib = _lib.load()
-        with _on(dev):
-            if not (B and T):
-                g = [torch.zeros_like(t) if (t is not None and n) else None
-                     for t, n in zip((u, dt, A, Bm, Cm, D, z, dt_bias), need)]
-                dh0 = None
-                if need[8]:
-                    dh0 = dhT.clone() if dhT is not None else torch.zeros(B, Dn, N, dtype=torch.float32, device=dev)
-                return (*g, dh0, None, None, None, None)
-            dout = torch.zeros(B, T, Dn, dtype=u.dtype, device=dev) if dout is None else _last_dense(dout)
-            dhT = None if dhT is None else dhT.contiguous()
-            like = lambda t, n: torch.empty(t.shape, dtype=t.dtype, device=dev) if (t is not None and n) else None
-            g = [like(t, n) for t, n in zip((u, dt, A, Bm, Cm, D, z, dt_bias), need)]
-            dh0 = torch.empty(B, Dn, N, dtype=torch.float32, device=dev) if need[8] else None
-            du, ddt, dA, dB, dC, dD, dz, dbias = g
-            ws = _bytes(lib.tb_scan_workspace_bytes(B, T, Dn, N, G, 1), dev)
-            _lib.call("tb_scan_bwd", _ptr(dout), _ptr(u), _ptr(dt), _ptr(z), _ptr(Bm), _ptr(Cm),
-                      _longs(*strides, dout.stride(0), dout.stride(1)), _ptr(A), _ptr(D), _ptr(dt_bias), softplus, _ptr(lengths),
-                      _ptr(states), _ptr(dhT), _ptr(du), _ptr(ddt), _ptr(dz), _ptr(dB), _ptr(dC), _ptr(dA), _ptr(dD), _ptr(dbias),
-                      _ptr(dh0), B, T, Dn, N, G, _DTYPES[u.dtype], _ptr(ws), ws.numel(), _stream(dev.index))
-        return (*g, dh0, None, None, None, None)
+    """causal_conv for one step: x (B,D) -> (B,D).  state (B,K-1,D), rows dense, is shifted and takes x, IN PLACE.  No
+    gradient: refused where one would be recorded."""
+    return (_SSM or _ssm()).causal_conv_step(x, state, weight, bias, act)
 
 
 def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, h0=None, lengths=None, return_state=False):
@@ -801,127 +577,22 @@ def selective_scan(u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True, 
 
     dt, z like u; B, C (B,T,N) or (B,T,G,N) with G groups of D/G channels, 1 to 64 states N; A (D,N), D and dt_bias (D,) fp32;
     h0 (B,D,N) fp32, zero without; lengths (B,) int32: steps at or behind a sequence's length leave the state as it is and
-    give zero.  return_state: also the state behind each sequence's last step, (B,D,N) fp32.  Differentiable in every tensor,
-    the states included."""
-    _ssm_check("selective_scan", u, dt, B, C, z)
-    if u.dim() != 3:
-        raise RuntimeError("selective_scan: u must be (B, T, D)")
-    Bn, T, Dn = u.shape
-    _shape("selective_scan: dt", dt, u.shape)
-    _shape("selective_scan: z", z, u.shape)
-    if B.dim() == 3:
-        B = B.unsqueeze(2)
-    if C.dim() == 3:
-        C = C.unsqueeze(2)
-    if B.dim() != 4 or tuple(B.shape[:2]) != (Bn, T) or C.shape != B.shape:
-        raise RuntimeError(f"selective_scan: B and C must be ({Bn}, {T}, N) or ({Bn}, {T}, G, N)")
-    G, N = B.shape[2:]
-    if G < 1 or Dn % G:
-        raise RuntimeError(f"selective_scan: {Dn} channels do not divide into {G} groups")
-    A = _par32("selective_scan: A", A, (Dn, N), u.device)
-    D = _par32("selective_scan: D", D, (Dn,), u.device)
-    dt_bias = _par32("selective_scan: dt_bias", dt_bias, (Dn,), u.device)
-    h0 = _par32("selective_scan: h0", h0, (Bn, Dn, N), u.device)
-    lengths = _lengths("selective_scan", lengths, Bn, u.device)
-    out, hT = _ScanFn.apply(_last_dense(u), _last_dense(dt), A, _last_dense(B), _last_dense(C), D, _last_dense(z), dt_bias, h0,
-                            lengths, int(bool(softplus)), bool(return_state), _graph_wanted(u, dt, A, B, C, D, z, dt_bias, h0))
-    return (out, hT) if return_state else out
+    give zero.  return_state: also the state behind each sequence's last step, (B,D,N) fp32.  Differentiable (once) in every
+    tensor, the states included."""
+    return (_SSM or _ssm()).selective_scan(u, dt, A, B, C, D, z, dt_bias, softplus, h0, lengths, return_state)
 
 
 def selective_scan_step(state, u, dt, A, B, C, D=None, z=None, dt_bias=None, softplus=True):
     """selective_scan for one step: u, dt, z (B,D), B, C (B,N) or (B,G,N) -> (B,D).  state (B,D,N) fp32, rows dense, is
-    updated IN PLACE."""
-    code = _ssm_check("selective_scan_step", u, dt, B, C, z)
-    if u.dim() != 2:
-        raise RuntimeError("selective_scan_step: u must be (B, D)")
-    Bn, Dn = u.shape
-    _shape("selective_scan_step: dt", dt, u.shape)
-    _shape("selective_scan_step: z", z, u.shape)
-    if B.dim() == 2:
-        B = B.unsqueeze(1)
-    if C.dim() == 2:
-        C = C.unsqueeze(1)
-    if B.dim() != 3 or B.shape[0] != Bn or C.shape != B.shape:
-        raise RuntimeError(f"selective_scan_step: B and C must be ({Bn}, N) or ({Bn}, G, N)")
-    G, N = B.shape[1:]
-    if G < 1 or Dn % G:
-        raise RuntimeError(f"selective_scan_step: {Dn} channels do not divide into {G} groups")
-    A = _par32("selective_scan_step: A", A, (Dn, N), u.device)
-    D = _par32("selective_scan_step: D", D, (Dn,), u.device)
-    dt_bias = _par32("selective_scan_step: dt_bias", dt_bias, (Dn,), u.device)
-    if state.dtype != torch.float32 or tuple(state.shape) != (Bn, Dn, N) or state.device != u.device:
-        raise RuntimeError(f"selective_scan_step: state must be float32 ({Bn}, {Dn}, {N}) on {u.device}")
-    _no_grad_here("selective_scan_step", state, u, dt, A, B, C, D, z, dt_bias)
-    if not state[0:1].is_contiguous():
-        raise RuntimeError("selective_scan_step: the rows of state must be dense (it is updated in place)")
-    if Bn > 1 and state.stride(0) < Dn * N:
-        raise RuntimeError("selective_scan_step: the rows of state overlap")
-    u, dt, z, B, C = (_last_dense(t) for t in (u, dt, z, B, C))
-    with _on(u.device):
-        out = torch.empty(Bn, Dn, dtype=u.dtype, device=u.device)
-        _lib.call("tb_scan_step", _ptr(state), state.stride(0), _ptr(u), _ptr(dt), _ptr(z), _ptr(B), _ptr(C),
-                  _longs(u.stride(0), dt.stride(0), 0 if z is None else z.stride(0), B.stride(0), B.stride(1), C.stride(0), C.stride(1)),
-                  _ptr(A), _ptr(D), _ptr(dt_bias), int(bool(softplus)), _ptr(out), Bn, Dn, N, G, code, _stream(u.device.index))
-    return out
-
-
-class _LinResFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, W, b, act, residual, train):
-        M, K = x.shape
-        N = W.shape[0]
-        code = _DTYPES[x.dtype]
-        with _on(x.device):
-            y = torch.empty(M, N, dtype=x.dtype, device=x.device)
-            z = torch.empty(M, N, dtype=torch.float32, device=x.device) if train and act else None
-            ws = _bytes(_lib.load().tb_linres_workspace_bytes(M, K, N, code, 0), x.device)
-            _lib.call("tb_linres_fwd", _ptr(x), x.stride(0), _ptr(W), W.stride(0), _ptr(b), _ptr(residual),
-                      0 if residual is None else residual.stride(0), _ptr(y), _ptr(z), M, K, N, act, code, _ptr(ws), ws.numel(),
-                      _stream(x.device.index))
-        if train:
-            ctx.save_for_backward(x, W, z)
-            ctx.act = act
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        need = ctx.needs_input_grad
-        dres = dy if need[4] else None
-        if not any(need[:3]):
-            return None, None, None, None, dres, None
-        x, W, z = ctx.saved_tensors
-        M, K = x.shape
-        N = W.shape[0]
-        code = _DTYPES[x.dtype]
-        with _on(x.device):
-            new = torch.empty if M else torch.zeros
-            dx = new(M, K, dtype=x.dtype, device=x.device) if need[0] else None
-            dW = new(N, K, dtype=x.dtype, device=x.device) if need[1] else None
-            db = new(N, dtype=x.dtype, device=x.device) if need[2] else None
-            if M:
-                dy = _last_dense(dy)
-                ws = _bytes(_lib.load().tb_linres_workspace_bytes(M, K, N, code, 1), x.device)
-                _lib.call("tb_linres_bwd", _ptr(dy), dy.stride(0), _ptr(x), x.stride(0), _ptr(W), W.stride(0), _ptr(z), ctx.act,
-                          _ptr(dx), _ptr(dW), _ptr(db), M, K, N, code, _ptr(ws), ws.numel(), _stream(x.device.index))
-        return dx, dW, db, None, dres, None
+    updated IN PLACE.  No gradient: refused where one would be recorded."""
+    return (_SSM or _ssm()).selective_scan_step(state, u, dt, A, B, C, D, z, dt_bias, softplus)
 
 
 def linear_residual(x, W, b=None, act=ACT_NONE, residual=None):
     """act(x @ W.T + b) + residual for x (..., K), W (N, K), b (N,), residual (..., N), all of one type (float32, bfloat16 or
-    float16).  fp32 products are exact (linear_act's are split into bf16 parts).  act: any ACT_*."""
-    _ssm_check("linear_residual", x, W, b, residual)
-    if x.dim() < 1 or W.dim() != 2 or W.shape[1] != x.shape[-1] or min(W.shape) < 1:
-        raise RuntimeError(f"linear_residual: weight {tuple(W.shape)} does not match the input {tuple(x.shape)}")
-    N, K = W.shape
-    _shape("linear_residual: b", b, (N,))
-    _shape("linear_residual: residual", residual, (*x.shape[:-1], N))
-    if not ACT_NONE <= int(act) <= ACT_GELU:
-        raise RuntimeError(f"linear_residual: activation {act} is not supported")
-    rows = lambda t, n: None if t is None else _last_dense(t.reshape(-1, n))
-    y = _LinResFn.apply(rows(x, K), _last_dense(W), None if b is None else b.contiguous(), int(act), rows(residual, N),
-                        _graph_wanted(x, W, b, residual) and _grad_wanted(x, W, b))
-    return y.view(*x.shape[:-1], N)
+    float16).  fp32 products are exact (linear_act's are split into bf16 parts).  act: any ACT_*.  Under graph capture, no
+    autograd graph of the same leaves made outside the capture may be alive (refused), as for the operators above."""
+    return (_SSM or _ssm()).linear_residual(x, W, b, act, residual)
 
 
 # ----------------------------------------------------------------------------------------------
