@@ -24,15 +24,17 @@
 namespace {
 
 constexpr int CB = 64;          // channels a block
+constexpr int YS = CB + 16;     // row length of what four lanes store for four rows at once: they fall on different banks
 constexpr int NMAX = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// steps a tile of the backward pass: the states of a tile stay in registers, TT * S = 128 of them at most
+// steps a tile of the backward pass.  The states of a tile stay in registers, BWD * S of them: 64 leave room for three waves
+// a SIMD, 128 for two; a state is kept in memory every BWD steps.
+constexpr int bwd_tile(int S) { return S <= 2 ? 32 : S <= 8 ? 16 : 8; }
 template <int S>
 struct Tile {
-  static constexpr int BWD = S <= 4 ? 32 : S == 8 ? 16 : 8;
+  static constexpr int BWD = bwd_tile(S), WAVES = BWD * S > 64 ? 2 : 3;
 };
-int bwd_tile(int S) { return S <= 4 ? 32 : S == 8 ? 16 : 8; }
 
 struct ScanArgs {
   const void *u, *dt, *z, *Bm, *Cm, *dout;
@@ -70,22 +72,30 @@ __device__ __forceinline__ float quad_sum(float v) {
   return v + dpp<0x4E>(v); // lanes 2 3 0 1
 }
 
-// EPT neighbouring channels of a row; channels behind the group's last and rows that are off read as 0
-template <typename T, int EPT>
-__device__ __forceinline__ void fetch(const void* base, long off, int c0, int Dg, bool vec, bool on, float (&r)[EPT]) {
-  const T* p = static_cast<const T*>(base) + off;
-  if (on && vec && c0 + EPT <= Dg) {
-    tb_load_n(p + c0, r);
-  } else {
+// EPT neighbouring channels of a row as they lie in memory.  The address is always one of the tensor's (the caller clamps the
+// row; channels behind the group's last read another), so that nothing branches and all of a tile's loads are under way at
+// once: converted and masked as each arrived, they were waited for one after the other.
+template <typename T, int EPT, bool VEC>
+struct Raw {
+  T v[EPT];
+  __device__ __forceinline__ void fetch(const void* base, long off, int c0, int Dg) {
+    const T* p = static_cast<const T*>(base) + off;
+    if constexpr (VEC) {
+      constexpr int W = 16 / sizeof(T) < EPT ? 16 / sizeof(T) : EPT;
+      const T* q = p + (c0 < Dg ? c0 : 0);
 #pragma unroll
-    for (int i = 0; i < EPT; ++i) r[i] = on && c0 + i < Dg ? (float)p[c0 + i] : 0.f;
+      for (int i = 0; i < EPT; i += W) *reinterpret_cast<TbVec<T, W>*>(v + i) = *reinterpret_cast<const TbVec<T, W>*>(q + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < EPT; ++i) v[i] = p[min(c0 + i, Dg - 1)];
+    }
   }
-}
-template <typename T, int EPT>
-__device__ __forceinline__ void put(void* base, long off, int c0, int Dg, bool vec, const float (&r)[EPT]) {
+};
+template <typename T, int EPT, bool VEC>
+__device__ __forceinline__ void put(void* base, long off, int c0, int Dg, const float (&r)[EPT]) {
   T* p = static_cast<T*>(base) + off;
-  if (vec && c0 + EPT <= Dg) {
-    tb_store_n(p + c0, r);
+  if constexpr (VEC) {
+    if (c0 < Dg) tb_store_n(p + c0, r);
   } else {
 #pragma unroll
     for (int i = 0; i < EPT; ++i)
@@ -127,23 +137,43 @@ __device__ __forceinline__ void load_row(const float* p, float (&v)[S]) { tb_loa
 template <int S>
 __device__ __forceinline__ void store_row(float* p, const float (&v)[S]) { tb_store_n(p, v); }
 
-// rows of B or C of a tile into LDS as fp32, [TT][4 S], zero behind N and where the step is off
+// rows of B or C of a tile on their way into LDS as fp32, [TT][4 S], zero behind N and where the step is off
 template <typename T, int S, int TT>
-__device__ __forceinline__ void stage_bc(const void* base, long off, long st, int t0, int t1, int N, float* lds) {
-  constexpr int NP = 4 * S;
-  for (int i = threadIdx.x; i < TT * NP; i += 256) {
-    const int t = i / NP, n = i % NP;
-    lds[i] = t0 + t < t1 && n < N ? (float)static_cast<const T*>(base)[off + (long)(t0 + t) * st + n] : 0.f;
+struct RawRows {
+  static constexpr int NP = 4 * S, COUNT = (TT * NP + 255) / 256;
+  T v[COUNT];
+  __device__ __forceinline__ void fetch(const void* base, long off, long st, int t0, int t1, int N) {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      const int i = threadIdx.x + j * 256, t = max(min(t0 + i / NP, t1 - 1), 0), n = min(i % NP, N - 1);
+      v[j] = static_cast<const T*>(base)[off + (long)t * st + n];
+    }
   }
+  __device__ __forceinline__ void store(float* lds, int t0, int t1, int N) const {
+#pragma unroll
+    for (int j = 0; j < COUNT; ++j) {
+      const int i = threadIdx.x + j * 256;
+      if (TT * NP % 256 == 0 || i < TT * NP) lds[i] = t0 + i / NP < t1 && i % NP < N ? (float)v[j] : 0.f;
+    }
+  }
+};
+
+// the sums over the four lanes of a quad of four steps' values: lane l of the quad gets step l's.  Each exchange adds what is
+// left of two values in one instruction behind two selects: nine instructions instead of sixteen and one store instead of four.
+__device__ __forceinline__ float quad_sum4(const float (&y)[4], int lane) {
+  const bool o = lane & 1, h = lane & 2;
+  const float a = (o ? y[1] : y[0]) + dpp<0xB1>(o ? y[0] : y[1]);
+  const float b = (o ? y[3] : y[2]) + dpp<0xB1>(o ? y[2] : y[3]);
+  return (h ? b : a) + dpp<0x4E>(h ? a : b);
 }
 
 // forward.  STATE: only the chunk's end state from zero and its sum of delta (first pass over chunks).
-template <typename T, int S, bool STATE>
+template <typename T, int S, bool STATE, bool VEC>
 __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
   constexpr int TT = 32, EPT = 8, NP = 4 * S;
   __shared__ float sD[TT][CB][2];            // delta, delta u
   __shared__ float sB[TT * NP], sC[STATE ? 1 : TT * NP];
-  __shared__ float sY[STATE ? 1 : TT][CB];
+  __shared__ float sY[STATE ? 1 : TT][YS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Where w = where(a, STATE ? a.chunks - 1 : a.chunks);
   // the coop part: one step, eight channels a thread
@@ -179,49 +209,63 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
   }
   const long uo = (long)w.b * a.sub + (long)w.g * a.Dg, dof = (long)w.b * a.sdb + (long)w.g * a.Dg,
              zo = (long)w.b * a.szb + (long)w.g * a.Dg, oo = (long)w.b * a.T * a.D + (long)w.g * a.Dg;
+  const long bo = (long)w.b * a.sBb + (long)w.g * a.sBg, co = (long)w.b * a.sCb + (long)w.g * a.sCg;
   const int ch = w.c0 + cc;
   float sum = 0.f;
-
+  Raw<T, EPT, VEC> ru, rd_, rz;
+  RawRows<T, S, TT> rB, rC;
+  auto load = [&](int t0) {
+    const int t = max(min(t0 + ct, tv - 1), 0);
+    ru.fetch(a.u, uo + (long)t * a.sut, ch, a.Dg);
+    rd_.fetch(a.dt, dof + (long)t * a.sdt, ch, a.Dg);
+    if (!STATE && a.z) rz.fetch(a.z, zo + (long)t * a.szt, ch, a.Dg);
+    rB.fetch(a.Bm, bo, a.sBt, t0, tv, a.N);
+    if (!STATE) rC.fetch(a.Cm, co, a.sCt, t0, tv, a.N);
+  };
+  load(ts);
   for (int t0 = ts; t0 < te; t0 += TT) {
     const int t = t0 + ct;
     const bool on = t < tv;
-    float u[EPT], dl[EPT], z[EPT];
-    fetch<T, EPT>(a.u, uo + (long)t * a.sut, ch, a.Dg, a.vec, on, u);
-    fetch<T, EPT>(a.dt, dof + (long)t * a.sdt, ch, a.Dg, a.vec, on, dl);
-    if (!STATE && a.z) fetch<T, EPT>(a.z, zo + (long)t * a.szt, ch, a.Dg, a.vec, on, z);
-    stage_bc<T, S, TT>(a.Bm, (long)w.b * a.sBb + (long)w.g * a.sBg, a.sBt, t0, tv, a.N, sB);
-    if (!STATE) stage_bc<T, S, TT>(a.Cm, (long)w.b * a.sCb + (long)w.g * a.sCg, a.sCt, t0, tv, a.N, sC);
+    float u[EPT], z[EPT];
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      float d = dl[i] + bias[i];
+      const bool in = on && ch + i < a.Dg;
+      u[i] = in ? (float)ru.v[i] : 0.f;
+      if (!STATE && a.z) z[i] = in ? (float)rz.v[i] : 0.f;
+      float d = (in ? (float)rd_.v[i] : 0.f) + bias[i];
       if (a.softplus) d = softplus(d);
-      d = on && ch + i < a.Dg ? d : 0.f;       // a step that does not count leaves the state as it is
+      d = in ? d : 0.f;                        // a step that does not count leaves the state as it is
       sD[ct][cc + i][0] = d;
       sD[ct][cc + i][1] = d * u[i];
     }
+    rB.store(sB, t0, tv, a.N);
+    if (!STATE) rC.store(sC, t0, tv, a.N);
     __syncthreads();
+    if (t0 + TT < te) load(t0 + TT);           // under way over the walk
     if (!STATE && a.ckt && ron) store_row<S>(a.ck + (((long)w.b * a.cktiles + t0 / a.ckt) * a.D + rd) * NP + n0, h);
-#pragma unroll 4
-    for (int k = 0; k < TT; ++k) {
-      if (!STATE && Tile<S>::BWD < TT) {          // a backward tile is shorter than this one: its start lies inside
+#pragma unroll 1
+    for (int k = 0; k < TT; k += 4) {
+      if (!STATE && Tile<S>::BWD < TT) {       // a backward tile is shorter than this one: its start lies inside
         if (k && a.ckt && k % Tile<S>::BWD == 0 && ron && t0 + k < a.T)
           store_row<S>(a.ck + (((long)w.b * a.cktiles + (t0 + k) / a.ckt) * a.D + rd) * NP + n0, h);
       }
-      const float d = sD[k][rc][0], x = sD[k][rc][1];
-      float bv[S], cv[S], y = 0.f;
-      load_row<S>(sB + k * NP + n0, bv);
-      if (!STATE) load_row<S>(sC + k * NP + n0, cv);
+      float y[4];
 #pragma unroll
-      for (int s = 0; s < S; ++s) {
-        const float e = __builtin_amdgcn_exp2f(d * A2[s]);
-        h[s] = fmaf(e, h[s], x * bv[s]);
-        if (!STATE) y = fmaf(h[s], cv[s], y);
+      for (int j = 0; j < 4; ++j) {
+        const float d = sD[k + j][rc][0], x = sD[k + j][rc][1];
+        float bv[S], cv[S];
+        load_row<S>(sB + (k + j) * NP + n0, bv);
+        if (!STATE) load_row<S>(sC + (k + j) * NP + n0, cv);
+        y[j] = 0.f;
+#pragma unroll
+        for (int s = 0; s < S; ++s) {
+          const float e = __builtin_amdgcn_exp2f(d * A2[s]);
+          h[s] = fmaf(e, h[s], x * bv[s]);
+          if (!STATE) y[j] = fmaf(h[s], cv[s], y[j]);
+        }
+        if (STATE) sum += d;
       }
-      if (STATE) sum += d;
-      else {
-        y = quad_sum(y);
-        if ((lane & 3) == 0) sY[k][rc] = y;
-      }
+      if (!STATE) sY[k + (lane & 3)][rc] = quad_sum4(y, lane);
     }
     __syncthreads();
     if (!STATE && t < te) {
@@ -232,7 +276,7 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
         if (a.z) y *= tb_silu(z[i]);
         o[i] = on ? y : 0.f;
       }
-      put<T, EPT>(a.out, oo + (long)t * a.D, ch, a.Dg, a.vec, o);
+      put<T, EPT, VEC>(a.out, oo + (long)t * a.D, ch, a.Dg, o);
     }
   }
   if (STATE) {
@@ -303,13 +347,14 @@ struct Row {
 };
 
 // backward.  STATE: only g in front of the chunk's first step from zero behind its last, and its sum of delta.
-template <typename T, int S, bool STATE>
-__global__ void __launch_bounds__(256, 2) scan_bwd(ScanArgs a) {
-  constexpr int TT = Tile<S>::BWD, EPT = TT / 4, NP = 4 * S;
+template <typename T, int S, bool STATE, bool VEC>
+__global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(ScanArgs a) {
+  constexpr int TT = STATE ? 32 : Tile<S>::BWD, EPT = TT / 4, NP = 4 * S;
   __shared__ float sD[TT][CB][2], sG[TT][CB];           // delta, delta u; dy
   __shared__ float sB[STATE ? 1 : TT * NP], sC[TT * NP];
-  __shared__ float sY[STATE ? 1 : TT][CB], sGB[STATE ? 1 : TT][CB], sGA[STATE ? 1 : TT][CB];
+  __shared__ float sY[STATE ? 1 : TT][YS], sGB[STATE ? 1 : TT][YS], sGA[STATE ? 1 : TT][YS];
   __shared__ float sP[STATE ? 1 : 4][STATE ? 1 : TT][2 * NP];
+  __shared__ float sPar[2][CB];                         // dt_bias, D
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   Where w = where(a, STATE ? a.chunks - 1 : a.chunks);
   if (STATE) ++w.chunk;
@@ -319,11 +364,15 @@ __global__ void __launch_bounds__(256, 2) scan_bwd(ScanArgs a) {
   const long rd = w.d0 + rc;
   const int ts = w.chunk * a.chunk, te = min(ts + a.chunk, a.T), tv = min(te, w.len);
 
-  float A2[S], Ar[S], g[S], dA[S];
-  load_state<S>(a.A, rd, n0, a.N, ron, Ar);
+  if (tid < 2 * CB) {
+    const float* p = tid < CB ? a.bias : a.Dp;
+    sPar[tid / CB][tid % CB] = p && w.c0 + tid % CB < a.Dg ? p[w.d0 + tid % CB] : 0.f;
+  }
+  float A2[S], g[S], dA[S];
+  load_state<S>(a.A, rd, n0, a.N, ron, A2);
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    A2[s] = Ar[s] * LOG2E;
+    A2[s] *= LOG2E;
     dA[s] = 0.f;
     g[s] = 0.f;
   }
@@ -340,32 +389,37 @@ __global__ void __launch_bounds__(256, 2) scan_bwd(ScanArgs a) {
   const long gof = (long)w.g * a.Dg;
   const long uo = (long)w.b * a.sub + gof, dof = (long)w.b * a.sdb + gof, zo = (long)w.b * a.szb + gof,
              go = (long)w.b * a.sob + gof, oo = (long)w.b * a.T * a.D + gof;
+  const long bo = (long)w.b * a.sBb + (long)w.g * a.sBg, co = (long)w.b * a.sCb + (long)w.g * a.sCg;
   const int ch = w.c0 + cc;
   float sum = 0.f;
+  __syncthreads();
 
   for (int t0 = ts + (te - ts - 1) / TT * TT; t0 >= ts; t0 -= TT) {
-    const int t = t0 + ct;
+    const int t = t0 + ct, tc = max(min(t, tv - 1), 0);
     const bool on = t < tv;
-    // what the tile's elements give by themselves.  Nothing of it is kept over the walk (its registers hold the tile's
-    // states): what is needed again behind it is fetched again, from the caches
+    // what the tile's elements give by themselves
+    Raw<T, EPT, VEC> ru, rdt, rz, ro;
     {
-      float u[EPT], dl[EPT], z[EPT], go_[EPT], bias[EPT];
-      if (!STATE) fetch<T, EPT>(a.u, uo + (long)t * a.sut, ch, a.Dg, a.vec, on, u);
-      fetch<T, EPT>(a.dt, dof + (long)t * a.sdt, ch, a.Dg, a.vec, on, dl);
-      fetch<T, EPT>(a.dout, go + (long)t * a.sot, ch, a.Dg, a.vec, on, go_);
-      if (a.z) fetch<T, EPT>(a.z, zo + (long)t * a.szt, ch, a.Dg, a.vec, on, z);
-      fetch<float, EPT>(a.bias, w.g * a.Dg, ch, a.Dg, false, a.bias != nullptr, bias);
-      if (!STATE) stage_bc<T, S, TT>(a.Bm, (long)w.b * a.sBb + (long)w.g * a.sBg, a.sBt, t0, tv, a.N, sB);
-      stage_bc<T, S, TT>(a.Cm, (long)w.b * a.sCb + (long)w.g * a.sCg, a.sCt, t0, tv, a.N, sC);
+      RawRows<T, S, TT> rB, rC;
+      if (!STATE) ru.fetch(a.u, uo + (long)tc * a.sut, ch, a.Dg);
+      rdt.fetch(a.dt, dof + (long)tc * a.sdt, ch, a.Dg);
+      ro.fetch(a.dout, go + (long)tc * a.sot, ch, a.Dg);
+      if (a.z) rz.fetch(a.z, zo + (long)tc * a.szt, ch, a.Dg);
+      if (!STATE) rB.fetch(a.Bm, bo, a.sBt, t0, tv, a.N);
+      rC.fetch(a.Cm, co, a.sCt, t0, tv, a.N);
 #pragma unroll
       for (int i = 0; i < EPT; ++i) {
-        float d = dl[i] + bias[i];
+        const bool in = on && ch + i < a.Dg;
+        float d = (in ? (float)rdt.v[i] : 0.f) + sPar[0][cc + i];
         if (a.softplus) d = softplus(d);
-        d = on && ch + i < a.Dg ? d : 0.f;
+        d = in ? d : 0.f;
         sD[ct][cc + i][0] = d;
-        if (!STATE) sD[ct][cc + i][1] = d * u[i];
-        sG[ct][cc + i] = a.z ? go_[i] * tb_silu(z[i]) : go_[i];
+        if (!STATE) sD[ct][cc + i][1] = d * (in ? (float)ru.v[i] : 0.f);
+        const float o = in ? (float)ro.v[i] : 0.f;
+        sG[ct][cc + i] = a.z ? o * tb_silu(in ? (float)rz.v[i] : 0.f) : o;
       }
+      if (!STATE) rB.store(sB, t0, tv, a.N);
+      rC.store(sC, t0, tv, a.N);
     }
     __syncthreads();
     if (STATE) {
@@ -387,6 +441,7 @@ __global__ void __launch_bounds__(256, 2) scan_bwd(ScanArgs a) {
       // one step ahead of the arithmetic, and no further: left alone, the compiler keeps all of a tile's rows in registers
       Row<S> r;
       r.load(sD[0][rc], sG[0][rc], sB + n0, sC + n0);
+      float q4[4], p4[4];
 #pragma unroll
       for (int k = 0; k < TT; ++k) {
         const Row<S> c = r;
@@ -399,8 +454,9 @@ __global__ void __launch_bounds__(256, 2) scan_bwd(ScanArgs a) {
           h[k + 1][s] = fmaf(__builtin_amdgcn_exp2f(c.d * A2[s]), h[k][s], c.x * c.b[s]);
           y = fmaf(h[k + 1][s], c.c[s], y);
         }
-        y = quad_sum(y);
-        if ((lane & 3) == 0) sY[k][rc] = y;
+        asm volatile("" : "+v"(y));
+        q4[k & 3] = y;
+        if ((k & 3) == 3) sY[k - 3 + (lane & 3)][rc] = quad_sum4(q4, lane);
       }
 #pragma unroll
       for (int k = TT - 1; k >= 0; --k) {
@@ -417,14 +473,16 @@ __global__ void __launch_bounds__(256, 2) scan_bwd(ScanArgs a) {
           gB = fmaf(g[s], c.b[s], gB);
           g[s] *= __builtin_amdgcn_exp2f(c.d * A2[s]);
           const float q = g[s] * h[k][s];
-          gA = fmaf(q, Ar[s], gA);
+          gA = fmaf(q, A2[s], gA);                 // of A log2 e: divided out of the sum
           dA[s] = fmaf(q, c.d, dA[s]);
+          asm volatile("" : "+v"(g[s]), "+v"(dA[s]));      // here and now: put off, their operands stay in registers
         }
-        gB = quad_sum(gB);
-        gA = quad_sum(gA);
-        if ((lane & 3) == 0) {
-          sGB[k][rc] = gB;
-          sGA[k][rc] = gA;
+        asm volatile("" : "+v"(gB), "+v"(gA));
+        q4[k & 3] = gB;
+        p4[k & 3] = gA;
+        if ((k & 3) == 0) {
+          sGB[k + (lane & 3)][rc] = quad_sum4(q4, lane);
+          sGA[k + (lane & 3)][rc] = quad_sum4(p4, lane);
         }
         channel_sum<S>(v);
         constexpr int H = S > 1 ? S / 2 : 1;
@@ -433,6 +491,13 @@ __global__ void __launch_bounds__(256, 2) scan_bwd(ScanArgs a) {
 #pragma unroll
           for (int i = 0; i < H; ++i) p[i] = v[i];
         }
+      }
+      // again, from the caches: kept over the walk, they would take the registers of its states
+      ru.fetch(a.u, uo + (long)tc * a.sut, ch, a.Dg);
+      rdt.fetch(a.dt, dof + (long)tc * a.sdt, ch, a.Dg);
+      if (a.dz) {
+        ro.fetch(a.dout, go + (long)tc * a.sot, ch, a.Dg);
+        rz.fetch(a.z, zo + (long)tc * a.szt, ch, a.Dg);
       }
     }
     __syncthreads();
@@ -444,35 +509,31 @@ __global__ void __launch_bounds__(256, 2) scan_bwd(ScanArgs a) {
               t0 + k < tv ? (sP[0][k][n] + sP[1][k][n]) + (sP[2][k][n] + sP[3][k][n]) : 0.f;
       }
       if (t < te) {
-        float o[EPT], u[EPT], dl[EPT], par[EPT];
-        fetch<T, EPT>(a.u, uo + (long)t * a.sut, ch, a.Dg, a.vec, on, u);
-        fetch<T, EPT>(a.dt, dof + (long)t * a.sdt, ch, a.Dg, a.vec, on, dl);
-        fetch<float, EPT>(a.bias, gof, ch, a.Dg, false, a.bias != nullptr, par);
+        float o[EPT], u[EPT];
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
-          o[i] = on ? fmaf(u[i], sGB[ct][cc + i], sGA[ct][cc + i]) : 0.f;
-          if (a.softplus && on) o[i] *= tb_sig(dl[i] + par[i]);      // d delta / d raw
+          const bool in = on && ch + i < a.Dg;
+          u[i] = in ? (float)ru.v[i] : 0.f;
+          o[i] = in ? fmaf(u[i], sGB[ct][cc + i], sGA[ct][cc + i] * (1.f / LOG2E)) : 0.f;
+          if (a.softplus) o[i] *= tb_sig((in ? (float)rdt.v[i] : 0.f) + sPar[0][cc + i]);      // d delta / d raw
           dbias[i] += o[i];
         }
-        if (a.ddt) put<T, EPT>(a.ddt, oo + (long)t * a.D, ch, a.Dg, a.vec, o);
-        fetch<float, EPT>(a.Dp, gof, ch, a.Dg, false, a.Dp != nullptr, par);
+        if (a.ddt) put<T, EPT, VEC>(a.ddt, oo + (long)t * a.D, ch, a.Dg, o);
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
           const float dy = sG[ct][cc + i];
-          o[i] = on ? fmaf(sD[ct][cc + i][0], sGB[ct][cc + i], par[i] * dy) : 0.f;
+          o[i] = on ? fmaf(sD[ct][cc + i][0], sGB[ct][cc + i], sPar[1][cc + i] * dy) : 0.f;
           dD[i] = fmaf(dy, u[i], dD[i]);
         }
-        if (a.du) put<T, EPT>(a.du, oo + (long)t * a.D, ch, a.Dg, a.vec, o);
+        if (a.du) put<T, EPT, VEC>(a.du, oo + (long)t * a.D, ch, a.Dg, o);
         if (a.dz) {
-          float z[EPT];
-          fetch<T, EPT>(a.dout, go + (long)t * a.sot, ch, a.Dg, a.vec, on, o);
-          fetch<T, EPT>(a.z, zo + (long)t * a.szt, ch, a.Dg, a.vec, on, z);
 #pragma unroll
           for (int i = 0; i < EPT; ++i) {
-            const float q = tb_sig(z[i]), y = fmaf(par[i], u[i], sY[ct][cc + i]);
-            o[i] = on ? o[i] * y * (q * (1.f + z[i] * (1.f - q))) : 0.f;
+            const bool in = on && ch + i < a.Dg;
+            const float z = in ? (float)rz.v[i] : 0.f, q = tb_sig(z), y = fmaf(sPar[1][cc + i], u[i], sY[ct][cc + i]);
+            o[i] = in ? (float)ro.v[i] * y * (q * (1.f + z * (1.f - q))) : 0.f;
           }
-          put<T, EPT>(a.dz, oo + (long)t * a.D, ch, a.Dg, a.vec, o);
+          put<T, EPT, VEC>(a.dz, oo + (long)t * a.D, ch, a.Dg, o);
         }
       }
       __syncthreads();
@@ -636,11 +697,15 @@ struct FwdLaunch {
   hipStream_t s;
   template <typename T, int S>
   int operator()() {
+    return a.vec ? run<T, S, true>() : run<T, S, false>();
+  }
+  template <typename T, int S, bool VEC>
+  int run() {
     if (a.chunks > 1) {
-      scan_fwd<T, S, true><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
+      scan_fwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
       scan_chain<S, false><<<(unsigned)(((long)a.B * a.D * 4 * S + 255) / 256), 256, 0, s>>>(a);
     }
-    scan_fwd<T, S, false><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
+    scan_fwd<T, S, false, VEC><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
     return 0;
   }
 };
@@ -652,11 +717,15 @@ struct BwdLaunch {
   hipStream_t s;
   template <typename T, int S>
   int operator()() {
+    return a.vec ? run<T, S, true>() : run<T, S, false>();
+  }
+  template <typename T, int S, bool VEC>
+  int run() {
     if (a.chunks > 1) {
-      scan_bwd<T, S, true><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
+      scan_bwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
       scan_chain<S, true><<<(unsigned)(((long)a.B * a.D * 4 * S + 255) / 256), 256, 0, s>>>(a);
     }
-    scan_bwd<T, S, false><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
+    scan_bwd<T, S, false, VEC><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
     if (dA || dD || dbias)
       scan_finish_par<<<(unsigned)(((long)a.D * (4 * S + 2) + 63) / 64), 256, 0, s>>>(a.par, a.B * a.chunks, a.D, a.N, 4 * S, dA, dD, dbias);
     if (dB || dC)
@@ -698,10 +767,10 @@ int check_common(const char* what, int B, long T, int D, int N, int G, int dtype
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-// 16-byte accesses: every row of every tensor starts on 16 bytes, and so does every group
+// 16-byte accesses: every row of every tensor starts on 16 bytes, and the channels of a group are whole threads' shares (eight)
 bool can_vec(const ScanArgs& a, int dtype) {
   const int v = dtype == TB_F32 ? 4 : 8;
-  if (a.D % v || a.Dg % v || a.sub % v || a.sut % v || a.sdb % v || a.sdt % v) return false;
+  if (a.Dg % 8 || a.sub % v || a.sut % v || a.sdb % v || a.sdt % v) return false;
   if (a.z && (a.szb % v || a.szt % v)) return false;
   if (a.dout && (a.sob % v || a.sot % v)) return false;
   const void* p[] = {a.u, a.dt, a.z, a.dout, a.out, a.du, a.ddt, a.dz};
