@@ -40,6 +40,33 @@ __device__ __forceinline__ void tb_store_n(T* p, const float (&r)[N]) {
   }
 }
 
+// The same for addresses that are only aligned to an element: still one access of 16 bytes (the memory path takes any address).
+template <typename T, int W>
+struct __attribute__((packed, aligned(sizeof(T)))) TbVecU {
+  T v[W];
+};
+template <typename T, int N>
+__device__ __forceinline__ void tb_load_u(const T* p, float (&r)[N]) {
+  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    const TbVecU<T, W> t = *reinterpret_cast<const TbVecU<T, W>*>(p + i);
+#pragma unroll
+    for (int j = 0; j < W; ++j) r[i + j] = (float)t.v[j];
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void tb_store_u(T* p, const float (&r)[N]) {
+  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+#pragma unroll
+  for (int i = 0; i < N; i += W) {
+    TbVecU<T, W> t;
+#pragma unroll
+    for (int j = 0; j < W; ++j) t.v[j] = (T)r[i + j];
+    *reinterpret_cast<TbVecU<T, W>*>(p + i) = t;
+  }
+}
+
 // A parameter that is kept either in the operator's element type or in fp32 (f32 != 0): read / written once per thread
 template <typename T>
 __device__ __forceinline__ float tb_load_par(const void* p, long i, int f32) {

@@ -101,33 +101,39 @@ struct Epi {
   int act;
 };
 
-// four neighbouring columns n .. n+3 of row m
-template <typename T>
-__device__ __forceinline__ void finish4(const Epi& e, long M, int N, long m, int n, f32x4 v, bool four) {
-  if (m >= M || n >= N) return;
+// COUNT neighbouring columns n .. of row m.  EVEN: every row consists of such pieces, on their own alignment; otherwise they lie
+// anywhere, and the last ones of a row go element by element.
+template <typename T, int COUNT, bool EVEN>
+__device__ __forceinline__ void finish(const Epi& e, int N, long m, int n, float (&o)[COUNT]) {
   const long at = m * N + n;
-  float o[4] = {v[0], v[1], v[2], v[3]};
-  if (four) {
+  auto load = [&](const T* p, float (&r)[COUNT]) {
+    if constexpr (EVEN) tb_load_n(p, r);
+    else tb_load_u(p, r);
+  };
+  if (EVEN || n + COUNT <= N) {
+    float q[COUNT];
+    if (e.res) load(static_cast<const T*>(e.res) + m * e.ldr + n, q);
     if (e.bias) {
-      float b[4];
-      tb_load_n(static_cast<const T*>(e.bias) + n, b);
+      float b[COUNT];
+      load(static_cast<const T*>(e.bias) + n, b);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += b[i];
+      for (int i = 0; i < COUNT; ++i) o[i] += b[i];
     }
-    if (e.z) tb_store_n(e.z + at, o);
+    if (e.z) {
+      if constexpr (EVEN) tb_store_n(e.z + at, o);
+      else tb_store_u(e.z + at, o);
+    }
     if (e.act)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] = act_of(o[i], e.act);
-    if (e.res) {
-      float r[4];
-      tb_load_n(static_cast<const T*>(e.res) + m * e.ldr + n, r);
+      for (int i = 0; i < COUNT; ++i) o[i] = act_of(o[i], e.act);
+    if (e.res)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[i] += r[i];
-    }
-    tb_store_n(static_cast<T*>(e.y) + at, o);
+      for (int i = 0; i < COUNT; ++i) o[i] += q[i];
+    if constexpr (EVEN) tb_store_n(static_cast<T*>(e.y) + at, o);
+    else tb_store_u(static_cast<T*>(e.y) + at, o);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < COUNT; ++i) {
       if (n + i >= N) break;
       float w = o[i];
       if (e.bias) w += (float)static_cast<const T*>(e.bias)[n + i];
@@ -145,7 +151,7 @@ struct GemmArgs {
   long M;
   int N, K;
   int tm, tn, splits, per;  // tiles; k tiles a split
-  int four;                 // rows of y, z, the residual and the bias allow 16-byte accesses
+  int width;                // columns an access of the epilogue, of which every row is whole: 8 (16-bit types), 4, 2 or 1
   Epi e;
 };
 
@@ -164,27 +170,6 @@ template <typename T>
 __device__ __forceinline__ void write_block(const GemmArgs& a, const float* own, long m0, int n0, int lane) {
   const Epi& e = a.e;
   auto piece = [&](int r, int c) { return *reinterpret_cast<const f32x4*>(own + r * 64 + ((c ^ (r & 15)) * 4)); };
-  if (!a.four) {                       // any width: a lane a column, element by element
-    const int n = n0 + lane;
-    if (n >= a.N) return;
-    const float b = e.bias && !e.slab ? (float)static_cast<const T*>(e.bias)[n] : 0.f;
-#pragma unroll 2
-    for (int r = 0; r < 64; ++r) {
-      const long m = m0 + r;
-      if (m >= a.M) break;
-      float v = own[r * 64 + (((lane >> 2) ^ (r & 15)) * 4) + (lane & 3)];
-      if (e.slab) {
-        e.slab[((long)blockIdx.y * a.M + m) * a.N + n] = v;
-        continue;
-      }
-      v += b;
-      if (e.z) e.z[m * a.N + n] = v;
-      v = act_of(v, e.act);
-      if (e.res) v += (float)static_cast<const T*>(e.res)[m * e.ldr + n];
-      static_cast<T*>(e.y)[m * a.N + n] = (T)v;
-    }
-    return;
-  }
   if (e.slab) {
     const int c = lane & 15, n = n0 + c * 4;
     if (n >= a.N) return;
@@ -192,38 +177,48 @@ __device__ __forceinline__ void write_block(const GemmArgs& a, const float* own,
     for (int r = lane >> 4; r < 64; r += 4) {
       const long m = m0 + r;
       if (m >= a.M) break;
-      *reinterpret_cast<f32x4*>(e.slab + ((long)blockIdx.y * a.M + m) * a.N + n) = piece(r, c);
+      const f32x4 v = piece(r, c);
+      float* s = e.slab + ((long)blockIdx.y * a.M + m) * a.N + n;
+      if (n + 4 <= a.N) {
+        const float o[4] = {v[0], v[1], v[2], v[3]};
+        tb_store_u(s, o);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (n + i < a.N) s[i] = v[i];
+      }
     }
     return;
   }
-  constexpr int V = 16 / sizeof(T), L = 64 / V;       // columns a lane, lanes a row
-  const int c = lane % L, n = n0 + c * V;
-  if (n >= a.N) return;                                // four: N is a multiple of V
-  float b[V];
-#pragma unroll
-  for (int i = 0; i < V; ++i) b[i] = 0.f;
-  if (e.bias) tb_load_n(static_cast<const T*>(e.bias) + n, b);
+  // accesses of 16 bytes off their alignment cost more than smaller ones on theirs (N = 1500 of fp16: 6 us of a 17 us call)
+  auto rows = [&](auto width) {
+    constexpr int V = width, L = 64 / V;               // columns a lane, lanes a row
+    const int c = lane % L * V, n = n0 + c;
+    if (n >= a.N) return;
 #pragma unroll 2
-  for (int r = lane / L; r < 64; r += V) {
-    const long m = m0 + r;
-    if (m >= a.M) break;
-    float o[V], q[V];
-    if (e.res) tb_load_n(static_cast<const T*>(e.res) + m * e.ldr + n, q);
+    for (int r = lane / L; r < 64; r += V) {
+      const long m = m0 + r;
+      if (m >= a.M) break;
+      float o[V];
+      if constexpr (V >= 4) {
 #pragma unroll
-    for (int k = 0; k < V / 4; ++k) {
-      const f32x4 v = piece(r, c * (V / 4) + k);
+        for (int k = 0; k < V / 4; ++k) {
+          const f32x4 v = piece(r, c / 4 + k);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) o[k * 4 + i] = v[i] + b[k * 4 + i];
+          for (int i = 0; i < 4; ++i) o[k * 4 + i] = v[i];
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = own[r * 64 + ((c / 4) ^ (r & 15)) * 4 + c % 4 + i];
+      }
+      finish<T, V, true>(e, a.N, m, n, o);
     }
-    if (e.z) tb_store_n(e.z + m * a.N + n, o);
-    if (e.act)
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = act_of(o[i], e.act);
-    if (e.res)
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] += q[i];
-    tb_store_n(static_cast<T*>(e.y) + m * a.N + n, o);
-  }
+  };
+  if (a.width == 8) {
+    if constexpr (sizeof(T) == 2) rows(std::integral_constant<int, 8>{});
+  } else if (a.width == 4) rows(std::integral_constant<int, 4>{});
+  else if (a.width == 2) rows(std::integral_constant<int, 2>{});
+  else rows(std::integral_constant<int, 1>{});
 }
 
 // 64 bytes of k a tile, four tiles in LDS: while one tile is multiplied from registers, the next one's fragments are read
@@ -368,30 +363,46 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm_nt(GemmArg
   }
 }
 
-// the splits' sums, in their order, and the epilogue
+// the splits' sums and the epilogue: four columns a thread, four threads share a place's splits and are added in their order
 template <typename T>
-__global__ void __launch_bounds__(256) split_finish(Epi e, long M, int N, int splits, int four) {
-  const int nq = (N + 3) / 4;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= M * nq) return;
-  const long m = id / nq;
-  const int n = (int)(id % nq) * 4;
-  f32x4 s = (f32x4){0.f, 0.f, 0.f, 0.f};
+__global__ void __launch_bounds__(256) split_finish(Epi e, long M, int N, int splits) {
+  __shared__ float red[4][64][4];
+  const int nq = (N + 3) / 4, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const long id = (long)blockIdx.x * 64 + x;
+  const bool on = id < M * nq;
+  const long m = on ? id / nq : 0;
+  const int n = on ? (int)(id % nq) * 4 : 0;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  if (on) {
+    const int per = (splits + 3) / 4, k1 = min(splits, (y + 1) * per);
+    if (n + 4 <= N) {
 #pragma unroll 4
-  for (int k = 0; k < splits; ++k) {
-    const float* p = e.slab + ((long)k * M + m) * N + n;
-    if (four) s += *reinterpret_cast<const f32x4*>(p);
-    else
-      for (int q = 0; q < 4; ++q)
-        if (n + q < N) s[q] += p[q];
+      for (int k = y * per; k < k1; ++k) {
+        float v[4];
+        tb_load_u(e.slab + ((long)k * M + m) * N + n, v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[i] += v[i];
+      }
+    } else {
+      for (int k = y * per; k < k1; ++k)
+#pragma unroll
+        for (int i = 0; i < 3; ++i)
+          if (n + i < N) s[i] += e.slab[((long)k * M + m) * N + n + i];
+    }
   }
-  finish4<T>(e, M, N, m, n, s, four);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) red[y][x][i] = s[i];
+  __syncthreads();
+  if (y || !on) return;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) s[i] = (red[0][x][i] + red[1][x][i]) + (red[2][x][i] + red[3][x][i]);
+  finish<T, 4, false>(e, N, m, n, s);
 }
 
 struct FewArgs {
   const void *x, *W;
   long ldx, ldw, M;
-  int N, K, vec, four;
+  int N, K, vec;
   Epi e;
 };
 
@@ -450,7 +461,10 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_few(FewArgs a) {
     f32x4 s = red[0][wave][lane];
 #pragma unroll
     for (int k = 1; k < WAVES; ++k) s += red[k][wave][lane];
-    finish4<T>(a.e, a.M, a.N, wave * 16 + row, n0 + (lane >> 4) * 4, s, a.four);
+    const long m = wave * 16 + row;
+    const int n = n0 + (lane >> 4) * 4;
+    float o[4] = {s[0], s[1], s[2], s[3]};
+    if (m < a.M && n < a.N) finish<T, 4, false>(a.e, a.N, m, n, o);
   }
 }
 
@@ -469,23 +483,51 @@ __global__ void __launch_bounds__(256) pack_rows(const T* src, long ld, long R, 
   *reinterpret_cast<TbVec<T, CE>*>(dst + r * Cp + c) = v;
 }
 
-// dst[c][r] = src[r][c]; dst's rows are padded by zeros to Rp
+// eight neighbouring elements of row r from column c on: zeros behind C and R
+template <typename T>
+__device__ __forceinline__ void load8(const T* src, long ld, long R, int C, long r, int c, float (&v)[8]) {
+  if (r < R && c + 8 <= C) {
+    tb_load_u(src + r * ld + c, v);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = r < R && c + i < C ? (float)src[r * ld + c + i] : 0.f;
+  }
+}
+// row c of the tile's columns r0 + x0 .. + 8 to dst[c][r], whose rows are Rp long (a multiple of 16 bytes)
+template <typename T>
+__device__ __forceinline__ void store_column(const float (&t)[64][65], int c, int x0, T* dst, long Rp, long r0) {
+  float v[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = t[x0 + i][c];
+  constexpr int W = 16 / sizeof(T);
+#pragma unroll
+  for (int i = 0; i < 8; i += W) {
+    if (r0 + x0 + i < Rp) {
+      float w[W];
+#pragma unroll
+      for (int j = 0; j < W; ++j) w[j] = v[i + j];
+      tb_store_n(dst + r0 + x0 + i, w);
+    }
+  }
+}
+
+// dst[c][r] = src[r][c]; dst's rows are padded by zeros to Rp.  64 x 64 a block, 16 bytes an access on both sides.
 template <typename T>
 __global__ void __launch_bounds__(256) transpose(const T* src, long ld, long R, int C, T* dst, long Rp) {
   __shared__ float t[64][65];
   const long r0 = (long)blockIdx.x * 64;
-  const int c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
+  const int c0 = blockIdx.y * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const long r = r0 + y + i * 4;
-    t[y + i * 4][x] = r < R && c0 + x < C ? (float)src[r * ld + c0 + x] : 0.f;
+  for (int i = 0; i < 64; i += 32) {
+    float v[8];
+    load8(src, ld, R, C, r0 + y + i, c0 + x, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[y + i][x + j] = v[j];
   }
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const int c = c0 + y + i * 4;
-    if (c < C && r0 + x < Rp) dst[c * Rp + r0 + x] = (T)t[x][y + i * 4];
-  }
+  for (int i = 0; i < 64; i += 32)
+    if (c0 + y + i < C) store_column<T>(t, y + i, x, dst + (long)(c0 + y + i) * Rp, Rp, r0);
 }
 
 // dz = dy act'(z) in both orders, each nullable, and the column sums of each 64 rows (fp32, before dz is rounded)
@@ -493,46 +535,68 @@ template <typename T>
 __global__ void __launch_bounds__(256) form_dz(const T* dy, long ldy, const float* z, int act, long M, int N, T* dz, int Np, T* dzT, long Mp,
                                                float* part) {
   __shared__ float t[64][65];
+  __shared__ float red[4][64];
   const long r0 = (long)blockIdx.x * 64;
-  const int c0 = blockIdx.y * 64, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-#pragma unroll 4
-  for (int i = 0; i < 16; ++i) {
-    const long r = r0 + y + i * 4;
-    float v = 0.f;
-    if (r < M && c0 + x < N) {
-      v = (float)dy[r * ldy + c0 + x];
-      if (z) v *= act_grad(z[r * N + c0 + x], act);
+  const int c0 = blockIdx.y * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
+#pragma unroll
+  for (int i = 0; i < 64; i += 32) {
+    const long r = r0 + y + i;
+    float v[8], p[8];
+    load8(dy, ldy, M, N, r, c0 + x, v);
+    if (z) {
+      load8(z, (long)N, M, N, r, c0 + x, p);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] *= act_grad(p[j], act);
     }
-    if (dz && r < M && c0 + x < Np) dz[r * Np + c0 + x] = (T)v;
-    t[y + i * 4][x] = v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t[y + i][x + j] = v[j];
+    if (dz && r < M) {
+      constexpr int W = 16 / sizeof(T);
+#pragma unroll
+      for (int k = 0; k < 8; k += W)
+        if (c0 + x + k < Np) {
+          float w[W];
+#pragma unroll
+          for (int j = 0; j < W; ++j) w[j] = v[k + j];
+          tb_store_n(dz + r * Np + c0 + x + k, w);
+        }
+    }
   }
   __syncthreads();
   if (dzT) {
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int c = c0 + y + i * 4;
-      if (c < N && r0 + x < Mp) dzT[c * Mp + r0 + x] = (T)t[x][y + i * 4];
-    }
+    for (int i = 0; i < 64; i += 32)
+      if (c0 + y + i < N) store_column<T>(t, y + i, x, dzT + (long)(c0 + y + i) * Mp, Mp, r0);
   }
-  if (part && y == 0 && c0 + x < N) {
+  if (part) {
+    const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
     float s = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < 64; ++i) s += t[i][x];
-    part[(long)blockIdx.x * N + c0 + x] = s;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) s += t[q * 16 + i][c];
+    red[q][c] = s;
+    __syncthreads();
+    if (q == 0 && c0 + c < N) part[(long)blockIdx.x * N + c0 + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
   }
 }
 
+// db from the sums of each 64 rows: sixteen columns a block, 64 threads a column, added in the order of the rows
 template <typename T>
 __global__ void __launch_bounds__(1024) colsum_finish(const float* part, long rows, int N, T* db) {
-  __shared__ float red[16][65];
-  const int x = threadIdx.x & 63, y = threadIdx.x >> 6, c = blockIdx.x * 64 + x;
+  __shared__ float red[64][17];
+  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
   float s = 0.f;
   if (c < N) {
-    const long per = (rows + 15) / 16, r1 = min(rows, (y + 1) * per);
+    const long per = (rows + 63) / 64, r1 = min(rows, (y + 1) * per);
 #pragma unroll 4
     for (long r = y * per; r < r1; ++r) s += part[r * N + c];
   }
   red[y][x] = s;
+  __syncthreads();
+  if (y < 16) {
+    s = (red[y * 4][x] + red[y * 4 + 1][x]) + (red[y * 4 + 2][x] + red[y * 4 + 3][x]);
+  }
+  __syncthreads();
+  if (y < 16) red[y][x] = s;
   __syncthreads();
   if (y == 0 && c < N) {
     s = 0.f;
@@ -550,7 +614,7 @@ struct Plan {
   bool big;
   int tm, tn, splits, per;
 };
-// 256 x 256 tiles where they fill the chip, 128 x 128 otherwise (two blocks a unit); k is split where even those leave units
+// 256 x 256 tiles where they fill the chip, 128 x 128 otherwise (two blocks a unit).  k is split where even those leave units
 // idle, into parts of sixteen k tiles (1 KB of a row) at least.
 Plan plan(long M, int N, long K, int esize) {
   Plan p;
@@ -562,8 +626,8 @@ Plan plan(long M, int N, long K, int esize) {
   p.tn = (N + b - 1) / b;
   const long tiles = (long)p.tm * p.tn;
   long s = 1;
-  if (!p.big && tiles < 2 * cus) {
-    s = 2 * cus / tiles;
+  if (!p.big && tiles <= cus / 2) {
+    s = cus / tiles;
     if (s > kt / 16) s = kt / 16;
     if (s > 64) s = 64;
     if (s < 1) s = 1;
@@ -580,16 +644,20 @@ size_t slab_bytes(long M, int N, long K, int esize) {
 template <typename T>
 int launch_gemm(const T* P, long ldp, const T* Q, long ldq, long M, int N, long K, Epi e, float* slab, hipStream_t s) {
   const Plan p = plan(M, N, K, sizeof(T));
-  constexpr int CE = 16 / sizeof(T);
-  GemmArgs a{P, Q, ldp, ldq, M, N, (int)K, p.tm, p.tn, p.splits, p.per, 0, e};
-  a.four = N % CE == 0 && aligned(e.y) && aligned(e.z) && aligned(e.bias) && aligned(e.res) && (!e.res || e.ldr % CE == 0);
+  GemmArgs a{P, Q, ldp, ldq, M, N, (int)K, p.tm, p.tn, p.splits, p.per, 16 / (int)sizeof(T), e};
+  auto whole = [&](int w) {
+    const uintptr_t bytes = w * sizeof(T);
+    return N % w == 0 && (!e.res || e.ldr % w == 0) && reinterpret_cast<uintptr_t>(e.y) % bytes == 0 && reinterpret_cast<uintptr_t>(e.res) % bytes == 0 &&
+           reinterpret_cast<uintptr_t>(e.bias) % bytes == 0 && reinterpret_cast<uintptr_t>(e.z) % (w < 4 ? w * 4 : 16) == 0;
+  };
+  while (a.width > 1 && !whole(a.width)) a.width /= 2;
   a.e.slab = p.splits > 1 ? slab : nullptr;
   const dim3 grid(p.tm * p.tn, p.splits);
   if (p.big) gemm_nt<T, 256, 256, 128, 64><<<grid, 512, 0, s>>>(a);
   else gemm_nt<T, 128, 128, 64, 64><<<grid, 256, 0, s>>>(a);
   TB_LAUNCH_CHECK("linres gemm");
   if (p.splits > 1) {
-    split_finish<T><<<(unsigned)((M * ((N + 3) / 4) + 255) / 256), 256, 0, s>>>(a.e, M, N, p.splits, a.four);
+    split_finish<T><<<(unsigned)((M * ((N + 3) / 4) + 63) / 64), 256, 0, s>>>(a.e, M, N, p.splits);
     TB_LAUNCH_CHECK("linres split_finish");
   }
   return TB_OK;
@@ -605,9 +673,8 @@ template <typename T>
 int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, int N, char* ws, hipStream_t s) {
   constexpr int CE = 16 / sizeof(T);
   if (M <= FEW) {
-    FewArgs a{x, W, ldx, ldw, M, N, K, 0, 0, e};
+    FewArgs a{x, W, ldx, ldw, M, N, K, 0, e};
     a.vec = direct<T>(x, ldx, K) && direct<T>(W, ldw, K);
-    a.four = N % 4 == 0 && aligned(e.y) && aligned(e.z) && aligned(e.bias) && aligned(e.res) && (!e.res || e.ldr % CE == 0);
     const unsigned grid = (N + 15) / 16;
     if (M <= 16) gemm_few<T, 1, 4><<<grid, 256, 0, s>>>(a);
     else gemm_few<T, 2, 4><<<grid, 256, 0, s>>>(a);
@@ -634,20 +701,23 @@ int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, in
   return launch_gemm<T>(x, ldx, W, ldw, M, N, Kp, e, reinterpret_cast<float*>(p), s);
 }
 
+// rows of what the backward pass lays out start on whole lines (a row off them costs its copies another line each)
+long pitch(long x, int esize) { return (x + 128 / esize - 1) / (128 / esize) * (128 / esize); }
+
 struct BwdSizes {
   size_t dz, dzT, WT, xT, part, slab, total;
   long Np, Mp;
 };
 BwdSizes bwd_sizes(long M, int K, int N, int es) {
   BwdSizes b;
-  b.Np = up(N, es);
-  b.Mp = up(M, es);
+  b.Np = pitch(N, es);
+  b.Mp = pitch(M, es);
   b.dz = tb_align_up((size_t)M * b.Np * es, 256);
   b.dzT = tb_align_up((size_t)N * b.Mp * es, 256);
   b.WT = tb_align_up((size_t)K * b.Np * es, 256);
   b.xT = tb_align_up((size_t)K * b.Mp * es, 256);
   b.part = tb_align_up((size_t)((M + 63) / 64) * N * 4, 256);
-  const size_t s1 = slab_bytes(M, K, b.Np, es), s2 = slab_bytes(N, K, b.Mp, es);
+  const size_t s1 = slab_bytes(M, K, up(N, es), es), s2 = slab_bytes(N, K, up(M, es), es);
   b.slab = s1 > s2 ? s1 : s2;
   b.total = b.dz + b.dzT + b.WT + b.xT + b.part + b.slab + 256;
   return b;
@@ -672,7 +742,7 @@ int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, 
     TB_LAUNCH_CHECK("linres form_dz");
   }
   if (db) {
-    colsum_finish<T><<<(unsigned)((N + 63) / 64), 1024, 0, s>>>(part, (M + 63) / 64, N, db);
+    colsum_finish<T><<<(unsigned)((N + 15) / 16), 1024, 0, s>>>(part, (M + 63) / 64, N, db);
     TB_LAUNCH_CHECK("linres colsum_finish");
   }
   Epi e{};
@@ -680,14 +750,14 @@ int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, 
     transpose<T><<<dim3((unsigned)((b.Np + 63) / 64), (unsigned)((K + 63) / 64)), 256, 0, s>>>(W, ldw, N, K, WT, b.Np);
     TB_LAUNCH_CHECK("linres transpose");
     e.y = dx;
-    const int rc = launch_gemm<T>(dzr, ldz, WT, b.Np, M, K, b.Np, e, slab, s);
+    const int rc = launch_gemm<T>(dzr, ldz, WT, b.Np, M, K, up(N, sizeof(T)), e, slab, s);
     if (rc) return rc;
   }
   if (dW) {
     transpose<T><<<dim3((unsigned)((b.Mp + 63) / 64), (unsigned)((K + 63) / 64)), 256, 0, s>>>(x, ldx, M, K, xT, b.Mp);
     TB_LAUNCH_CHECK("linres transpose");
     e.y = dW;
-    const int rc = launch_gemm<T>(dzT, b.Mp, xT, b.Mp, N, K, b.Mp, e, slab, s);
+    const int rc = launch_gemm<T>(dzT, b.Mp, xT, b.Mp, N, K, up(M, sizeof(T)), e, slab, s);
     if (rc) return rc;
   }
   return TB_OK;
