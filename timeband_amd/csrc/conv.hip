@@ -5,9 +5,11 @@
 //   dpre = dy act'(pre)    dx[t] = sum_j w[j] dpre[t+K-1-j]    dw[j] = sum_{b,t} dpre[t] x[t-K+1+j]    db = sum dpre
 //
 // Bound by memory: 2 K operations an element against 2 elements moved (forward), 4 moved backward.  A thread owns VEC channels
-// (16 bytes) and walks a run of steps with the K-1 last inputs in registers, so that each element is read once, plus K-1 of
-// its neighbour's a run; lanes are neighbours in the channels, so a wave reads whole lines.  Backward recomputes pre from x
-// instead of keeping it (K multiplications against 2 or 4 bytes an element written and read).
+// (16 bytes; backward of 16-bit types 8) and walks a run of steps with the K-1 last inputs in registers, so that each element is
+// read once, plus K-1 of its neighbour's a run; lanes are neighbours in the channels, so a wave reads whole lines.  Four steps
+// are fetched together and one group ahead of the arithmetic: a step at a time, the loop waited for memory at each (8 x 2048 x 2048
+// bf16: 34 and 91 us).  Backward recomputes pre from x instead of keeping it (K multiplications against 2 or 4 bytes an
+// element written and read).
 #include "elem.h"
 
 namespace {
@@ -60,6 +62,19 @@ __device__ __forceinline__ void load_par(const void* w, const void* bias, int f3
     for (int k = 0; k < K; ++k) r[k][i] = flat[i * K + k];
 }
 
+constexpr int GRP = 4;      // steps fetched together; a run is a multiple of it
+
+// GRP rows from step t on, as they lie in memory; rows behind the sequence's steps read another row of it
+template <typename T, int VEC>
+struct Rows {
+  TbVec<T, VEC> v[GRP];
+  __device__ __forceinline__ void fetch(const T* base, long st, int t, int T_) {
+#pragma unroll
+    for (int i = 0; i < GRP; ++i) v[i] = *reinterpret_cast<const TbVec<T, VEC>*>(base + (long)min(t + i, T_ - 1) * st);
+  }
+  __device__ __forceinline__ float get(int i, int c, bool on) const { return on ? (float)v[i].v[c] : 0.f; }
+};
+
 // block: blockDim.x channel groups of VEC by blockDim.y runs
 template <typename T, int K, int VEC>
 __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
@@ -69,27 +84,41 @@ __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
   const int b = (int)(r / a.runs), q = (int)(r % a.runs);
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
   const int t0 = q * a.run, t1 = min(t0 + a.run, a.T);
-  float w[K][VEC], bias[VEC], win[K][VEC];
-  load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
+  const T* x = static_cast<const T*>(a.x) + b * a.sxb + c;
+  T* y = static_cast<T*>(a.y) + (long)b * a.T * a.D + c;
+  if (t0 < t1) {
+    Rows<T, VEC> next;
+    next.fetch(x, a.sxt, t0, a.T);
+    float w[K][VEC], bias[VEC], win[K - 1 + GRP][VEC];
+    load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
 #pragma unroll
-  for (int k = 0; k < K - 1; ++k) load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
-  T* y = static_cast<T*>(a.y) + ((long)b * a.T) * a.D + c;
-  for (int t = t0; t < t1; ++t) {
-    load_x<T, VEC>(a, b, t, len, K, c, win[K - 1]);
-    float o[VEC];
+    for (int k = 0; k < K - 1; ++k) load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
+    for (int t = t0; t < t1; t += GRP) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      float s = bias[i];
+      for (int j = 0; j < GRP; ++j)
 #pragma unroll
-      for (int k = 0; k < K; ++k) s = fmaf(w[k][i], win[k][i], s);
-      if (a.act == TB_ACT_SILU) s = tb_silu(s);
-      o[i] = t < len ? s : 0.f;
+        for (int i = 0; i < VEC; ++i) win[K - 1 + j][i] = next.get(j, i, t + j < len);
+      if (t + GRP < t1) next.fetch(x, a.sxt, t + GRP, a.T);
+#pragma unroll
+      for (int j = 0; j < GRP; ++j) {
+        if (t + j < t1) {
+          float o[VEC];
+#pragma unroll
+          for (int i = 0; i < VEC; ++i) {
+            float s = bias[i];
+#pragma unroll
+            for (int k = 0; k < K; ++k) s = fmaf(w[k][i], win[j + k][i], s);
+            if (a.act == TB_ACT_SILU) s = tb_silu(s);
+            o[i] = t + j < len ? s : 0.f;
+          }
+          tb_store_n(y + (long)(t + j) * a.D, o);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) win[k][i] = win[k + GRP][i];
     }
-    tb_store_n(y + (long)t * a.D, o);
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) win[k][i] = win[k + 1][i];
   }
   if (a.state_out && q == 0) {
 #pragma unroll
@@ -103,7 +132,7 @@ __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
 
 template <typename T, int K, int VEC>
 __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
-  __shared__ float red[256];
+  __shared__ float red[256][VEC];
   const int c = (blockIdx.x * blockDim.x + threadIdx.x) * VEC;
   const long r = (long)blockIdx.y * blockDim.y + threadIdx.y;
   const bool on = c < a.D && r < (long)a.B * a.runs;
@@ -116,80 +145,95 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
     const int b = (int)(r / a.runs), q = (int)(r % a.runs);
     const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
     const int t0 = q * a.run, t1 = min(t0 + a.run, a.T);
-    float w[K][VEC], bias[VEC], win[K][VEC], dp[K][VEC];   // win: x[s-K+1 .. s]; dp: dpre[s-K+1 .. s]
-    load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
-#pragma unroll
-    for (int i = 0; i < VEC; ++i)
-#pragma unroll
-      for (int k = 0; k < K; ++k) dp[k][i] = 0.f;
-#pragma unroll
-    for (int k = 0; k < K - 1; ++k) load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
+    const T* x = static_cast<const T*>(a.x) + b * a.sxb + c;
     const T* dy = static_cast<const T*>(a.dy) + (long)b * a.T * a.D + c;
     T* dx = static_cast<T*>(a.dx) + (long)b * a.T * a.D + c;
-    for (int s = t0; s < t1 + K - 1; ++s) {
-      load_x<T, VEC>(a, b, s, len, K, c, win[K - 1]);
-      float g[VEC];
-      if (s < len) {
-        tb_load_n(dy + (long)s * a.D, g);
-        if (a.act == TB_ACT_SILU) {
+    Rows<T, VEC> nx, ny;
+    nx.fetch(x, a.sxt, t0, a.T);
+    ny.fetch(dy, a.D, t0, a.T);
+    // win[K-1+j]: x of step s + j; dp likewise of dpre
+    float w[K][VEC], bias[VEC], win[K - 1 + GRP][VEC], dp[K - 1 + GRP][VEC];
+    load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
 #pragma unroll
-          for (int i = 0; i < VEC; ++i) {
+    for (int k = 0; k < K - 1; ++k) {
+      load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) dp[k][i] = 0.f;
+    }
+    const int end = t1 + K - 1;               // dx of the run's last steps needs dpre of the next run's first
+    for (int s = t0; s < end; s += GRP) {
+      float g[GRP][VEC];
+#pragma unroll
+      for (int j = 0; j < GRP; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          win[K - 1 + j][i] = nx.get(j, i, s + j < len);
+          g[j][i] = ny.get(j, i, s + j < len);
+        }
+      if (s + GRP < end) {
+        nx.fetch(x, a.sxt, s + GRP, a.T);
+        ny.fetch(dy, a.D, s + GRP, a.T);
+      }
+#pragma unroll
+      for (int j = 0; j < GRP; ++j) {
+        const bool mine = s + j < t1;         // the run's own steps: their share of dw and db
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+          float d = g[j][i];
+          if (a.act == TB_ACT_SILU) {
             float p = bias[i];
 #pragma unroll
-            for (int k = 0; k < K; ++k) p = fmaf(w[k][i], win[k][i], p);
+            for (int k = 0; k < K; ++k) p = fmaf(w[k][i], win[j + k][i], p);
             const float sg = tb_sig(p);
-            g[i] *= sg * (1.f + p * (1.f - sg));
+            d *= sg * (1.f + p * (1.f - sg));
+            d = s + j < len ? d : 0.f;
           }
+          dp[K - 1 + j][i] = d;
+          const float m = mine ? d : 0.f;
+#pragma unroll
+          for (int k = 0; k < K; ++k) dw[k][i] = fmaf(m, win[j + k][i], dw[k][i]);
+          dw[K][i] += m;
         }
-      } else {
+        const int t = s + j - (K - 1);        // dx[t] needs dpre[t .. t+K-1] = dp[j .. j+K-1]
+        if (t >= t0 && t < t1) {
+          float o[VEC];
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) g[i] = 0.f;
-      }
+          for (int i = 0; i < VEC; ++i) {
+            float v = 0.f;
 #pragma unroll
-      for (int i = 0; i < VEC; ++i) dp[K - 1][i] = g[i];
-      if (s < t1) {
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-#pragma unroll
-          for (int k = 0; k < K; ++k) dw[k][i] = fmaf(g[i], win[k][i], dw[k][i]);
-          dw[K][i] += g[i];
+            for (int k = 0; k < K; ++k) v = fmaf(w[K - 1 - k][i], dp[j + k][i], v);
+            o[i] = t < len ? v : 0.f;
+          }
+          tb_store_n(dx + (long)t * a.D, o);
         }
-      }
-      const int t = s - (K - 1);                   // dx[t] needs dpre[t .. t+K-1] = dp[0 .. K-1]
-      if (t >= t0) {
-        float o[VEC];
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-          float v = 0.f;
-#pragma unroll
-          for (int k = 0; k < K; ++k) v = fmaf(w[K - 1 - k][i], dp[k][i], v);
-          o[i] = t < len ? v : 0.f;
-        }
-        tb_store_n(dx + (long)t * a.D, o);
       }
 #pragma unroll
       for (int k = 0; k < K - 1; ++k)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-          win[k][i] = win[k + 1][i];
-          dp[k][i] = dp[k + 1][i];
+          win[k][i] = win[k + GRP][i];
+          dp[k][i] = dp[k + GRP][i];
         }
     }
   }
   // sums of the block's runs, in the order of the runs
+  const int me = threadIdx.y * blockDim.x + threadIdx.x;
 #pragma unroll
-  for (int k = 0; k <= K; ++k)
+  for (int k = 0; k <= K; ++k) {
 #pragma unroll
-    for (int i = 0; i < VEC; ++i) {
-      red[threadIdx.y * blockDim.x + threadIdx.x] = dw[k][i];
-      __syncthreads();
-      if (threadIdx.y == 0 && c < a.D) {
-        float s = 0.f;
-        for (int j = 0; j < (int)blockDim.y; ++j) s += red[j * blockDim.x + threadIdx.x];
-        a.slab[((long)blockIdx.y * (K + 1) + k) * a.D + c + i] = s;
-      }
-      __syncthreads();
+    for (int i = 0; i < VEC; ++i) red[me][i] = dw[k][i];
+    __syncthreads();
+    if (threadIdx.y == 0 && c < a.D) {
+      float o[VEC];
+#pragma unroll
+      for (int i = 0; i < VEC; ++i) o[i] = 0.f;
+      for (int j = 0; j < (int)blockDim.y; ++j)
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] += red[j * blockDim.x + threadIdx.x][i];
+      tb_store_n(a.slab + ((long)blockIdx.y * (K + 1) + k) * a.D + c, o);
     }
+    __syncthreads();
+  }
 }
 
 // dw (D, K), db (D) from the slab's rows, summed in their order by sixteen threads a column
@@ -253,7 +297,7 @@ __global__ void __launch_bounds__(256) conv_step(ConvStepArgs a) {
 }
 
 // one instantiation per (type, taps, vector width): F is called with the kernel's template arguments
-template <typename F>
+template <int V16, typename F>
 int by_shape(int dtype, int K, bool vec, F&& f) {
 #define TB_K(T, V)                                                          \
   switch (K) {                                                              \
@@ -269,9 +313,9 @@ int by_shape(int dtype, int K, bool vec, F&& f) {
   if (dtype == TB_F32) {
     if (vec) TB_K(float, 4) else TB_K(float, 1)
   } else if (dtype == TB_BF16) {
-    if (vec) TB_K(__bf16, 8) else TB_K(__bf16, 1)
+    if (vec) TB_K(__bf16, V16) else TB_K(__bf16, 1)
   } else {
-    if (vec) TB_K(_Float16, 8) else TB_K(_Float16, 1)
+    if (vec) TB_K(_Float16, V16) else TB_K(_Float16, 1)
   }
 #undef TB_K
 }
@@ -324,7 +368,7 @@ Plan plan(int B, int T, int D, int vec) {
   while (p.bx > 1 && p.bx / 2 >= groups) p.bx /= 2;
   p.by = 256 / p.bx;
   const long want = ((long)B * T * groups) >> 18;
-  p.run = (int)(want < 8 ? 8 : want > 64 ? 64 : want);
+  p.run = (int)(want < 8 ? 8 : want > 64 ? 64 : want) / GRP * GRP;
   p.runs = (T + p.run - 1) / p.run;
   p.gx = (groups + p.bx - 1) / p.bx;
   p.gy = ((long)B * p.runs + p.by - 1) / p.by;
@@ -371,15 +415,16 @@ int tb_conv_fwd(const void* x, long x_batch_stride, long x_step_stride, const vo
   if (rc) return rc;
   ConvArgs a{x, w, bias, state, nullptr, lengths, y, state_out, nullptr, nullptr, x_batch_stride, x_step_stride, B, T, D, p.run,
              p.runs, act, w_f32};
-  by_shape(dtype, K, vec, FwdLaunch{a, dim3((unsigned)p.gx, (unsigned)p.gy), dim3(p.bx, p.by), static_cast<hipStream_t>(stream)});
+  by_shape<8>(dtype, K, vec, FwdLaunch{a, dim3((unsigned)p.gx, (unsigned)p.gy), dim3(p.bx, p.by), static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("conv_fwd");
   return TB_OK;
 }
 
 size_t tb_conv_bwd_workspace_bytes(int B, int T, int D, int K, int dtype) {
+  (void)dtype;
   if (B < 1 || T < 1 || D < 1 || K < 1) return 256;
   // the widest of the two layouts
-  const Plan p = plan(B, T, D, 1), q = plan(B, T, D, dtype == TB_F32 ? 4 : 8);
+  const Plan p = plan(B, T, D, 1), q = plan(B, T, D, 4);
   return tb_align_up((size_t)(p.gy > q.gy ? p.gy : q.gy) * (K + 1) * D * 4, 256);
 }
 
@@ -393,13 +438,13 @@ int tb_conv_bwd(const void* dy, const void* x, long x_batch_stride, long x_step_
   if (ws_bytes < tb_conv_bwd_workspace_bytes(B, T, D, K, dtype)) return tb_set_error(TB_ERR_WORKSPACE, "conv_bwd: workspace too small");
   const void* ptrs[] = {x, dy, dx, state, w, bias};
   const bool vec = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 6);
-  const Plan p = plan(B, T, D, vec ? (dtype == TB_F32 ? 4 : 8) : 1);
+  const Plan p = plan(B, T, D, vec ? 4 : 1);
   rc = check_grid("conv_bwd", p);
   if (rc) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   ConvArgs a{x, w, bias, state, dy, lengths, nullptr, nullptr, dx, static_cast<float*>(ws), x_batch_stride, x_step_stride, B, T, D,
              p.run, p.runs, act, w_f32};
-  by_shape(dtype, K, vec, BwdLaunch{a, dim3((unsigned)p.gx, (unsigned)p.gy), dim3(p.bx, p.by), s});
+  by_shape<4>(dtype, K, vec, BwdLaunch{a, dim3((unsigned)p.gx, (unsigned)p.gy), dim3(p.bx, p.by), s});
   TB_LAUNCH_CHECK("conv_bwd");
   if (dw || db) {
     const long cols = (long)(K + 1) * D;
@@ -422,7 +467,7 @@ int tb_conv_step(const void* x, long x_batch_stride, void* state, long state_bat
   const void* ptrs[] = {x, y, state, w, bias};
   const bool vec = can_vec(dtype, D, x_batch_stride, state_batch_stride, ptrs, 5);
   ConvStepArgs a{x, w, bias, state, y, x_batch_stride, state_batch_stride, B, D, act, w_f32};
-  by_shape(dtype, K, vec, StepLaunch{a, static_cast<hipStream_t>(stream)});
+  by_shape<8>(dtype, K, vec, StepLaunch{a, static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("conv_step");
   return TB_OK;
 }

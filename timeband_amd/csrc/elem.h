@@ -18,9 +18,17 @@ struct alignas(sizeof(T) * N) TbVec {
   T v[N];
 };
 
+// elements an access: at most 16 bytes, and N is made of whole accesses
+template <typename T, int N>
+constexpr int tb_width() {
+  int w = 16 / sizeof(T);
+  while (N % w) w /= 2;
+  return w;
+}
+
 template <typename T, int N>
 __device__ __forceinline__ void tb_load_n(const T* p, float (&r)[N]) {
-  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;   // at most 16 bytes an access
+  constexpr int W = tb_width<T, N>();
 #pragma unroll
   for (int i = 0; i < N; i += W) {
     const TbVec<T, W> t = *reinterpret_cast<const TbVec<T, W>*>(p + i);
@@ -30,7 +38,7 @@ __device__ __forceinline__ void tb_load_n(const T* p, float (&r)[N]) {
 }
 template <typename T, int N>
 __device__ __forceinline__ void tb_store_n(T* p, const float (&r)[N]) {
-  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  constexpr int W = tb_width<T, N>();
 #pragma unroll
   for (int i = 0; i < N; i += W) {
     TbVec<T, W> t;
@@ -47,7 +55,7 @@ struct __attribute__((packed, aligned(sizeof(T)))) TbVecU {
 };
 template <typename T, int N>
 __device__ __forceinline__ void tb_load_u(const T* p, float (&r)[N]) {
-  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  constexpr int W = tb_width<T, N>();
 #pragma unroll
   for (int i = 0; i < N; i += W) {
     const TbVecU<T, W> t = *reinterpret_cast<const TbVecU<T, W>*>(p + i);
@@ -57,7 +65,7 @@ __device__ __forceinline__ void tb_load_u(const T* p, float (&r)[N]) {
 }
 template <typename T, int N>
 __device__ __forceinline__ void tb_store_u(T* p, const float (&r)[N]) {
-  constexpr int W = 16 / sizeof(T) < N ? 16 / sizeof(T) : N;
+  constexpr int W = tb_width<T, N>();
 #pragma unroll
   for (int i = 0; i < N; i += W) {
     TbVecU<T, W> t;

@@ -28,12 +28,12 @@ constexpr int YS = CB + 16;     // row length of what four lanes store for four 
 constexpr int NMAX = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// steps a tile of the backward pass.  The states of a tile stay in registers, BWD * S of them: 64 leave room for three waves
-// a SIMD, 128 for two; a state is kept in memory every BWD steps.
+// steps a tile of the backward pass.  The states of a tile stay in registers, BWD * S of them, and a state is kept in memory every
+// BWD steps.  WAVES a SIMD: what registers (and for S < 4 LDS) leave room for.
 constexpr int bwd_tile(int S) { return S <= 2 ? 32 : S <= 8 ? 16 : 8; }
 template <int S>
 struct Tile {
-  static constexpr int BWD = bwd_tile(S), WAVES = BWD * S > 64 ? 2 : 3;
+  static constexpr int BWD = bwd_tile(S), WAVES = S == 4 ? 3 : 2;
 };
 
 struct ScanArgs {
