@@ -300,12 +300,23 @@ __global__ void __launch_bounds__(256) scan_chain(ScanArgs a) {
   const float* first = REV ? a.dhT : a.h0;
   float h = first && n < a.N ? first[(b * a.D + d) * a.N + n] : 0.f;
   const int last = a.chunks - 1;
-  for (int i = 0; i < last; ++i) {
-    const int c = REV ? last - i : i;
-    const long row = (b * a.chunks + c) * a.D + d;
-    const float own = a.cstate[row * NP + n], s = a.csum[row];
-    a.cstate[row * NP + n] = h;
-    h = fmaf(__builtin_amdgcn_exp2f(A2 * s), h, own);
+  for (int i = 0; i < last; i += 8) {          // eight chunks' values fetched together: only the products wait for each other
+    float own[8], s[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = min(i + j, last - 1), c = REV ? last - k : k;
+      const long row = (b * a.chunks + c) * a.D + d;
+      own[j] = a.cstate[row * NP + n];
+      s[j] = a.csum[row];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (i + j < last) {
+        const int c = REV ? last - i - j : i + j;
+        a.cstate[((b * a.chunks + c) * a.D + d) * NP + n] = h;
+        h = fmaf(__builtin_amdgcn_exp2f(A2 * s[j]), h, own[j]);
+      }
+    }
   }
   a.cstate[((b * a.chunks + (REV ? 0 : last)) * a.D + d) * NP + n] = h;
 }
@@ -743,16 +754,22 @@ struct StepLaunch {
   }
 };
 
-// chunks of the steps: none where the channel blocks alone give the chip a block per compute unit (cutting the steps costs
-// a second walk over them), else as many as bring it to four blocks a unit, of 128 steps at least
-void plan(int B, int T, int G, int Dg, int* cblk, int* chunk, int* chunks) {
+// Chunks of the steps.  Cutting them costs a second walk (about 0.9 of the first forward, 0.2 backward), and pays where the channel
+// blocks alone leave compute units or their waves' places empty: four blocks a unit forward, three backward (two where the
+// states take more registers).  As many chunks as fill those places; forward not for fewer than three.  16-bit, 2048 channels of 16
+// states, forward / with gradients, us: 128 blocks (4 x 2048 steps) in 4, 6, 8, 12 chunks 183 / 636, 155 / 535, 143 / 554, 152 / 548;
+// 256 blocks whole 288 / 1362, in three 266 / 971, in four 247 / 1041; 384 whole 361 / 1694, in two 380 / 1420; 512 whole 183 / 891,
+// in two 230 / 1014.  Chunks of 128 steps at least, of 32 where three quarters of the units would be idle (32 blocks of 512 steps whole
+// 75 / 309, in four 44 / 135, in sixteen 28 / 82; 256 blocks of 128 steps whole 28 / 110, in four 33 / 114).
+void plan(int B, int T, int G, int Dg, int S, int backward, int* cblk, int* chunk, int* chunks) {
   *cblk = (Dg + CB - 1) / CB;
-  const long blocks = (long)B * G * *cblk;
-  const long cus = tb_num_cus();
-  long n = 1;
-  if (blocks < cus * 3 / 4) n = (4 * cus + blocks - 1) / blocks;
+  const long blocks = (long)B * G * *cblk, cus = tb_num_cus();
+  const long places = cus * (!backward ? 4 : S == 4 ? 3 : 2);
+  long n = blocks > 0 ? places / blocks : 1;
+  if (n < (backward ? 2 : 3)) n = 1;
+  const long least = blocks * 4 <= cus ? 32 : 128;
   long len = (T + n - 1) / n;
-  if (len < 128) len = 128;
+  if (len < least) len = least;
   len = (len + 31) / 32 * 32;
   *chunk = (int)len;
   *chunks = T > 0 ? (int)((T + len - 1) / len) : 1;
@@ -784,7 +801,7 @@ struct Sizes {
 };
 Sizes sizes(int B, int T, int D, int N, int G, int backward) {
   int cblk, chunk, chunks;
-  plan(B, T, G, D / G, &cblk, &chunk, &chunks);
+  plan(B, T, G, D / G, states_per_lane(N), backward, &cblk, &chunk, &chunks);
   const size_t NP = 4 * states_per_lane(N);
   Sizes z;
   z.cstate = chunks > 1 ? tb_align_up((size_t)B * chunks * D * NP * 4, 256) : 0;
@@ -828,7 +845,7 @@ int tb_scan_fwd(const void* u, const void* dt, const void* z, const void* Bm, co
   a.sub = q[0]; a.sut = q[1]; a.sdb = q[2]; a.sdt = q[3]; a.szb = q[4]; a.szt = q[5];
   a.sBb = q[6]; a.sBt = q[7]; a.sBg = q[8]; a.sCb = q[9]; a.sCt = q[10]; a.sCg = q[11];
   a.B = B; a.T = T; a.D = D; a.N = N; a.G = G; a.Dg = D / G;
-  plan(B, T, G, a.Dg, &a.cblk, &a.chunk, &a.chunks);
+  plan(B, T, G, a.Dg, S, 0, &a.cblk, &a.chunk, &a.chunks);
   a.softplus = softplus;
   a.ckt = states ? bwd_tile(S) : 0;
   a.cktiles = states ? (T + a.ckt - 1) / a.ckt : 0;
@@ -861,7 +878,7 @@ int tb_scan_bwd(const void* dout, const void* u, const void* dt, const void* z, 
   a.sBb = q[6]; a.sBt = q[7]; a.sBg = q[8]; a.sCb = q[9]; a.sCt = q[10]; a.sCg = q[11];
   a.sob = q[12]; a.sot = q[13];
   a.B = B; a.T = T; a.D = D; a.N = N; a.G = G; a.Dg = D / G;
-  plan(B, T, G, a.Dg, &a.cblk, &a.chunk, &a.chunks);
+  plan(B, T, G, a.Dg, S, 1, &a.cblk, &a.chunk, &a.chunks);
   a.softplus = softplus;
   a.ckt = bwd_tile(S);
   a.cktiles = (T + a.ckt - 1) / a.ckt;
