@@ -90,6 +90,8 @@ __device__ __forceinline__ void tb_store_par(void* p, long i, float v, int f32) 
 #define TB_ACT_SILU 4
 #define TB_ACT_LAST 5
 
+// e^x on the hardware's 2^x alone: results below 2^-126 are 0
+__device__ __forceinline__ float tb_exp(float x) { return __builtin_amdgcn_exp2f(x * 1.4426950408889634f); }
 // 1 / (1 + e^-x) on the hardware exp and reciprocal (1 ulp each): e^-x = inf gives 0, e^-x = 0 gives 1
-__device__ __forceinline__ float tb_sig(float x) { return __builtin_amdgcn_rcpf(1.f + __expf(-x)); }
+__device__ __forceinline__ float tb_sig(float x) { return __builtin_amdgcn_rcpf(1.f + tb_exp(-x)); }
 __device__ __forceinline__ float tb_silu(float x) { return x * tb_sig(x); }

@@ -43,7 +43,7 @@ __device__ __forceinline__ float half_erfc(float z) {
   p = fmaf(p, t, 0.40185486f);
   p = fmaf(p, t, 1.00138551f);
   p = fmaf(p, t, -1.48869157f);
-  return 0.5f * t * __expf(fmaf(-x, x, p));
+  return 0.5f * t * tb_exp(fmaf(-x, x, p));
 }
 __device__ __forceinline__ float act_of(float z, int act) {
   switch (act) {
@@ -61,7 +61,7 @@ __device__ __forceinline__ float act_grad(float z, int act) {
     case 2: { const float y = tb_sig(z); return y * (1.f - y); }
     case 3: return z > 0.f ? 1.f : 0.f;
     case 4: { const float y = tb_sig(z); return y * (1.f + z * (1.f - y)); }
-    case 5: { const float e = half_erfc(z); return (z > 0.f ? 1.f - e : e) + z * 0.39894228f * __expf(-0.5f * z * z); }
+    case 5: { const float e = half_erfc(z); return (z > 0.f ? 1.f - e : e) + z * 0.39894228f * tb_exp(-0.5f * z * z); }
     default: return 1.f;
   }
 }

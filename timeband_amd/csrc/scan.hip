@@ -58,8 +58,8 @@ struct ScanArgs {
 // log(1 + e^x).  With w = 1 + e rounded, log(w) e / (w - 1) repairs what the rounding of w lost (w - 1 is exact);
 // above 20 the result is x to fp32.
 __device__ __forceinline__ float softplus(float x) {
-  const float e = __expf(x), w = 1.f + e, m = w - 1.f;
-  const float l = __logf(w) * e * __builtin_amdgcn_rcpf(m);
+  const float e = tb_exp(x), w = 1.f + e, m = w - 1.f;
+  const float l = __builtin_amdgcn_logf(w) * (e / LOG2E) * __builtin_amdgcn_rcpf(m);      // the hardware's log is of base 2
   return x > 20.f ? x : m > 0.f ? l : e;
 }
 
@@ -76,20 +76,45 @@ __device__ __forceinline__ float quad_sum(float v) {
 // row; channels behind the group's last read another), so that nothing branches and all of a tile's loads are under way at
 // once: converted and masked as each arrived, they were waited for one after the other.
 template <typename T, int EPT, bool VEC>
-struct Raw {
+struct Raw;
+template <typename T, int EPT>
+struct Raw<T, EPT, true> {
+  static constexpr int WORDS = EPT * sizeof(T) / 4;
+  unsigned v[WORDS];
+  __device__ __forceinline__ void fetch(const void* base, long off, int c0, int Dg) {
+    const unsigned* q = reinterpret_cast<const unsigned*>(static_cast<const T*>(base) + off + (c0 < Dg ? c0 : 0));
+    constexpr int W = WORDS < 4 ? WORDS : 4;
+#pragma unroll
+    for (int i = 0; i < WORDS; i += W) *reinterpret_cast<TbVec<unsigned, W>*>(v + i) = *reinterpret_cast<const TbVec<unsigned, W>*>(q + i);
+  }
+  // all of a thread's channels are of the group, or none: masked as words, half as many selects for 16-bit types
+  __device__ __forceinline__ void mask(bool on, int c0, int Dg, float fill) {
+    const bool in = on && c0 < Dg;
+    const T f = (T)fill;
+    unsigned w;
+    if constexpr (sizeof(T) == 4) w = __builtin_bit_cast(unsigned, f);
+    else w = __builtin_bit_cast(unsigned short, f) * 0x10001u;
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) v[i] = in ? v[i] : w;
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, v[i]);
+    else return (float)__builtin_bit_cast(T, (unsigned short)(v[i / 2] >> (i & 1) * 16));
+  }
+};
+template <typename T, int EPT>
+struct Raw<T, EPT, false> {
   T v[EPT];
   __device__ __forceinline__ void fetch(const void* base, long off, int c0, int Dg) {
     const T* p = static_cast<const T*>(base) + off;
-    if constexpr (VEC) {
-      constexpr int W = 16 / sizeof(T) < EPT ? 16 / sizeof(T) : EPT;
-      const T* q = p + (c0 < Dg ? c0 : 0);
 #pragma unroll
-      for (int i = 0; i < EPT; i += W) *reinterpret_cast<TbVec<T, W>*>(v + i) = *reinterpret_cast<const TbVec<T, W>*>(q + i);
-    } else {
-#pragma unroll
-      for (int i = 0; i < EPT; ++i) v[i] = p[min(c0 + i, Dg - 1)];
-    }
+    for (int i = 0; i < EPT; ++i) v[i] = p[min(c0 + i, Dg - 1)];
   }
+  __device__ __forceinline__ void mask(bool on, int c0, int Dg, float fill) {
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) v[i] = on && c0 + i < Dg ? v[i] : (T)fill;
+  }
+  __device__ __forceinline__ float get(int i) const { return (float)v[i]; }
 };
 template <typename T, int EPT, bool VEC>
 __device__ __forceinline__ void put(void* base, long off, int c0, int Dg, const float (&r)[EPT]) {
@@ -227,14 +252,17 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
     const int t = t0 + ct;
     const bool on = t < tv;
     float u[EPT], z[EPT];
+    // a step that does not count leaves the state as it is: its delta is softplus(-inf) = 0
+    ru.mask(on, ch, a.Dg, 0.f);
+    if (!STATE && a.z) rz.mask(on, ch, a.Dg, 0.f);
+    rd_.mask(on, ch, a.Dg, a.softplus ? -INFINITY : 0.f);
 #pragma unroll
     for (int i = 0; i < EPT; ++i) {
-      const bool in = on && ch + i < a.Dg;
-      u[i] = in ? (float)ru.v[i] : 0.f;
-      if (!STATE && a.z) z[i] = in ? (float)rz.v[i] : 0.f;
-      float d = (in ? (float)rd_.v[i] : 0.f) + bias[i];
+      u[i] = ru.get(i);
+      if (!STATE && a.z) z[i] = rz.get(i);
+      float d = rd_.get(i) + bias[i];
       if (a.softplus) d = softplus(d);
-      d = in ? d : 0.f;                        // a step that does not count leaves the state as it is
+      else d = on ? d : 0.f;
       sD[ct][cc + i][0] = d;
       sD[ct][cc + i][1] = d * u[i];
     }
@@ -418,16 +446,18 @@ __global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(Scan
       if (a.z) rz.fetch(a.z, zo + (long)tc * a.szt, ch, a.Dg);
       if (!STATE) rB.fetch(a.Bm, bo, a.sBt, t0, tv, a.N);
       rC.fetch(a.Cm, co, a.sCt, t0, tv, a.N);
+      if (!STATE) ru.mask(on, ch, a.Dg, 0.f);
+      rdt.mask(on, ch, a.Dg, a.softplus ? -INFINITY : 0.f);
+      ro.mask(on, ch, a.Dg, 0.f);
+      if (a.z) rz.mask(on, ch, a.Dg, 0.f);
 #pragma unroll
       for (int i = 0; i < EPT; ++i) {
-        const bool in = on && ch + i < a.Dg;
-        float d = (in ? (float)rdt.v[i] : 0.f) + sPar[0][cc + i];
+        float d = rdt.get(i) + sPar[0][cc + i];
         if (a.softplus) d = softplus(d);
-        d = in ? d : 0.f;
+        else d = on ? d : 0.f;
         sD[ct][cc + i][0] = d;
-        if (!STATE) sD[ct][cc + i][1] = d * (in ? (float)ru.v[i] : 0.f);
-        const float o = in ? (float)ro.v[i] : 0.f;
-        sG[ct][cc + i] = a.z ? o * tb_silu(in ? (float)rz.v[i] : 0.f) : o;
+        if (!STATE) sD[ct][cc + i][1] = d * ru.get(i);
+        sG[ct][cc + i] = a.z ? ro.get(i) * tb_silu(rz.get(i)) : ro.get(i);
       }
       if (!STATE) rB.store(sB, t0, tv, a.N);
       rC.store(sC, t0, tv, a.N);
@@ -521,12 +551,15 @@ __global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(Scan
       }
       if (t < te) {
         float o[EPT], u[EPT];
+        // dy, delta and what the walk left are 0 where a step does not count
+        ru.mask(on, ch, a.Dg, 0.f);
+        rdt.mask(on, ch, a.Dg, a.softplus ? -INFINITY : 0.f);
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
-          const bool in = on && ch + i < a.Dg;
-          u[i] = in ? (float)ru.v[i] : 0.f;
-          o[i] = in ? fmaf(u[i], sGB[ct][cc + i], sGA[ct][cc + i] * (1.f / LOG2E)) : 0.f;
-          if (a.softplus) o[i] *= tb_sig((in ? (float)rdt.v[i] : 0.f) + sPar[0][cc + i]);      // d delta / d raw
+          u[i] = ru.get(i);
+          o[i] = fmaf(u[i], sGB[ct][cc + i], sGA[ct][cc + i] * (1.f / LOG2E));
+          if (a.softplus) o[i] *= tb_sig(rdt.get(i) + sPar[0][cc + i]);      // d delta / d raw
+          o[i] = on ? o[i] : 0.f;
           dbias[i] += o[i];
         }
         if (a.ddt) put<T, EPT, VEC>(a.ddt, oo + (long)t * a.D, ch, a.Dg, o);
@@ -538,11 +571,12 @@ __global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(Scan
         }
         if (a.du) put<T, EPT, VEC>(a.du, oo + (long)t * a.D, ch, a.Dg, o);
         if (a.dz) {
+          ro.mask(on, ch, a.Dg, 0.f);
+          rz.mask(on, ch, a.Dg, 0.f);
 #pragma unroll
           for (int i = 0; i < EPT; ++i) {
-            const bool in = on && ch + i < a.Dg;
-            const float z = in ? (float)rz.v[i] : 0.f, q = tb_sig(z), y = fmaf(sPar[1][cc + i], u[i], sY[ct][cc + i]);
-            o[i] = in ? (float)ro.v[i] * y * (q * (1.f + z * (1.f - q))) : 0.f;
+            const float z = rz.get(i), q = tb_sig(z), y = fmaf(sPar[1][cc + i], u[i], sY[ct][cc + i]);
+            o[i] = on ? ro.get(i) * y * (q * (1.f + z * (1.f - q))) : 0.f;
           }
           put<T, EPT, VEC>(a.dz, oo + (long)t * a.D, ch, a.Dg, o);
         }
