@@ -461,7 +461,7 @@ __device__ __forceinline__ u32x4 load_piece(const T* row, long k, int K, bool ve
 // up to 16 MT rows: a block owns sixteen columns, its waves take turns along K and are summed at the end
 template <typename T, int MT, int WAVES>
 __global__ void __launch_bounds__(WAVES * 64) gemm_few(FewArgs a) {
-  constexpr int CE = 16 / sizeof(T), U = 4, STEP = 4 * CE * U;
+  constexpr int CE = 16 / sizeof(T), U = MT == 1 ? 8 : 4, STEP = 4 * CE * U;
   __shared__ f32x4 red[WAVES][MT][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, row = lane & 15, piece = (lane >> 4) * CE;
   const int n0 = blockIdx.x * 16;
@@ -713,8 +713,8 @@ int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, in
     FewArgs a{x, W, ldx, ldw, M, N, K, 0, e};
     a.vec = direct<T>(x, ldx, K) && direct<T>(W, ldw, K);
     const unsigned grid = (N + 15) / 16;
-    if (M <= 16) gemm_few<T, 1, 4><<<grid, 256, 0, s>>>(a);
-    else gemm_few<T, 2, 4><<<grid, 256, 0, s>>>(a);
+    if (M <= 16) gemm_few<T, 1, 8><<<grid, 512, 0, s>>>(a);
+    else gemm_few<T, 2, 8><<<grid, 512, 0, s>>>(a);
     TB_LAUNCH_CHECK("linres gemm_few");
     return TB_OK;
   }

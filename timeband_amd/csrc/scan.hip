@@ -15,8 +15,8 @@
 // registers one tile ahead, what does not depend on the state (softplus, the gate's derivative) is computed once per element
 // by all lanes and left in LDS in fp32, then each wave walks the tile's steps with its states in registers.
 // Where the batch has too few channel blocks for the chip, the steps are cut into chunks: a first pass finds each chunk's own
-// end state from zero and the sum of its delta, a small kernel chains them (exp(A sum delta) is the chunk's decay), and the
-// main pass starts every chunk from its true state.
+// end state from zero and the sum of its delta, and the main pass starts every chunk from its true state, which it finds by chaining
+// those of the chunks before it (exp(A sum delta) is a chunk's decay).
 // States, sums and gradients of parameters are fp32; every output is rounded once.  No atomics: partial sums are added in a
 // fixed order.
 #include "elem.h"
@@ -192,6 +192,29 @@ __device__ __forceinline__ float quad_sum4(const float (&y)[4], int lane) {
   return (h ? b : a) + dpp<0x4E>(h ? a : b);
 }
 
+// The state that a chunk starts from: the chunks before it (REV: behind it), each with its own end state from zero and the sum of
+// its delta, chained from the first (REV: last) one on.  Eight are fetched together: only the products wait for each other.
+template <int S, bool REV>
+__device__ __forceinline__ void chain(const ScanArgs& a, int b, int chunk, long rd, int n0, const float (&A2)[S], float (&h)[S]) {
+  constexpr int NP = 4 * S;
+  const int count = REV ? a.chunks - 1 - chunk : chunk;
+  for (int i = 0; i < count; i += 8) {
+    float own[8][S], sum[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int k = min(i + j, count - 1);
+      const long row = ((long)b * a.chunks + (REV ? a.chunks - 1 - k : k)) * a.D + rd;
+      load_row<S>(a.cstate + row * NP + n0, own[j]);
+      sum[j] = a.csum[row];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (i + j < count)
+#pragma unroll
+        for (int s = 0; s < S; ++s) h[s] = fmaf(__builtin_amdgcn_exp2f(A2[s] * sum[j]), h[s], own[j][s]);
+  }
+}
+
 // forward.  STATE: only the chunk's end state from zero and its sum of delta (first pass over chunks).
 template <typename T, int S, bool STATE, bool VEC>
 __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
@@ -217,13 +240,9 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
   if (STATE) {
 #pragma unroll
     for (int s = 0; s < S; ++s) h[s] = 0.f;
-  } else if (a.chunks > 1) {
-    if (ron) load_row<S>(a.cstate + (((long)w.b * a.chunks + w.chunk) * a.D + rd) * NP + n0, h);
-    else
-#pragma unroll
-      for (int s = 0; s < S; ++s) h[s] = 0.f;
   } else {
     load_state<S>(a.h0, (long)w.b * a.D + rd, n0, a.N, ron, h);
+    if (ron) chain<S, false>(a, w.b, w.chunk, rd, n0, A2, h);
   }
   float bias[EPT], Dp[EPT];
 #pragma unroll
@@ -316,39 +335,6 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
   }
 }
 
-// chunks' own end states -> their start states (forward: from h0 on; REV: from the last chunk's dhT back)
-template <int S, bool REV>
-__global__ void __launch_bounds__(256) scan_chain(ScanArgs a) {
-  constexpr int NP = 4 * S;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  if (id >= (long)a.B * a.D * NP) return;
-  const int n = (int)(id % NP);
-  const long d = id / NP % a.D, b = id / NP / a.D;
-  const float A2 = n < a.N ? a.A[d * a.N + n] * LOG2E : 0.f;
-  const float* first = REV ? a.dhT : a.h0;
-  float h = first && n < a.N ? first[(b * a.D + d) * a.N + n] : 0.f;
-  const int last = a.chunks - 1;
-  for (int i = 0; i < last; i += 8) {          // eight chunks' values fetched together: only the products wait for each other
-    float own[8], s[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const int k = min(i + j, last - 1), c = REV ? last - k : k;
-      const long row = (b * a.chunks + c) * a.D + d;
-      own[j] = a.cstate[row * NP + n];
-      s[j] = a.csum[row];
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (i + j < last) {
-        const int c = REV ? last - i - j : i + j;
-        a.cstate[((b * a.chunks + c) * a.D + d) * NP + n] = h;
-        h = fmaf(__builtin_amdgcn_exp2f(A2 * s[j]), h, own[j]);
-      }
-    }
-  }
-  a.cstate[((b * a.chunks + (REV ? 0 : last)) * a.D + d) * NP + n] = h;
-}
-
 // v[0..2S) of the wave's sixteen channels (lane bits 2..5) summed: halves are exchanged so that each step adds what is left,
 // and the lanes with bits 2 and 3 clear end with S/2 sums each (S = 1: one), of v[0..S) in the lower half of the wave and of
 // v[S..2S) in the upper; bit 4 says which half of the S.
@@ -416,11 +402,8 @@ __global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(Scan
     g[s] = 0.f;
   }
   if (!STATE) {
-    if (a.chunks > 1) {
-      if (ron) load_row<S>(a.cstate + (((long)w.b * a.chunks + w.chunk) * a.D + rd) * NP + n0, g);
-    } else {
-      load_state<S>(a.dhT, (long)w.b * a.D + rd, n0, a.N, ron, g);
-    }
+    load_state<S>(a.dhT, (long)w.b * a.D + rd, n0, a.N, ron, g);
+    if (ron) chain<S, true>(a, w.b, w.chunk, rd, n0, A2, g);
   }
   float dD[EPT], dbias[EPT];
 #pragma unroll
@@ -746,10 +729,7 @@ struct FwdLaunch {
   }
   template <typename T, int S, bool VEC>
   int run() {
-    if (a.chunks > 1) {
-      scan_fwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
-      scan_chain<S, false><<<(unsigned)(((long)a.B * a.D * 4 * S + 255) / 256), 256, 0, s>>>(a);
-    }
+    if (a.chunks > 1) scan_fwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
     scan_fwd<T, S, false, VEC><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
     return 0;
   }
@@ -766,10 +746,7 @@ struct BwdLaunch {
   }
   template <typename T, int S, bool VEC>
   int run() {
-    if (a.chunks > 1) {
-      scan_bwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
-      scan_chain<S, true><<<(unsigned)(((long)a.B * a.D * 4 * S + 255) / 256), 256, 0, s>>>(a);
-    }
+    if (a.chunks > 1) scan_bwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
     scan_bwd<T, S, false, VEC><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
     if (dA || dD || dbias)
       scan_finish_par<<<(unsigned)(((long)a.D * (4 * S + 2) + 63) / 64), 256, 0, s>>>(a.par, a.B * a.chunks, a.D, a.N, 4 * S, dA, dD, dbias);
