@@ -342,8 +342,8 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
 }
 
 // v[0..2S) of the wave's sixteen channels (lane bits 2..5) summed: halves are exchanged so that each step adds what is left,
-// and the lanes with bits 2 and 3 clear end with S/2 sums each (S = 1: one), of v[0..S) in the lower half of the wave and of
-// v[S..2S) in the upper; bit 4 says which half of the S.
+// and every lane ends with S/2 sums (S = 1: one), of v[0..S) in the lower half of the wave and of v[S..2S) in the upper; bit 4 says
+// which half of the S, bits 2 and 3 nothing.
 template <int S>
 __device__ __forceinline__ void channel_sum(float (&v)[2 * S]) {
 #pragma unroll
@@ -516,7 +516,9 @@ __global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(Scan
         }
         channel_sum<S>(v);
         constexpr int H = S > 1 ? S / 2 : 1;
-        if ((lane & 12) == 0 && (S > 1 || (lane & 16) == 0)) {
+        // Lanes that differ in bits 2 and 3 hold and store the same: selecting one of them costs a branch a step (16 x 1024 x 2048
+        // bf16 with gradients 861 us, without 813), which pays only where a lane stores many sums (64 states: 202 us, without 227).
+        if (S <= 8 || (lane & 12) == 0) {
           float* p = &sP[wave][k][(lane >> 5) * NP + n0 + (S > 1 && (lane & 16) ? H : 0)];
 #pragma unroll
           for (int i = 0; i < H; ++i) p[i] = v[i];
