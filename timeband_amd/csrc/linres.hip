@@ -4,8 +4,8 @@
 //
 // One matrix kernel serves all three products: C[m][n] = sum_k P[m][k] Q[n][k] with k running along the rows of both operands,
 // which is what a matrix instruction's lanes want (16 neighbouring bytes each).  For dx and dW the operands are written once
-// with their axes exchanged (W, x and dz: 2 bytes an element moved against K or M operations on it); the kernel that forms
-// dz = dy act'(z) writes both orders and the column sums of db in its one pass.
+// with their axes exchanged (W, x and dz: 2 bytes an element moved against K or M operations on it; fp32 takes dW's as they are);
+// the kernel that forms dz = dy act'(z) writes both orders and the column sums of db in its one pass.
 // 16-bit operands go through v_mfma_f32_16x16x32, fp32 ones through v_mfma_f32_16x16x4 (exact fp32 products: no splitting
 // into 16-bit parts, so infinities and the type's whole range pass).  Sums are fp32, z is kept in fp32 for the gradient (kept in 16 bits it
 // would add a second rounding to act'), and dz is rounded to the operands' type because it enters the matrix instructions.
@@ -226,7 +226,7 @@ __device__ __forceinline__ void whole_rows(const GemmArgs& a, const float* own, 
   }
 }
 
-// 64 x 64 sums of a wave, in LDS as gemm_nt leaves them, through the epilogue to memory
+// 64 x 64 sums of a wave, in LDS as gemm leaves them, through the epilogue to memory
 template <typename T>
 __device__ __forceinline__ void write_block(const GemmArgs& a, const float* own, long m0, int n0, int lane) {
   const Epi& e = a.e;
@@ -262,8 +262,14 @@ __device__ __forceinline__ void write_block(const GemmArgs& a, const float* own,
 // from LDS and the copies of the three behind it are under way.  One barrier a tile: behind it the tile that was just read into
 // registers by every wave is free for a new copy, and the next one has landed (the copies still under way are counted, not
 // drained).
-template <typename T, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm_nt(GemmArgs a) {
+//
+// DOWN (fp32, for dW): k runs down the columns of both operands as they are, P[k][m] and Q[k][n], K rows of M and N columns that are
+// whole 16-byte pieces on 16 bytes.  A tile is sixteen rows of BM (BN) columns; a lane takes its k one by one (4 bytes), which the
+// fp32 instructions, a quarter of the 16-bit ones' rate a byte, leave time for.  Saves the transposed copies of dz and x
+// (65536 x 256 x 256: 345 -> 300 us of a training step).
+template <typename T, int BM, int BN, int WM, int WN, bool DOWN>
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm(GemmArgs a) {
+  static_assert(!DOWN || (sizeof(T) == 4 && BM == 128 && BN == 128), "rows of 512 bytes, two a copy");
   constexpr int WAVES = (BM / WM) * (BN / WN), CE = 16 / sizeof(T), BK = 4 * CE;
   constexpr int MF = WM / 16, NF = WN / 16, LP = BM / 16 / WAVES, LQ = BN / 16 / WAVES;
   constexpr int STAGE = (BM + BN) * 64;
@@ -277,22 +283,39 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm_nt(GemmArg
   const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
   const int kt0 = blockIdx.y * a.per, nt = min(a.per, (a.K + BK - 1) / BK - kt0);
 
-  // what this lane copies: row 16 i + lane / 4 of each of its pieces, and of that row's four 16-byte pieces the one whose place
-  // in LDS is lane % 4: piece p of row r lies at p ^ (r / 2 % 4), so that eight neighbouring rows fill all banks
-  const int lr = lane >> 2, piece = ((lane & 3) ^ ((lr >> 1) & 3)) * CE;
+  // What this lane copies: row 16 i + lane / 4 of each of its pieces, and of that row's four 16-byte pieces the one whose place
+  // in LDS is lane % 4: piece p of row r lies at p ^ (r / 2 % 4), so that eight neighbouring rows fill all banks.
+  // DOWN: row 2 i + lane / 32 of the tile's sixteen, of 32 pieces; piece p of row r lies at p ^ (r % 4 * 4), so that the four rows
+  // of a read fall on different banks.
+  const int lr = DOWN ? lane >> 5 : lane >> 2;
+  const int piece = (DOWN ? (lane & 31) : (lane & 3) ^ ((lr >> 1) & 3)) * CE;
   const T* pp[LP];
   const T* qp[LQ];
+  int pr[LP], qr[LQ];              // DOWN: the row within a tile, or past every K where the columns are behind the last
 #pragma unroll
   for (int i = 0; i < LP; ++i) {
-    long r = m0 + (wave * LP + i) * 16 + lr;
-    r = r < a.M ? r : a.M - 1;                  // rows behind the last: any row, never stored
-    pp[i] = static_cast<const T*>(a.P) + r * a.ldp + piece;
+    if constexpr (DOWN) {
+      const int row = (wave * LP + i) * 2 + lr;
+      const long c = m0 + (piece ^ (row & 3) * 16);
+      pp[i] = static_cast<const T*>(a.P) + (c < a.M ? c : 0) + row * a.ldp;
+      pr[i] = c < a.M ? row : 1 << 30;
+    } else {
+      long r = m0 + (wave * LP + i) * 16 + lr;
+      r = r < a.M ? r : a.M - 1;                // rows behind the last: any row, never stored
+      pp[i] = static_cast<const T*>(a.P) + r * a.ldp + piece;
+    }
   }
 #pragma unroll
   for (int i = 0; i < LQ; ++i) {
-    int r = n0 + (wave * LQ + i) * 16 + lr;
-    r = r < a.N ? r : a.N - 1;
-    qp[i] = static_cast<const T*>(a.Q) + (long)r * a.ldq + piece;
+    if constexpr (DOWN) {
+      const int row = (wave * LQ + i) * 2 + lr, c = n0 + (piece ^ (row & 3) * 16);
+      qp[i] = static_cast<const T*>(a.Q) + (c < a.N ? c : 0) + row * a.ldq;
+      qr[i] = c < a.N ? row : 1 << 30;
+    } else {
+      int r = n0 + (wave * LQ + i) * 16 + lr;
+      r = r < a.N ? r : a.N - 1;
+      qp[i] = static_cast<const T*>(a.Q) + (long)r * a.ldq + piece;
+    }
   }
   // TAIL: the tile may reach behind the end of K, whose pieces come from a row of zeros
   auto copy = [&](int t, auto tail) {
@@ -301,22 +324,38 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm_nt(GemmArg
     const bool in_k = !tail || k + piece < a.K;
     const uintptr_t zero = reinterpret_cast<uintptr_t>(g_zeros);
 #pragma unroll
-    for (int i = 0; i < LP; ++i)
-      __builtin_amdgcn_global_load_lds((gvoid*)(in_k ? reinterpret_cast<uintptr_t>(pp[i] + k) : zero),
-                                       (lvoid*)(to + (wave * LP + i) * 1024), 16, 0, 0);
+    for (int i = 0; i < LP; ++i) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(pp[i] + (DOWN ? k * a.ldp : k));
+      __builtin_amdgcn_global_load_lds((gvoid*)((DOWN ? k + pr[i] < a.K : in_k) ? at : zero), (lvoid*)(to + (wave * LP + i) * 1024), 16, 0, 0);
+    }
 #pragma unroll
-    for (int i = 0; i < LQ; ++i)
-      __builtin_amdgcn_global_load_lds((gvoid*)(in_k ? reinterpret_cast<uintptr_t>(qp[i] + k) : zero),
-                                       (lvoid*)(to + BM * 64 + (wave * LQ + i) * 1024), 16, 0, 0);
+    for (int i = 0; i < LQ; ++i) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(qp[i] + (DOWN ? k * a.ldq : k));
+      __builtin_amdgcn_global_load_lds((gvoid*)((DOWN ? k + qr[i] < a.K : in_k) ? at : zero), (lvoid*)(to + BM * 64 + (wave * LQ + i) * 1024), 16, 0, 0);
+    }
   };
   const int place = ((lane >> 4) ^ ((lane >> 1) & 3)) * 16;
   const int po = (wm + (lane & 15)) * 64 + place, qo = BM * 64 + (wn + (lane & 15)) * 64 + place;
   auto read = [&](int t, u32x4 (&fp)[MF], u32x4 (&fq)[NF]) {
     const char* from = lds + (t & 3) * STAGE;
+    if constexpr (DOWN) {
+      // k = 4 j + lane / 16 of column lane % 16: in the j-th instruction's order of k
+      const int row = (lane >> 4) * 512, col = lane & 15, turn = (lane >> 4) * 16;
 #pragma unroll
-    for (int j = 0; j < NF; ++j) fq[j] = *reinterpret_cast<const u32x4*>(from + qo + j * 1024);
+      for (int j = 0; j < 4; ++j) {
 #pragma unroll
-    for (int i = 0; i < MF; ++i) fp[i] = *reinterpret_cast<const u32x4*>(from + po + i * 1024);
+        for (int i = 0; i < NF; ++i)
+          fq[i][j] = *reinterpret_cast<const unsigned*>(from + BM * 64 + j * 2048 + row + (((wn + i * 16) ^ turn) + col) * 4);
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+          fp[i][j] = *reinterpret_cast<const unsigned*>(from + j * 2048 + row + (((wm + i * 16) ^ turn) + col) * 4);
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < NF; ++j) fq[j] = *reinterpret_cast<const u32x4*>(from + qo + j * 1024);
+#pragma unroll
+      for (int i = 0; i < MF; ++i) fp[i] = *reinterpret_cast<const u32x4*>(from + po + i * 1024);
+    }
   };
 
   f32x4 acc[MF][NF];
@@ -653,11 +692,11 @@ struct Plan {
 };
 // 256 x 256 tiles where they fill the chip, 128 x 128 otherwise (two blocks a unit).  k is split where even those leave units
 // idle, into parts of sixteen k tiles (1 KB of a row) at least.
-Plan plan(long M, int N, long K, int esize) {
+Plan plan(long M, int N, long K, int esize, bool down = false) {
   Plan p;
   const long cus = tb_num_cus(), kt = (K * esize + 63) / 64;
   const long big = ((M + 255) / 256) * ((N + 255) / 256);
-  p.big = big >= cus;
+  p.big = big >= cus && !down;
   const int b = p.big ? 256 : 128;
   p.tm = (int)((M + b - 1) / b);
   p.tn = (N + b - 1) / b;
@@ -673,14 +712,14 @@ Plan plan(long M, int N, long K, int esize) {
   p.splits = (int)((kt + p.per - 1) / p.per);
   return p;
 }
-size_t slab_bytes(long M, int N, long K, int esize) {
-  const Plan p = plan(M, N, K, esize);
+size_t slab_bytes(long M, int N, long K, int esize, bool down = false) {
+  const Plan p = plan(M, N, K, esize, down);
   return p.splits > 1 ? tb_align_up((size_t)p.splits * M * N * 4, 256) : 0;
 }
 
-template <typename T>
+template <typename T, bool DOWN = false>
 int launch_gemm(const T* P, long ldp, const T* Q, long ldq, long M, int N, long K, Epi e, float* slab, hipStream_t s) {
-  const Plan p = plan(M, N, K, sizeof(T));
+  const Plan p = plan(M, N, K, sizeof(T), DOWN);
   GemmArgs a{P, Q, ldp, ldq, M, N, (int)K, p.tm, p.tn, p.splits, p.per, 16 / (int)sizeof(T), e};
   auto whole = [&](int w) {
     const uintptr_t bytes = w * sizeof(T);
@@ -690,8 +729,9 @@ int launch_gemm(const T* P, long ldp, const T* Q, long ldq, long M, int N, long 
   while (a.width > 1 && !whole(a.width)) a.width /= 2;
   a.e.slab = p.splits > 1 ? slab : nullptr;
   const dim3 grid(p.tm * p.tn, p.splits);
-  if (p.big) gemm_nt<T, 256, 256, 128, 64><<<grid, 512, 0, s>>>(a);
-  else gemm_nt<T, 128, 128, 64, 64><<<grid, 256, 0, s>>>(a);
+  if constexpr (DOWN) gemm<T, 128, 128, 64, 64, true><<<grid, 256, 0, s>>>(a);
+  else if (p.big) gemm<T, 256, 256, 128, 64, false><<<grid, 512, 0, s>>>(a);
+  else gemm<T, 128, 128, 64, 64, false><<<grid, 256, 0, s>>>(a);
   TB_LAUNCH_CHECK("linres gemm");
   if (p.splits > 1) {
     split_finish<T><<<(unsigned)((M * ((N + 3) / 4) + 63) / 64), 256, 0, s>>>(a.e, M, N, p.splits);
@@ -754,8 +794,9 @@ BwdSizes bwd_sizes(long M, int K, int N, int es) {
   b.WT = tb_align_up((size_t)K * b.Np * es, 256);
   b.xT = tb_align_up((size_t)K * b.Mp * es, 256);
   b.part = tb_align_up((size_t)((M + 63) / 64) * N * 4, 256);
-  const size_t s1 = slab_bytes(M, K, up(N, es), es), s2 = slab_bytes(N, K, up(M, es), es);
+  const size_t s1 = slab_bytes(M, K, up(N, es), es), s2 = slab_bytes(N, K, up(M, es), es), s3 = slab_bytes(N, K, M, es, true);
   b.slab = s1 > s2 ? s1 : s2;
+  if (s3 > b.slab) b.slab = s3;
   b.total = b.dz + b.dzT + b.WT + b.xT + b.part + b.slab + 256;
   return b;
 }
@@ -773,9 +814,11 @@ int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, 
   const bool as_is = !z && direct<T>(dy, ldy, N);      // dz = dy, and its rows can be copied as they are
   const T* dzr = as_is ? dy : dz;
   const long ldz = as_is ? ldy : b.Np;
-  if (!as_is || dW || db) {
+  const bool down = sizeof(T) == 4 && dW && direct<T>(x, ldx, K);      // dW from dz and x as they are
+  const bool across = dW && !down;
+  if (!as_is || across || db) {
     form_dz<T><<<dim3((unsigned)((M + 63) / 64), (unsigned)((b.Np + 63) / 64)), 256, 0, s>>>(
-        dy, ldy, z, act, M, N, as_is || !dx ? nullptr : dz, (int)b.Np, dW ? dzT : nullptr, b.Mp, db ? part : nullptr);
+        dy, ldy, z, act, M, N, as_is || !(dx || down) ? nullptr : dz, (int)b.Np, across ? dzT : nullptr, b.Mp, db ? part : nullptr);
     TB_LAUNCH_CHECK("linres form_dz");
   }
   if (db) {
@@ -790,7 +833,14 @@ int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, 
     const int rc = launch_gemm<T>(dzr, ldz, WT, b.Np, M, K, up(N, sizeof(T)), e, slab, s);
     if (rc) return rc;
   }
-  if (dW) {
+  if constexpr (sizeof(T) == 4) {
+    if (down) {
+      e.y = dW;
+      const int rc = launch_gemm<T, true>(dzr, ldz, x, ldx, N, K, M, e, slab, s);
+      if (rc) return rc;
+    }
+  }
+  if (across) {
     transpose<T><<<dim3((unsigned)((b.Mp + 63) / 64), (unsigned)((K + 63) / 64)), 256, 0, s>>>(x, ldx, M, K, xT, b.Mp);
     TB_LAUNCH_CHECK("linres transpose");
     e.y = dW;
@@ -802,7 +852,7 @@ int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, 
 
 int check_common(const char* what, long M, int K, int N, int act, int dtype) {
   // the tile counts and the transposes' grids are 32 and 16 bits wide
-  if (M < 0 || K < 1 || N < 1 || K > 4000000 || N > 4000000 || M > (1L << 31)) return tb_set_error(TB_ERR_ARG, "%s: bad sizes M=%ld K=%d N=%d", what, M, K, N);
+  if (M < 0 || K < 1 || N < 1 || K > 4000000 || N > 4000000 || M > 2000000000L) return tb_set_error(TB_ERR_ARG, "%s: bad sizes M=%ld K=%d N=%d", what, M, K, N);
   if (act < 0 || act > TB_ACT_LAST) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: activation %d is not supported", what, act);
   if (!tb_dtype_ok(dtype)) return tb_set_error(TB_ERR_ARG, "%s: bad element type %d", what, dtype);
   return TB_OK;
