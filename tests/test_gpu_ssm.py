@@ -344,6 +344,95 @@ def test_linear_no_rows():
     assert g[0].shape == x.shape and not g[1].any() and not g[2].any()
 
 
+def test_what_lies_between_rows_is_not_used():
+    """NaN in the gaps between rows (and behind the last columns of a tile's k): the same results as from dense tensors."""
+    from timeband_amd import ops
+    for type, M, K, N in itertools.product((FP, BF, HF), (5, 200), (24, 40, 45), (24,)):
+        x, W, res, dy = rnd(1, M, K, type=type), rnd(2, N, K, type=type), rnd(3, M, N, type=type), rnd(4, M, N, type=type)
+        gap = lambda t: torch.cat([t, torch.full((t.shape[0], 16), NAN, dtype=type, device="cuda")], 1)[:, :t.shape[1]]
+        out = []
+        for f in (lambda t: t.clone(), gap):
+            a = [f(t).detach().requires_grad_(True) for t in (x, W, res)]
+            y = ops.linear_residual(a[0], a[1], None, ops.ACT_GELU, residual=a[2])
+            out.append([y, *torch.autograd.grad(y, a, f(dy))])
+        assert all(torch.equal(p, q) for p, q in zip(*out)), (type, M, K)
+        x, w = rnd(5, 2, 37, K, type=type), rnd(6, K, 4, type=type)
+        wide = torch.full((2, 37, K + 16), NAN, dtype=type, device="cuda")
+        wide[..., :K] = x
+        out = []
+        for v in (x, wide[..., :K]):
+            v = v.detach().requires_grad_(True)
+            y = ops.causal_conv(v, w, None, ops.ACT_SILU)
+            t = scan_inputs(2, 37, K, 6, 1, type, False, False)
+            h = ops.selective_scan(v, v, t["A"], t["Bm"], t["Cm"], z=v)
+            out.append([y, h, *torch.autograd.grad((y, h), v, (x, x))])
+        assert all(torch.equal(p, q) for p, q in zip(*out)), (type, K)
+
+
+def test_lengths_outside_the_steps_are_taken_as_the_nearest():
+    from timeband_amd import ops
+    x, w = rnd(1, 3, 10, 16), rnd(2, 16, 4)
+    t = scan_inputs(3, 10, 16, 4, 1, FP, True, True)
+    for f in (lambda ln: ops.causal_conv(x, w, lengths=ln, return_state=True), lambda ln: call_scan(t, lengths=ln, return_state=True)):
+        assert all(torch.equal(p, q) for p, q in zip(f(ints([-3, 99, 4])), f(ints([0, 10, 4]))))
+
+
+def test_tensors_of_more_than_2_31_elements():
+    """Offsets behind 2^31 elements: the last rows of one large call against a call on those rows alone."""
+    from timeband_amd import ops
+    D, T = 32768, 70000                     # 2.3 G elements
+    x = torch.zeros(1, T, D, dtype=BF, device="cuda")
+    x[:, -40:] = rnd(1, 1, 40, D, type=BF)
+    w = rnd(2, D, 4, type=BF)
+    y, st = ops.causal_conv(x, w, None, ops.ACT_SILU, return_state=True)
+    assert torch.equal(y[:, -30:], ops.causal_conv(x[:, -40:], w, None, ops.ACT_SILU)[:, -30:]) and torch.equal(st, x[:, -3:])
+    del y
+    A = torch.full((D, 4), -0.5, device="cuda")
+    B = rnd(3, 1, T, 4, type=BF)
+    y, h = ops.selective_scan(x, x, A, B, B, return_state=True)
+    # the steps before are of zeros: they leave the state at 0
+    y2, h2 = ops.selective_scan(x[:, -40:], x[:, -40:], A, B[:, -40:], B[:, -40:], return_state=True)
+    assert float((y[:, -40:].float() - y2.float()).norm() / y2.float().norm()) < 2.0 ** -7 and float((h - h2).norm() / h2.norm()) < 1e-4
+    del y
+    W = rnd(4, 40, D, type=BF, scale=D ** -0.5)
+    flat = x[0]
+    y = ops.linear_residual(flat, W)
+    y2 = ops.linear_residual(flat[-64:], W)
+    assert not y[:-40].any() and float((y[-64:].float() - y2.float()).norm() / y2.float().norm()) < 2.0 ** -7
+
+
+def test_gradients_into_a_flat_buffer():
+    """Parameters of a FlatParams module (what the trainer's optimizer works on): the gradients land in its buffer, added up."""
+    from timeband_amd import ops, optim
+    lin = torch.nn.Linear(24, 40).cuda()
+    flat = optim.FlatParams(lin)
+    x, dy = rnd(1, 50, 24), rnd(2, 50, 40)
+    want = torch.autograd.grad(ops.linear_residual(x, lin.weight, lin.bias, ops.ACT_SILU), (lin.weight, lin.bias), dy)
+    for _ in range(2):
+        ops.linear_residual(x, lin.weight, lin.bias, ops.ACT_SILU).backward(dy)
+    assert torch.equal(flat.grad[:960].view(40, 24), want[0] + want[0]) and torch.equal(flat.grad[960:], want[1] + want[1])
+
+
+def test_captured_steps_move_their_states():
+    """A token's path captured once and replayed: each replay reads the input buffer and moves the states, as eager calls do."""
+    p = layer(type=BF)
+    with torch.no_grad():
+        x = rnd(95, 6, 3, 40, type=BF)
+        _, cs, h = run_layer(p, rnd(94, 3, 9, 40, type=BF))
+        cs2, h2, buf = cs.clone(), h.clone(), x[0].clone()
+        step_layer(p, buf, cs.clone(), h.clone())
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step_layer(p, buf, cs2, h2)
+        for i in range(6):
+            buf.copy_(x[i])
+            g.replay()
+            want = step_layer(p, x[i], cs, h)
+            torch.cuda.synchronize()
+            assert torch.equal(out, want) and torch.equal(cs, cs2) and torch.equal(h, h2)
+
+
 # ---- all of them ---------------------------------------------------------------------------------------------------------
 def layer(D=64, N=16, R_=8, model=40, K=4, type=FP, seed=50):
     """The weights of one state space layer: in-projection, convolution, what makes dt, B and C, scan, out-projection."""

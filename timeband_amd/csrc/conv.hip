@@ -24,6 +24,7 @@ struct ConvArgs {
   long sxb, sxt;             // strides of x in elements; y, dy, dx, state are dense
   int B, T, D, run, runs;    // runs of `run` steps each, `runs` of them a sequence
   int act, wf32;
+  unsigned gx;               // blocks along the channels; blocks go along them first
 };
 
 template <typename T, int VEC>
@@ -78,8 +79,8 @@ struct Rows {
 // block: blockDim.x channel groups of VEC by blockDim.y runs
 template <typename T, int K, int VEC>
 __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
-  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * VEC;
-  const long r = (long)blockIdx.y * blockDim.y + threadIdx.y;
+  const int c = (blockIdx.x % a.gx * blockDim.x + threadIdx.x) * VEC;
+  const long row = blockIdx.x / a.gx, r = row * blockDim.y + threadIdx.y;
   if (c >= a.D || r >= (long)a.B * a.runs) return;
   const int b = (int)(r / a.runs), q = (int)(r % a.runs);
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
@@ -133,8 +134,8 @@ __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
 template <typename T, int K, int VEC>
 __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
   __shared__ float red[256][VEC];
-  const int c = (blockIdx.x * blockDim.x + threadIdx.x) * VEC;
-  const long r = (long)blockIdx.y * blockDim.y + threadIdx.y;
+  const int c = (blockIdx.x % a.gx * blockDim.x + threadIdx.x) * VEC;
+  const long row = blockIdx.x / a.gx, r = row * blockDim.y + threadIdx.y;
   const bool on = c < a.D && r < (long)a.B * a.runs;
   float dw[K + 1][VEC];
 #pragma unroll
@@ -230,7 +231,7 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
       for (int j = 0; j < (int)blockDim.y; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] += red[j * blockDim.x + threadIdx.x][i];
-      tb_store_n(a.slab + ((long)blockIdx.y * (K + 1) + k) * a.D + c, o);
+      tb_store_n(a.slab + (row * (K + 1) + k) * a.D + c, o);
     }
     __syncthreads();
   }
@@ -391,9 +392,9 @@ bool can_vec(int dtype, int D, long sb, long st, const void* const* p, int n) {
   return true;
 }
 
-// grid.y is 16 bits wide in some launch paths; the runs' blocks stay far below that
+// a launch has at most 2^32 threads
 int check_grid(const char* what, const Plan& p) {
-  if (p.gy > 65535 || p.gx > 0x7fffffffL) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: too many sequences in one call", what);
+  if (p.gx * p.gy >= 1L << 24) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: too many steps in one call", what);
   return TB_OK;
 }
 
@@ -414,8 +415,8 @@ int tb_conv_fwd(const void* x, long x_batch_stride, long x_step_stride, const vo
   rc = check_grid("conv_fwd", p);
   if (rc) return rc;
   ConvArgs a{x, w, bias, state, nullptr, lengths, y, state_out, nullptr, nullptr, x_batch_stride, x_step_stride, B, T, D, p.run,
-             p.runs, act, w_f32};
-  by_shape<8>(dtype, K, vec, FwdLaunch{a, dim3((unsigned)p.gx, (unsigned)p.gy), dim3(p.bx, p.by), static_cast<hipStream_t>(stream)});
+             p.runs, act, w_f32, (unsigned)p.gx};
+  by_shape<8>(dtype, K, vec, FwdLaunch{a, dim3((unsigned)(p.gx * p.gy)), dim3(p.bx, p.by), static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("conv_fwd");
   return TB_OK;
 }
@@ -443,8 +444,8 @@ int tb_conv_bwd(const void* dy, const void* x, long x_batch_stride, long x_step_
   if (rc) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   ConvArgs a{x, w, bias, state, dy, lengths, nullptr, nullptr, dx, static_cast<float*>(ws), x_batch_stride, x_step_stride, B, T, D,
-             p.run, p.runs, act, w_f32};
-  by_shape<4>(dtype, K, vec, BwdLaunch{a, dim3((unsigned)p.gx, (unsigned)p.gy), dim3(p.bx, p.by), s});
+             p.run, p.runs, act, w_f32, (unsigned)p.gx};
+  by_shape<4>(dtype, K, vec, BwdLaunch{a, dim3((unsigned)(p.gx * p.gy)), dim3(p.bx, p.by), s});
   TB_LAUNCH_CHECK("conv_bwd");
   if (dw || db) {
     const long cols = (long)(K + 1) * D;
