@@ -8,8 +8,10 @@
 //   ddelta = sum_n q A + u sum_n g B,  du = delta sum_n g B + D dy,  dA = sum q delta,  dB_t = sum_c g delta u,
 //   dC_t = sum_c dy h,  dD = sum dy u,  dz = dout y silu'(z),  ddt = ddelta sigmoid(dt + bias)
 //
-// Bound by arithmetic: an exponential (a quarter of the vector rate) and four other operations a state and step forward, two
-// exponentials and about fourteen backward, against two bytes an element and tensor.  Layout: a lane owns one channel and S = N/4 of
+// Bound by arithmetic: an exponential (a quarter of the vector rate) and four other operations a state and step forward, as many again and
+// nine more backward, against two bytes an element and tensor; where the steps are cut, the first walk comes on top.  Measured, bf16,
+// 16 states, gated: 1 x 16384 x 2048 267 us (537 M state steps; the exponentials and operations of both walks alone are 215 at
+// the vector units' full rate); 4 x 2048 x 2048 with gradients 480.  Layout: a lane owns one channel and S = N/4 of
 // its states, four neighbouring lanes a channel, so that the sum over the states is two quad permutes and a block of four
 // waves owns 64 neighbouring channels (whole lines of every tensor).  Steps go in tiles: a tile's rows are fetched into
 // registers one tile ahead, what does not depend on the state (softplus, the gate's derivative) is computed once per element
@@ -28,12 +30,13 @@ constexpr int YS = CB + 16;     // row length of what four lanes store for four 
 constexpr int NMAX = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
-// steps a tile of the backward pass.  The states of a tile stay in registers, BWD * S of them, and a state is kept in memory every
-// BWD steps.  WAVES a SIMD: what registers (and for S < 4 LDS) leave room for.
+// steps a tile of the backward pass.  The states of a tile stay in registers, BWD * S of them, and up to S = 4 as many decays (computed
+// again on the way back, with three waves a SIMD instead of two: 16 x 1024 x 2048 bf16 818 us, so 721; beyond, they would spill:
+// 32 states 250 us, so 512).  A state is kept in memory every BWD steps.
 constexpr int bwd_tile(int S) { return S <= 2 ? 32 : S <= 8 ? 16 : 8; }
 template <int S>
 struct Tile {
-  static constexpr int BWD = bwd_tile(S), WAVES = S == 4 ? 3 : 2;
+  static constexpr int BWD = bwd_tile(S);
 };
 
 struct ScanArgs {
@@ -379,7 +382,7 @@ struct Row {
 
 // backward.  STATE: only g in front of the chunk's first step from zero behind its last, and its sum of delta.
 template <typename T, int S, bool STATE, bool VEC>
-__global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(ScanArgs a) {
+__global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
   constexpr int TT = STATE ? 32 : Tile<S>::BWD, EPT = TT / 4, NP = 4 * S;
   __shared__ float sD[TT][CB][2], sG[TT][CB];           // delta, delta u; dy
   __shared__ float sB[STATE ? 1 : TT * NP], sC[TT * NP];
@@ -463,6 +466,8 @@ __global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(Scan
         for (int s = 0; s < S; ++s) g[s] = fmaf(cv[s], y, g[s]) * __builtin_amdgcn_exp2f(d * A2[s]);
       }
     } else {
+      constexpr bool KEEP = S <= 4;      // each step's decay, too, where registers allow
+      float ea[KEEP ? TT : 1][S];
       float h[TT + 1][S];      // h[k]: the state in front of step k
       if (ron) load_row<S>(a.ck + (((long)w.b * a.cktiles + t0 / TT) * a.D + rd) * NP + n0, h[0]);
       else
@@ -481,7 +486,9 @@ __global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(Scan
         float y = 0.f;
 #pragma unroll
         for (int s = 0; s < S; ++s) {
-          h[k + 1][s] = fmaf(__builtin_amdgcn_exp2f(c.d * A2[s]), h[k][s], c.x * c.b[s]);
+          const float e = __builtin_amdgcn_exp2f(c.d * A2[s]);
+          if constexpr (KEEP) ea[k][s] = e;
+          h[k + 1][s] = fmaf(e, h[k][s], c.x * c.b[s]);
           y = fmaf(h[k + 1][s], c.c[s], y);
         }
         asm volatile("" : "+v"(y));
@@ -501,7 +508,8 @@ __global__ void __launch_bounds__(256, STATE ? 4 : Tile<S>::WAVES) scan_bwd(Scan
           v[s] = g[s] * c.x;                       // dB
           v[S + s] = h[k + 1][s] * c.y;            // dC
           gB = fmaf(g[s], c.b[s], gB);
-          g[s] *= __builtin_amdgcn_exp2f(c.d * A2[s]);
+          if constexpr (KEEP) g[s] *= ea[k][s];
+          else g[s] *= __builtin_amdgcn_exp2f(c.d * A2[s]);
           const float q = g[s] * h[k][s];
           gA = fmaf(q, A2[s], gA);                 // of A log2 e: divided out of the sum
           dA[s] = fmaf(q, c.d, dA[s]);
@@ -774,18 +782,18 @@ struct StepLaunch {
 };
 
 // Chunks of the steps.  Cutting them costs a second walk (about 0.9 of the first forward, 0.2 backward), and pays where the channel
-// blocks alone leave compute units or their waves' places empty: four blocks a unit forward, three backward (two where the
-// states take more registers).  As many chunks as fill those places; forward not for fewer than three.  16-bit, 2048 channels of 16
-// states, forward / with gradients, us: 128 blocks (4 x 2048 steps) in 4, 6, 8, 12 chunks 183 / 636, 155 / 535, 143 / 554, 152 / 548;
-// 256 blocks whole 288 / 1362, in three 266 / 971, in four 247 / 1041; 384 whole 361 / 1694, in two 380 / 1420; 512 whole 183 / 891,
-// in two 230 / 1014.  Chunks of 128 steps at least, of 32 where three quarters of the units would be idle (32 blocks of 512 steps whole
-// 75 / 309, in four 44 / 135, in sixteen 28 / 82; 256 blocks of 128 steps whole 28 / 110, in four 33 / 114).
-void plan(int B, int T, int G, int Dg, int S, int backward, int* cblk, int* chunk, int* chunks) {
+// blocks alone leave compute units, or their waves' places, empty: as many chunks as bring four blocks a unit, not for fewer
+// than three.  bf16, 2048 channels of 16 states, us forward, and with gradients by the backward pass' chunks:
+//   128 blocks (4 x 2048 steps): forward in 4, 6, 8, 12 chunks 183, 155, 143, 152; backward in 4, 6, 8 509, 525, 479
+//   256 blocks (8 x 2048): forward whole 288, in three 266, in four 247; backward whole 1084, in two, three, four 906, 973, 883
+//   384 blocks (12 x 2048): forward whole 361, in two 380; backward whole 1409, in two 1427
+// Chunks of 128 steps at least, of 32 where three quarters of the units would be idle (32 blocks of 512 steps: whole 77 / 261, in four
+// 41 / 118, in sixteen 22 / 114; 256 blocks of 128 steps fp32: whole 25 / 111, in four 25 / 113).
+void plan(int B, int T, int G, int Dg, int* cblk, int* chunk, int* chunks) {
   *cblk = (Dg + CB - 1) / CB;
   const long blocks = (long)B * G * *cblk, cus = tb_num_cus();
-  const long places = cus * (!backward ? 4 : S == 4 ? 3 : 2);
-  long n = blocks > 0 ? places / blocks : 1;
-  if (n < (backward ? 2 : 3)) n = 1;
+  long n = blocks > 0 ? 4 * cus / blocks : 1;
+  if (n < 3) n = 1;
   const long least = blocks * 4 <= cus ? 32 : 128;
   long len = (T + n - 1) / n;
   if (len < least) len = least;
@@ -820,7 +828,7 @@ struct Sizes {
 };
 Sizes sizes(int B, int T, int D, int N, int G, int backward) {
   int cblk, chunk, chunks;
-  plan(B, T, G, D / G, states_per_lane(N), backward, &cblk, &chunk, &chunks);
+  plan(B, T, G, D / G, &cblk, &chunk, &chunks);
   const size_t NP = 4 * states_per_lane(N);
   Sizes z;
   z.cstate = chunks > 1 ? tb_align_up((size_t)B * chunks * D * NP * 4, 256) : 0;
@@ -864,7 +872,7 @@ int tb_scan_fwd(const void* u, const void* dt, const void* z, const void* Bm, co
   a.sub = q[0]; a.sut = q[1]; a.sdb = q[2]; a.sdt = q[3]; a.szb = q[4]; a.szt = q[5];
   a.sBb = q[6]; a.sBt = q[7]; a.sBg = q[8]; a.sCb = q[9]; a.sCt = q[10]; a.sCg = q[11];
   a.B = B; a.T = T; a.D = D; a.N = N; a.G = G; a.Dg = D / G;
-  plan(B, T, G, a.Dg, S, 0, &a.cblk, &a.chunk, &a.chunks);
+  plan(B, T, G, a.Dg, &a.cblk, &a.chunk, &a.chunks);
   a.softplus = softplus;
   a.ckt = states ? bwd_tile(S) : 0;
   a.cktiles = states ? (T + a.ckt - 1) / a.ckt : 0;
@@ -897,7 +905,7 @@ int tb_scan_bwd(const void* dout, const void* u, const void* dt, const void* z, 
   a.sBb = q[6]; a.sBt = q[7]; a.sBg = q[8]; a.sCb = q[9]; a.sCt = q[10]; a.sCg = q[11];
   a.sob = q[12]; a.sot = q[13];
   a.B = B; a.T = T; a.D = D; a.N = N; a.G = G; a.Dg = D / G;
-  plan(B, T, G, a.Dg, S, 1, &a.cblk, &a.chunk, &a.chunks);
+  plan(B, T, G, a.Dg, &a.cblk, &a.chunk, &a.chunks);
   a.softplus = softplus;
   a.ckt = bwd_tile(S);
   a.cktiles = (T + a.ckt - 1) / a.ckt;
