@@ -12,6 +12,8 @@
 // element written and read).
 #include "elem.h"
 
+#include <type_traits>
+
 namespace {
 
 constexpr int KMAX = 8;
@@ -27,12 +29,29 @@ struct ConvArgs {
   unsigned gx;               // blocks along the channels; blocks go along them first
 };
 
-template <typename T, int VEC>
+// AL: every row, and the taps, lie on the access' alignment.  Otherwise accesses of the same width off it, and the last thread of a
+// row moves back to the row's last VEC channels: some it shares with its neighbour, who finds and stores the same.
+template <bool AL, typename T, int N>
+__device__ __forceinline__ void load_n(const T* p, float (&r)[N]) {
+  if constexpr (AL) tb_load_n(p, r);
+  else tb_load_u(p, r);
+}
+template <bool AL, typename T, int N>
+__device__ __forceinline__ void store_n(T* p, const float (&r)[N]) {
+  if constexpr (AL) tb_store_n(p, r);
+  else tb_store_u(p, r);
+}
+template <bool AL, int VEC>
+__device__ __forceinline__ int first_channel(int group, int D) {
+  return AL ? group * VEC : min(group * VEC, max(D - VEC, 0));
+}
+
+template <typename T, int VEC, bool AL>
 __device__ __forceinline__ void load_x(const ConvArgs& a, int b, long t, int len, int K, int c, float (&r)[VEC]) {
   if (t >= 0 && t < len) {
-    tb_load_n(static_cast<const T*>(a.x) + b * a.sxb + t * a.sxt + c, r);
+    load_n<AL>(static_cast<const T*>(a.x) + b * a.sxb + t * a.sxt + c, r);
   } else if (t < 0 && a.state && t >= 1 - K) {
-    tb_load_n(static_cast<const T*>(a.state) + ((long)b * (K - 1) + (K - 1 + t)) * a.D + c, r);
+    load_n<AL>(static_cast<const T*>(a.state) + ((long)b * (K - 1) + (K - 1 + t)) * a.D + c, r);
   } else {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) r[i] = 0.f;
@@ -41,7 +60,7 @@ __device__ __forceinline__ void load_x(const ConvArgs& a, int b, long t, int len
 
 // the taps of VEC channels: K VEC neighbouring values, fetched whole where the channels are (the caller has seen to the
 // alignment of w and bias then)
-template <typename T, int K, int VEC>
+template <typename T, int K, int VEC, bool AL>
 __device__ __forceinline__ void load_par(const void* w, const void* bias, int f32, int c, float (&r)[K][VEC], float (&b)[VEC]) {
   float flat[K * VEC];
   if constexpr (VEC == 1) {
@@ -49,13 +68,13 @@ __device__ __forceinline__ void load_par(const void* w, const void* bias, int f3
     for (int k = 0; k < K; ++k) flat[k] = tb_load_par<T>(w, (long)c * K + k, f32);
     b[0] = bias ? tb_load_par<T>(bias, c, f32) : 0.f;
   } else {
-    if (f32) tb_load_n(static_cast<const float*>(w) + (long)c * K, flat);
-    else tb_load_n(static_cast<const T*>(w) + (long)c * K, flat);
+    if (f32) load_n<AL>(static_cast<const float*>(w) + (long)c * K, flat);
+    else load_n<AL>(static_cast<const T*>(w) + (long)c * K, flat);
     if (!bias) {
 #pragma unroll
       for (int i = 0; i < VEC; ++i) b[i] = 0.f;
-    } else if (f32) tb_load_n(static_cast<const float*>(bias) + c, b);
-    else tb_load_n(static_cast<const T*>(bias) + c, b);
+    } else if (f32) load_n<AL>(static_cast<const float*>(bias) + c, b);
+    else load_n<AL>(static_cast<const T*>(bias) + c, b);
   }
 #pragma unroll
   for (int i = 0; i < VEC; ++i)
@@ -66,34 +85,35 @@ __device__ __forceinline__ void load_par(const void* w, const void* bias, int f3
 constexpr int GRP = 4;      // steps fetched together; a run is a multiple of it
 
 // GRP rows from step t on, as they lie in memory; rows behind the sequence's steps read another row of it
-template <typename T, int VEC>
+template <typename T, int VEC, bool AL>
 struct Rows {
-  TbVec<T, VEC> v[GRP];
+  typedef std::conditional_t<AL, TbVec<T, VEC>, TbVecU<T, VEC>> Access;
+  Access v[GRP];
   __device__ __forceinline__ void fetch(const T* base, long st, int t, int T_) {
 #pragma unroll
-    for (int i = 0; i < GRP; ++i) v[i] = *reinterpret_cast<const TbVec<T, VEC>*>(base + (long)min(t + i, T_ - 1) * st);
+    for (int i = 0; i < GRP; ++i) v[i] = *reinterpret_cast<const Access*>(base + (long)min(t + i, T_ - 1) * st);
   }
   __device__ __forceinline__ float get(int i, int c, bool on) const { return on ? (float)v[i].v[c] : 0.f; }
 };
 
 // block: blockDim.x channel groups of VEC by blockDim.y runs
-template <typename T, int K, int VEC>
+template <typename T, int K, int VEC, bool AL>
 __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
-  const int c = (blockIdx.x % a.gx * blockDim.x + threadIdx.x) * VEC;
+  const int group = blockIdx.x % a.gx * blockDim.x + threadIdx.x, c = first_channel<AL, VEC>(group, a.D);
   const long row = blockIdx.x / a.gx, r = row * blockDim.y + threadIdx.y;
-  if (c >= a.D || r >= (long)a.B * a.runs) return;
+  if ((long)group * VEC >= a.D || r >= (long)a.B * a.runs) return;
   const int b = (int)(r / a.runs), q = (int)(r % a.runs);
   const int len = a.lengths ? min(max(a.lengths[b], 0), a.T) : a.T;
   const int t0 = q * a.run, t1 = min(t0 + a.run, a.T);
   const T* x = static_cast<const T*>(a.x) + b * a.sxb + c;
   T* y = static_cast<T*>(a.y) + (long)b * a.T * a.D + c;
   if (t0 < t1) {
-    Rows<T, VEC> next;
+    Rows<T, VEC, AL> next;
     next.fetch(x, a.sxt, t0, a.T);
     float w[K][VEC], bias[VEC], win[K - 1 + GRP][VEC];
-    load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
+    load_par<T, K, VEC, AL>(a.w, a.bias, a.wf32, c, w, bias);
 #pragma unroll
-    for (int k = 0; k < K - 1; ++k) load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
+    for (int k = 0; k < K - 1; ++k) load_x<T, VEC, AL>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
     for (int t = t0; t < t1; t += GRP) {
 #pragma unroll
       for (int j = 0; j < GRP; ++j)
@@ -112,7 +132,7 @@ __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
             if (a.act == TB_ACT_SILU) s = tb_silu(s);
             o[i] = t + j < len ? s : 0.f;
           }
-          tb_store_n(y + (long)(t + j) * a.D, o);
+          store_n<AL>(y + (long)(t + j) * a.D, o);
         }
       }
 #pragma unroll
@@ -125,18 +145,18 @@ __global__ void __launch_bounds__(256) conv_fwd(ConvArgs a) {
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
       float s[VEC];
-      load_x<T, VEC>(a, b, (long)len - (K - 1) + k, len, K, c, s);
-      tb_store_n(static_cast<T*>(a.state_out) + ((long)b * (K - 1) + k) * a.D + c, s);
+      load_x<T, VEC, AL>(a, b, (long)len - (K - 1) + k, len, K, c, s);
+      store_n<AL>(static_cast<T*>(a.state_out) + ((long)b * (K - 1) + k) * a.D + c, s);
     }
   }
 }
 
-template <typename T, int K, int VEC>
+template <typename T, int K, int VEC, bool AL>
 __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
   __shared__ float red[256][VEC];
-  const int c = (blockIdx.x % a.gx * blockDim.x + threadIdx.x) * VEC;
+  const int group = blockIdx.x % a.gx * blockDim.x + threadIdx.x, c = first_channel<AL, VEC>(group, a.D);
   const long row = blockIdx.x / a.gx, r = row * blockDim.y + threadIdx.y;
-  const bool on = c < a.D && r < (long)a.B * a.runs;
+  const bool mine = (long)group * VEC < a.D, on = mine && r < (long)a.B * a.runs;
   float dw[K + 1][VEC];
 #pragma unroll
   for (int k = 0; k <= K; ++k)
@@ -149,15 +169,15 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
     const T* x = static_cast<const T*>(a.x) + b * a.sxb + c;
     const T* dy = static_cast<const T*>(a.dy) + (long)b * a.T * a.D + c;
     T* dx = static_cast<T*>(a.dx) + (long)b * a.T * a.D + c;
-    Rows<T, VEC> nx, ny;
+    Rows<T, VEC, AL> nx, ny;
     nx.fetch(x, a.sxt, t0, a.T);
     ny.fetch(dy, a.D, t0, a.T);
     // win[K-1+j]: x of step s + j; dp likewise of dpre
     float w[K][VEC], bias[VEC], win[K - 1 + GRP][VEC], dp[K - 1 + GRP][VEC];
-    load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
+    load_par<T, K, VEC, AL>(a.w, a.bias, a.wf32, c, w, bias);
 #pragma unroll
     for (int k = 0; k < K - 1; ++k) {
-      load_x<T, VEC>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
+      load_x<T, VEC, AL>(a, b, (long)t0 - (K - 1) + k, len, K, c, win[k]);
 #pragma unroll
       for (int i = 0; i < VEC; ++i) dp[k][i] = 0.f;
     }
@@ -177,7 +197,7 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < GRP; ++j) {
-        const bool mine = s + j < t1;         // the run's own steps: their share of dw and db
+        const bool own = s + j < t1;          // the run's own steps: their share of dw and db
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           float d = g[j][i];
@@ -190,7 +210,7 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
             d = s + j < len ? d : 0.f;
           }
           dp[K - 1 + j][i] = d;
-          const float m = mine ? d : 0.f;
+          const float m = own ? d : 0.f;
 #pragma unroll
           for (int k = 0; k < K; ++k) dw[k][i] = fmaf(m, win[j + k][i], dw[k][i]);
           dw[K][i] += m;
@@ -205,7 +225,7 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
             for (int k = 0; k < K; ++k) v = fmaf(w[K - 1 - k][i], dp[j + k][i], v);
             o[i] = t < len ? v : 0.f;
           }
-          tb_store_n(dx + (long)t * a.D, o);
+          store_n<AL>(dx + (long)t * a.D, o);
         }
       }
 #pragma unroll
@@ -224,14 +244,14 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
 #pragma unroll
     for (int i = 0; i < VEC; ++i) red[me][i] = dw[k][i];
     __syncthreads();
-    if (threadIdx.y == 0 && c < a.D) {
+    if (threadIdx.y == 0 && mine) {
       float o[VEC];
 #pragma unroll
       for (int i = 0; i < VEC; ++i) o[i] = 0.f;
       for (int j = 0; j < (int)blockDim.y; ++j)
 #pragma unroll
         for (int i = 0; i < VEC; ++i) o[i] += red[j * blockDim.x + threadIdx.x][i];
-      tb_store_n(a.slab + (row * (K + 1) + k) * a.D + c, o);
+      store_n<AL>(a.slab + (row * (K + 1) + k) * a.D + c, o);
     }
     __syncthreads();
   }
@@ -281,7 +301,7 @@ __global__ void __launch_bounds__(256) conv_step(ConvStepArgs a) {
   const int b = (int)(id / groups), c = (int)(id % groups) * VEC;
   T* st = static_cast<T*>(a.state) + b * a.ssb + c;
   float win[K][VEC], w[K][VEC], bias[VEC], o[VEC];
-  load_par<T, K, VEC>(a.w, a.bias, a.wf32, c, w, bias);
+  load_par<T, K, VEC, true>(a.w, a.bias, a.wf32, c, w, bias);
 #pragma unroll
   for (int k = 0; k < K - 1; ++k) tb_load_n(st + (long)k * a.D, win[k]);
   tb_load_n(static_cast<const T*>(a.x) + b * a.sxb + c, win[K - 1]);
@@ -297,27 +317,33 @@ __global__ void __launch_bounds__(256) conv_step(ConvStepArgs a) {
   tb_store_n(static_cast<T*>(a.y) + (long)b * a.D + c, o);
 }
 
-// one instantiation per (type, taps, vector width): F is called with the kernel's template arguments
+// one instantiation per (type, taps, access): a thread's channels on their alignment, off it, or one by one (fewer channels than
+// an access, and the in-place step off the alignment)
+enum Access { ALIGNED, OFF, SINGLE };
+
 template <int V16, typename F>
-int by_shape(int dtype, int K, bool vec, F&& f) {
-#define TB_K(T, V)                                                          \
+int by_shape(int dtype, int K, Access how, F&& f) {
+#define TB_K(T, V, AL)                                                      \
   switch (K) {                                                              \
-    case 1: return f.template operator()<T, 1, V>();                        \
-    case 2: return f.template operator()<T, 2, V>();                        \
-    case 3: return f.template operator()<T, 3, V>();                        \
-    case 4: return f.template operator()<T, 4, V>();                        \
-    case 5: return f.template operator()<T, 5, V>();                        \
-    case 6: return f.template operator()<T, 6, V>();                        \
-    case 7: return f.template operator()<T, 7, V>();                        \
-    default: return f.template operator()<T, 8, V>();                       \
+    case 1: return f.template operator()<T, 1, V, AL>();                    \
+    case 2: return f.template operator()<T, 2, V, AL>();                    \
+    case 3: return f.template operator()<T, 3, V, AL>();                    \
+    case 4: return f.template operator()<T, 4, V, AL>();                    \
+    case 5: return f.template operator()<T, 5, V, AL>();                    \
+    case 6: return f.template operator()<T, 6, V, AL>();                    \
+    case 7: return f.template operator()<T, 7, V, AL>();                    \
+    default: return f.template operator()<T, 8, V, AL>();                   \
   }
-  if (dtype == TB_F32) {
-    if (vec) TB_K(float, 4) else TB_K(float, 1)
-  } else if (dtype == TB_BF16) {
-    if (vec) TB_K(__bf16, V16) else TB_K(__bf16, 1)
-  } else {
-    if (vec) TB_K(_Float16, V16) else TB_K(_Float16, 1)
+#define TB_A(T, V)                          \
+  {                                         \
+    if (how == ALIGNED) TB_K(T, V, true)    \
+    if (how == OFF) TB_K(T, V, false)       \
+    TB_K(T, 1, true)                        \
   }
+  if (dtype == TB_F32) TB_A(float, 4)
+  if (dtype == TB_BF16) TB_A(__bf16, V16)
+  TB_A(_Float16, V16)
+#undef TB_A
 #undef TB_K
 }
 
@@ -325,9 +351,9 @@ struct FwdLaunch {
   ConvArgs a;
   dim3 grid, block;
   hipStream_t s;
-  template <typename T, int K, int V>
+  template <typename T, int K, int V, bool AL>
   int operator()() {
-    conv_fwd<T, K, V><<<grid, block, 0, s>>>(a);
+    conv_fwd<T, K, V, AL><<<grid, block, 0, s>>>(a);
     return 0;
   }
 };
@@ -335,19 +361,19 @@ struct BwdLaunch {
   ConvArgs a;
   dim3 grid, block;
   hipStream_t s;
-  template <typename T, int K, int V>
+  template <typename T, int K, int V, bool AL>
   int operator()() {
-    conv_bwd<T, K, V><<<grid, block, 0, s>>>(a);
+    conv_bwd<T, K, V, AL><<<grid, block, 0, s>>>(a);
     return 0;
   }
 };
 struct StepLaunch {
   ConvStepArgs a;
   hipStream_t s;
-  template <typename T, int K, int V>
+  template <typename T, int K, int V, bool AL>
   int operator()() {
     const long n = (long)a.B * (a.D / V);
-    conv_step<T, K, V><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
+    if constexpr (AL) conv_step<T, K, V><<<(unsigned)((n + 255) / 256), 256, 0, s>>>(a);
     return 0;
   }
 };
@@ -410,13 +436,14 @@ int tb_conv_fwd(const void* x, long x_batch_stride, long x_step_stride, const vo
   if (B == 0 || (T == 0 && !state_out)) return TB_OK;
   if (!w || (T > 0 && (!x || !y))) return tb_set_error(TB_ERR_ARG, "conv_fwd: null pointer");
   const void* ptrs[] = {x, y, state, state_out, w, bias};
-  const bool vec = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 6);
-  const Plan p = plan(B, T > 0 ? T : 1, D, vec ? (dtype == TB_F32 ? 4 : 8) : 1);
+  const int v = dtype == TB_F32 ? 4 : 8;
+  const Access how = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 6) ? ALIGNED : D >= v ? OFF : SINGLE;
+  const Plan p = plan(B, T > 0 ? T : 1, D, how == SINGLE ? 1 : v);
   rc = check_grid("conv_fwd", p);
   if (rc) return rc;
   ConvArgs a{x, w, bias, state, nullptr, lengths, y, state_out, nullptr, nullptr, x_batch_stride, x_step_stride, B, T, D, p.run,
              p.runs, act, w_f32, (unsigned)p.gx};
-  by_shape<8>(dtype, K, vec, FwdLaunch{a, dim3((unsigned)(p.gx * p.gy)), dim3(p.bx, p.by), static_cast<hipStream_t>(stream)});
+  by_shape<8>(dtype, K, how, FwdLaunch{a, dim3((unsigned)(p.gx * p.gy)), dim3(p.bx, p.by), static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("conv_fwd");
   return TB_OK;
 }
@@ -438,14 +465,14 @@ int tb_conv_bwd(const void* dy, const void* x, long x_batch_stride, long x_step_
   if (!dy || !x || !w || !dx || !ws) return tb_set_error(TB_ERR_ARG, "conv_bwd: null pointer");
   if (ws_bytes < tb_conv_bwd_workspace_bytes(B, T, D, K, dtype)) return tb_set_error(TB_ERR_WORKSPACE, "conv_bwd: workspace too small");
   const void* ptrs[] = {x, dy, dx, state, w, bias};
-  const bool vec = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 6);
-  const Plan p = plan(B, T, D, vec ? 4 : 1);
+  const Access how = can_vec(dtype, D, x_batch_stride, x_step_stride, ptrs, 6) ? ALIGNED : D >= 4 ? OFF : SINGLE;
+  const Plan p = plan(B, T, D, how == SINGLE ? 1 : 4);
   rc = check_grid("conv_bwd", p);
   if (rc) return rc;
   hipStream_t s = static_cast<hipStream_t>(stream);
   ConvArgs a{x, w, bias, state, dy, lengths, nullptr, nullptr, dx, static_cast<float*>(ws), x_batch_stride, x_step_stride, B, T, D,
              p.run, p.runs, act, w_f32, (unsigned)p.gx};
-  by_shape<4>(dtype, K, vec, BwdLaunch{a, dim3((unsigned)(p.gx * p.gy)), dim3(p.bx, p.by), s});
+  by_shape<4>(dtype, K, how, BwdLaunch{a, dim3((unsigned)(p.gx * p.gy)), dim3(p.bx, p.by), s});
   TB_LAUNCH_CHECK("conv_bwd");
   if (dw || db) {
     const long cols = (long)(K + 1) * D;
@@ -468,7 +495,7 @@ int tb_conv_step(const void* x, long x_batch_stride, void* state, long state_bat
   const void* ptrs[] = {x, y, state, w, bias};
   const bool vec = can_vec(dtype, D, x_batch_stride, state_batch_stride, ptrs, 5);
   ConvStepArgs a{x, w, bias, state, y, x_batch_stride, state_batch_stride, B, D, act, w_f32};
-  by_shape<8>(dtype, K, vec, StepLaunch{a, static_cast<hipStream_t>(stream)});
+  by_shape<8>(dtype, K, vec ? ALIGNED : SINGLE, StepLaunch{a, static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("conv_step");
   return TB_OK;
 }

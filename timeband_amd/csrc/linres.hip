@@ -491,10 +491,12 @@ __device__ __forceinline__ u32x4 load_piece(const T* row, long k, int K, bool ve
   u32x4 r = (u32x4){0u, 0u, 0u, 0u};
   if (vec) {
     if (on && k < K) r = *reinterpret_cast<const u32x4*>(row + k);
-  } else {
+  } else if (on && k + CE <= K) {
+    r = __builtin_bit_cast(u32x4, *reinterpret_cast<const TbVecU<T, CE>*>(row + k));
+  } else if (on && k < K) {
     TbVec<T, CE> v;
 #pragma unroll
-    for (int i = 0; i < CE; ++i) v.v[i] = on && k + i < K ? row[k + i] : (T)0.f;
+    for (int i = 0; i < CE; ++i) v.v[i] = k + i < K ? row[k + i] : (T)0.f;
     r = __builtin_bit_cast(u32x4, v);
   }
   return r;

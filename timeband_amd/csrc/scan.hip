@@ -609,49 +609,56 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
   }
 }
 
-// dA (D, N), dD (D), dbias (D) from the rows of (sequence, chunk), in their order by four threads a value
-__global__ void __launch_bounds__(256) scan_finish_par(const float* par, int rows, int D, int N, int NP, float* dA, float* dD, float* dbias) {
-  __shared__ float red[4][64];
-  const long cols = (long)D * (NP + 2), col = (long)blockIdx.x * 64 + (threadIdx.x & 63);
-  const int q = threadIdx.x >> 6, per = (rows + 3) / 4;
-  float s = 0.f;
-  if (col < cols) {
-    const int r1 = min(rows, (q + 1) * per);
-#pragma unroll 4
-    for (int r = q * per; r < r1; ++r) s += par[r * cols + col];
-  }
-  red[q][threadIdx.x & 63] = s;
-  __syncthreads();
-  if (q == 0 && col < cols) {
-    const int l = threadIdx.x;
-    s = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
-    const long d = col / (NP + 2);
-    const int n = (int)(col % (NP + 2));
-    if (n < N) {
-      if (dA) dA[d * N + n] = s;
-    } else if (n == NP) {
-      if (dD) dD[d] = s;
-    } else if (n == NP + 1) {
-      if (dbias) dbias[d] = s;
-    }
-  }
-}
+struct FinishArgs {
+  const float *par, *bc;
+  float *dA, *dD, *dbias;
+  void *dB, *dC;
+  int rows, B, T, D, N, G, NP, cblk;
+  unsigned first;          // blocks of the parameters' sums; behind them those of dB and dC
+};
 
-// dB, dC (B, T, G, N) from the channel blocks' sums
+// dA (D, N), dD (D), dbias (D) from the rows of (sequence, chunk), in their order by four threads a value; dB, dC (B, T, G, N) from
+// the channel blocks' sums
 template <typename T>
-__global__ void __launch_bounds__(256) scan_finish_bc(const float* bc, int B, int Tn, int G, int N, int NP, int cblk, void* dB, void* dC) {
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
-  const long per = (long)Tn * 2 * NP;
-  if (id >= (long)B * G * per) return;
+__global__ void __launch_bounds__(256) scan_finish(FinishArgs a) {
+  __shared__ float red[4][64];
+  if (blockIdx.x < a.first) {
+    const long cols = (long)a.D * (a.NP + 2), col = (long)blockIdx.x * 64 + (threadIdx.x & 63);
+    const int q = threadIdx.x >> 6, per = (a.rows + 3) / 4;
+    float s = 0.f;
+    if (col < cols) {
+      const int r1 = min(a.rows, (q + 1) * per);
+#pragma unroll 4
+      for (int r = q * per; r < r1; ++r) s += a.par[r * cols + col];
+    }
+    red[q][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (q == 0 && col < cols) {
+      const int l = threadIdx.x;
+      s = (red[0][l] + red[1][l]) + (red[2][l] + red[3][l]);
+      const long d = col / (a.NP + 2);
+      const int n = (int)(col % (a.NP + 2));
+      if (n < a.N) {
+        if (a.dA) a.dA[d * a.N + n] = s;
+      } else if (n == a.NP) {
+        if (a.dD) a.dD[d] = s;
+      } else if (n == a.NP + 1) {
+        if (a.dbias) a.dbias[d] = s;
+      }
+    }
+    return;
+  }
+  const long id = (long)(blockIdx.x - a.first) * 256 + threadIdx.x, per = (long)a.T * 2 * a.NP;
+  if (id >= (long)a.B * a.G * per) return;
   const long bg = id / per, r = id % per;
-  const int n = (int)(r % (2 * NP)), t = (int)(r / (2 * NP));
-  const int half = n >= NP, k = n - half * NP;
-  if (k >= N) return;
+  const int n = (int)(r % (2 * a.NP)), t = (int)(r / (2 * a.NP));
+  const int half = n >= a.NP, k = n - half * a.NP;
+  if (k >= a.N) return;
   float s = 0.f;
 #pragma unroll 4
-  for (int c = 0; c < cblk; ++c) s += bc[(bg * cblk + c) * per + r];
-  void* o = half ? dC : dB;
-  if (o) static_cast<T*>(o)[(((bg / G) * Tn + t) * G + bg % G) * N + k] = (T)s;
+  for (int c = 0; c < a.cblk; ++c) s += a.bc[(bg * a.cblk + c) * per + r];
+  void* o = half ? a.dC : a.dB;
+  if (o) static_cast<T*>(o)[(((bg / a.G) * a.T + t) * a.G + bg % a.G) * a.N + k] = (T)s;
 }
 
 struct StepArgs {
@@ -764,10 +771,10 @@ struct BwdLaunch {
   int run() {
     if (a.chunks > 1) scan_bwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
     scan_bwd<T, S, false, VEC><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
-    if (dA || dD || dbias)
-      scan_finish_par<<<(unsigned)(((long)a.D * (4 * S + 2) + 63) / 64), 256, 0, s>>>(a.par, a.B * a.chunks, a.D, a.N, 4 * S, dA, dD, dbias);
-    if (dB || dC)
-      scan_finish_bc<T><<<(unsigned)(((long)a.B * a.G * a.T * 8 * S + 255) / 256), 256, 0, s>>>(a.bc, a.B, a.T, a.G, a.N, 4 * S, a.cblk, dB, dC);
+    FinishArgs f{a.par, a.bc, dA, dD, dbias, dB, dC, a.B * a.chunks, a.B, a.T, a.D, a.N, a.G, 4 * S, a.cblk, 0};
+    f.first = dA || dD || dbias ? (unsigned)(((long)a.D * (4 * S + 2) + 63) / 64) : 0;
+    const unsigned rest = dB || dC ? (unsigned)(((long)a.B * a.G * a.T * 8 * S + 255) / 256) : 0;
+    if (f.first + rest) scan_finish<T><<<f.first + rest, 256, 0, s>>>(f);
     return 0;
   }
 };
