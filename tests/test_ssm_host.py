@@ -119,3 +119,25 @@ def test_library_refuses_bad_calls_before_launching():
     assert lin(wsb=0) == 4 and lin(W=0) == 1 and lin(M=0) == 0
     assert lib.tb_linres_bwd(p, 8, p, 8, p, 8, 0, 4, p, p, p, 100, 8, 8, 0, p, 1 << 30, 0) == 1        # no pre-activation kept
     assert lib.tb_linres_bwd(p, 8, p, 8, p, 8, 0, 0, p, p, p, 100, 8, 8, 0, p, 16, 0) == 4
+
+
+def test_library_refuses_sizes_past_its_indexes():
+    """Steps whose sums with a run pass 32 bits, and launches of 2^32 threads: refused (3) before anything is launched."""
+    from timeband_amd import _lib
+    lib = _lib.load()
+    p, ls, wide = 4096, (ctypes.c_long * 14)(), 1 << 62
+    top = 2 ** 31 - 1
+    assert lib.tb_conv_fwd(p, top, 1, p, 0, 0, 0, 0, p, 0, 1, top, 1, 4, 0, 1, 0) == 3
+    assert lib.tb_conv_bwd(p, p, top, 1, p, 0, 0, 0, 0, p, p, p, 1, top, 1, 4, 0, 1, p, wide, 0) == 3
+    assert lib.tb_conv_step(p, 4097, p, 4097 * 3, p, 0, 0, p, 1 << 20, 4097, 4, 0, 1, 0) == 3        # element by element
+    assert lib.tb_conv_step(p, 1 << 15, p, 3 << 15, p, 0, 0, p, 1 << 20, 1 << 15, 4, 0, 1, 0) == 3    # eight a thread
+    fwd = lambda B, T, D, N: lib.tb_scan_fwd(p, p, 0, p, p, ls, p, 0, 0, 1, 0, 0, p, 0, 0, B, T, D, N, 1, 1, p, wide, 0)
+    bwd = lambda B, T, D, N: lib.tb_scan_bwd(p, p, p, 0, p, p, ls, p, 0, 0, 1, 0, p, 0, p, p, 0, p, p, p, 0, 0, 0, B, T, D, N, 1, 1, p, wide, 0)
+    assert fwd(1, top, 1, 16) == 3 and bwd(1, top, 1, 16) == 3
+    assert fwd(1 << 20, 1, 1024, 16) == 3 and bwd(1 << 20, 1, 1024, 16) == 3
+    assert bwd(1 << 10, 1 << 17, 1, 16) == 3                     # the sums of dB and dC
+    assert lib.tb_scan_step(p, 1 << 14, p, p, 0, p, p, ls, p, 0, 0, 1, p, 1 << 20, 1024, 16, 1, 1, 0) == 3
+    lin = lambda M, K, N: lib.tb_linres_fwd(p, K, p, K, 0, 0, 0, p, 0, M, K, N, 0, 0, p, wide, 0)
+    back = lambda M, K, N: lib.tb_linres_bwd(p, N, p, K, p, K, 0, 0, p, p, p, M, K, N, 0, p, wide, 0)
+    assert lin(2 ** 30 + 64, 4, 4) == 3 and back(2 ** 30 + 64, 4, 4) == 3
+    assert lin(1 << 28, 65, 4) == 3 and lin(100, 4000001, 4) == 3 and lin(100, 4, 4000001) == 3

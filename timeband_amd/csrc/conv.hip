@@ -404,6 +404,7 @@ Plan plan(int B, int T, int D, int vec) {
 
 int check_common(const char* what, int B, long T, int D, int K, int act, int dtype) {
   if (B < 0 || T < 0 || D < 1) return tb_set_error(TB_ERR_ARG, "%s: bad sizes B=%d T=%ld D=%d", what, B, T, D);
+  if (T > TB_STEPS_MAX) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: too many steps in one call", what);
   if (K < 1 || K > KMAX) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: %d taps are not supported (1 to %d)", what, K, KMAX);
   if (act != 0 && act != TB_ACT_SILU) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: activation %d is not supported (none, silu)", what, act);
   if (!tb_dtype_ok(dtype)) return tb_set_error(TB_ERR_ARG, "%s: bad element type %d", what, dtype);
@@ -418,9 +419,8 @@ bool can_vec(int dtype, int D, long sb, long st, const void* const* p, int n) {
   return true;
 }
 
-// a launch has at most 2^32 threads
 int check_grid(const char* what, const Plan& p) {
-  if (p.gx * p.gy >= 1L << 24) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: too many steps in one call", what);
+  if (!tb_grid_ok(p.gx * p.gy, 256)) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: too many steps in one call", what);
   return TB_OK;
 }
 
@@ -494,6 +494,8 @@ int tb_conv_step(const void* x, long x_batch_stride, void* state, long state_bat
   if (!x || !w || !y || (K > 1 && !state)) return tb_set_error(TB_ERR_ARG, "conv_step: null pointer");
   const void* ptrs[] = {x, y, state, w, bias};
   const bool vec = can_vec(dtype, D, x_batch_stride, state_batch_stride, ptrs, 5);
+  if (!tb_grid_ok(((long)B * (vec ? D / (dtype == TB_F32 ? 4 : 8) : D) + 255) / 256, 256))
+    return tb_set_error(TB_ERR_UNSUPPORTED, "conv_step: too many rows in one call");
   ConvStepArgs a{x, w, bias, state, y, x_batch_stride, state_batch_stride, B, D, act, w_f32};
   by_shape<8>(dtype, K, vec ? ALIGNED : SINGLE, StepLaunch{a, static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("conv_step");

@@ -10,6 +10,10 @@
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 static inline size_t tb_dtype_size(int dt) { return dt == TB_F32 ? 4 : 2; }
+// steps a call: sums of a step and a run or chunk of them stay within 32 bits
+#define TB_STEPS_MAX 2147418112L
+// a launch has fewer than 2^32 threads
+static inline bool tb_grid_ok(long blocks, int threads) { return blocks * threads < 1L << 32; }
 static inline bool tb_dtype_ok(int dt) { return dt >= TB_F32 && dt <= TB_F16; }
 
 // N consecutive elements as one access where the address allows it (the caller knows), element by element otherwise

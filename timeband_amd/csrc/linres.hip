@@ -766,6 +766,8 @@ int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, in
   const long Kp = up(K, sizeof(T));
   const bool dxr = direct<T>(x, ldx, K), dwr = direct<T>(W, ldw, K);
   char* p = ws;
+  if ((!dxr && !tb_grid_ok((M * (Kp / CE) + 255) / 256, 256)) || (!dwr && !tb_grid_ok(((long)N * (Kp / CE) + 255) / 256, 256)))
+    return tb_set_error(TB_ERR_UNSUPPORTED, "linres_fwd: M=%ld K=%d N=%d, off the alignment of 16 bytes, are too many in one call", M, K, N);
   if (!dxr) {
     pack_rows<T><<<(unsigned)((M * (Kp / CE) + 255) / 256), 256, 0, s>>>(x, ldx, M, K, reinterpret_cast<T*>(p), (int)Kp);
     TB_LAUNCH_CHECK("linres pack");
@@ -856,8 +858,10 @@ int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, 
 }
 
 int check_common(const char* what, long M, int K, int N, int act, int dtype) {
-  // the tile counts and the transposes' grids are 32 and 16 bits wide
-  if (M < 0 || K < 1 || N < 1 || K > 4000000 || N > 4000000 || M > 2000000000L) return tb_set_error(TB_ERR_ARG, "%s: bad sizes M=%ld K=%d N=%d", what, M, K, N);
+  if (M < 0 || K < 1 || N < 1) return tb_set_error(TB_ERR_ARG, "%s: bad sizes M=%ld K=%d N=%d", what, M, K, N);
+  // The transposes' grids are 16 bits wide across; a block of them takes 64 rows, and DOWN puts columns that are not there 2^30 rows away.
+  if (K > 4000000 || N > 4000000 || M > 1000000000L)
+    return tb_set_error(TB_ERR_UNSUPPORTED, "%s: M=%ld K=%d N=%d are too many in one call", what, M, K, N);
   if (act < 0 || act > TB_ACT_LAST) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: activation %d is not supported", what, act);
   if (!tb_dtype_ok(dtype)) return tb_set_error(TB_ERR_ARG, "%s: bad element type %d", what, dtype);
   return TB_OK;

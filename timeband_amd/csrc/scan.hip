@@ -742,6 +742,10 @@ int by_shape(int dtype, int S, F&& f) {
 #undef TB_S
 }
 
+// blocks of scan_finish: the parameters' sums, and those of dB and dC
+long finish_blocks_par(const ScanArgs& a, int S) { return ((long)a.D * (4 * S + 2) + 63) / 64; }
+long finish_blocks_bc(const ScanArgs& a, int S) { return ((long)a.B * a.G * a.T * 8 * S + 255) / 256; }
+
 struct FwdLaunch {
   ScanArgs a;
   long blocks;       // channel blocks of the batch
@@ -772,8 +776,8 @@ struct BwdLaunch {
     if (a.chunks > 1) scan_bwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
     scan_bwd<T, S, false, VEC><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
     FinishArgs f{a.par, a.bc, dA, dD, dbias, dB, dC, a.B * a.chunks, a.B, a.T, a.D, a.N, a.G, 4 * S, a.cblk, 0};
-    f.first = dA || dD || dbias ? (unsigned)(((long)a.D * (4 * S + 2) + 63) / 64) : 0;
-    const unsigned rest = dB || dC ? (unsigned)(((long)a.B * a.G * a.T * 8 * S + 255) / 256) : 0;
+    f.first = dA || dD || dbias ? (unsigned)finish_blocks_par(a, S) : 0;
+    const unsigned rest = dB || dC ? (unsigned)finish_blocks_bc(a, S) : 0;
     if (f.first + rest) scan_finish<T><<<f.first + rest, 256, 0, s>>>(f);
     return 0;
   }
@@ -811,6 +815,7 @@ void plan(int B, int T, int G, int Dg, int* cblk, int* chunk, int* chunks) {
 
 int check_common(const char* what, int B, long T, int D, int N, int G, int dtype) {
   if (B < 0 || T < 0 || D < 1 || N < 1 || G < 1 || D % G) return tb_set_error(TB_ERR_ARG, "%s: bad sizes B=%d T=%ld D=%d N=%d G=%d", what, B, T, D, N, G);
+  if (T > TB_STEPS_MAX) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: too many steps in one call", what);
   if (N > NMAX) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: %d states a channel are not supported (1 to %d)", what, N, NMAX);
   if (!tb_dtype_ok(dtype)) return tb_set_error(TB_ERR_ARG, "%s: bad element type %d", what, dtype);
   return TB_OK;
@@ -885,6 +890,7 @@ int tb_scan_fwd(const void* u, const void* dt, const void* z, const void* Bm, co
   a.cktiles = states ? (T + a.ckt - 1) / a.ckt : 0;
   a.cstate = static_cast<float*>(ws);
   a.csum = reinterpret_cast<float*>(static_cast<char*>(ws) + sz.cstate);
+  if (!tb_grid_ok((long)B * G * a.cblk * a.chunks, 256)) return tb_set_error(TB_ERR_UNSUPPORTED, "scan_fwd: too many rows in one call");
   a.vec = can_vec(a, dtype);
   by_shape(dtype, S, FwdLaunch{a, (long)B * G * a.cblk, static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("scan_fwd");
@@ -921,6 +927,8 @@ int tb_scan_bwd(const void* dout, const void* u, const void* dt, const void* z, 
   a.csum = reinterpret_cast<float*>(p + sz.cstate);
   a.bc = reinterpret_cast<float*>(p + sz.cstate + sz.csum);
   a.par = reinterpret_cast<float*>(p + sz.cstate + sz.csum + sz.bc);
+  if (!tb_grid_ok((long)B * G * a.cblk * a.chunks, 256) || !tb_grid_ok(finish_blocks_par(a, S) + finish_blocks_bc(a, S), 256))
+    return tb_set_error(TB_ERR_UNSUPPORTED, "scan_bwd: too many rows or steps in one call");
   a.vec = can_vec(a, dtype);
   by_shape(dtype, S, BwdLaunch{a, (long)B * G * a.cblk, dA, dD, dbias, dB, dC, static_cast<hipStream_t>(stream)});
   TB_LAUNCH_CHECK("scan_bwd");
@@ -937,6 +945,7 @@ int tb_scan_step(float* state, long state_batch_stride, const void* u, const voi
   const long* q = strides;
   StepArgs a{state, u, dt, z, Bm, Cm, A, Dp, dt_bias, out, q[0], q[1], q[2], q[3], q[4], q[5], q[6], state_batch_stride,
              B, D, N, G, D / G, softplus, 0, 0};
+  if (!tb_grid_ok(((long)B * D + 63) / 64, 256)) return tb_set_error(TB_ERR_UNSUPPORTED, "scan_step: too many rows in one call");
   const int S = states_per_lane(N), v = dtype == TB_F32 ? 4 : 8;
   a.vec = N == 4 * S && state_batch_stride % 4 == 0 && aligned(state) && aligned(A);
   a.vecbc = N == 4 * S && N % v == 0 && aligned(Bm) && aligned(Cm) && q[3] % v == 0 && q[4] % v == 0 && q[5] % v == 0 && q[6] % v == 0;
