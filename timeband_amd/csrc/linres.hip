@@ -549,19 +549,26 @@ __global__ void __launch_bounds__(WAVES * 64) gemm_few(FewArgs a) {
   }
 }
 
-// rows copied with their k padded by zeros to whole 16-byte pieces (rows that do not start on 16 bytes)
+// rows copied with their k padded by zeros to whole 16-byte pieces (rows that do not start on 16 bytes): one operand, or both in a launch
 template <typename T>
-__global__ void __launch_bounds__(256) pack_rows(const T* src, long ld, long R, int C, T* dst, int Cp) {
+struct Rows {
+  const T* src;
+  long ld, R;
+  T* dst;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) pack_rows(Rows<T> x, Rows<T> w, unsigned first, int C, int Cp) {
   constexpr int CE = 16 / sizeof(T);
   const int per = Cp / CE;
-  const long id = (long)blockIdx.x * 256 + threadIdx.x;
+  const bool is_x = blockIdx.x < first;
+  const T* src = is_x ? x.src : w.src;
+  T* dst = is_x ? x.dst : w.dst;
+  const long ld = is_x ? x.ld : w.ld, R = is_x ? x.R : w.R;
+  const long id = (long)(blockIdx.x - (is_x ? 0 : first)) * 256 + threadIdx.x;
   if (id >= R * per) return;
   const long r = id / per;
   const int c = (int)(id % per) * CE;
-  TbVec<T, CE> v;
-#pragma unroll
-  for (int i = 0; i < CE; ++i) v.v[i] = c + i < C ? src[r * ld + c + i] : (T)0.f;
-  *reinterpret_cast<TbVec<T, CE>*>(dst + r * Cp + c) = v;
+  *reinterpret_cast<u32x4*>(dst + r * Cp + c) = load_piece(src + r * ld, c, C, false, true);
 }
 
 // eight neighbouring elements of row r from column c on: zeros behind C and R
@@ -696,7 +703,9 @@ struct Plan {
   int tm, tn, splits, per;
 };
 // 256 x 256 tiles where they fill the chip, 128 x 128 otherwise (two blocks a unit).  k is split where even those leave units
-// idle, into parts of sixteen k tiles (1 KB of a row) at least.
+// idle, into parts of sixteen k tiles (1 KB of a row) at least, of fp32, whose products take longer a byte, of four: 1000 x 1000 x 1000
+// fp32 in parts of 16, 8, 4, 2 tiles 33.5, 29.9, 29.6, 29.7 us, 241 x 2048 x 272 24.5, 18.2, 16.4, 16.4; 1024 x 1024 x 1024 bf16
+// 16.7, 20.4, 20.4, 20.5.
 Plan plan(long M, int N, long K, int esize, bool down = false) {
   Plan p;
   const long cus = tb_num_cus(), kt = (K * esize + 63) / 64;
@@ -709,7 +718,8 @@ Plan plan(long M, int N, long K, int esize, bool down = false) {
   long s = 1;
   if (!p.big && tiles <= cus / 2) {
     s = cus / tiles;
-    if (s > kt / 16) s = kt / 16;
+    const int least = esize == 4 ? 4 : 16;
+    if (s > kt / least) s = kt / least;
     if (s > 64) s = 64;
     if (s < 1) s = 1;
   }
@@ -765,24 +775,26 @@ int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, in
   }
   const long Kp = up(K, sizeof(T));
   const bool dxr = direct<T>(x, ldx, K), dwr = direct<T>(W, ldw, K);
-  char* p = ws;
-  if ((!dxr && !tb_grid_ok((M * (Kp / CE) + 255) / 256, 256)) || (!dwr && !tb_grid_ok(((long)N * (Kp / CE) + 255) / 256, 256)))
+  T* xp = reinterpret_cast<T*>(ws);
+  ws += tb_align_up((size_t)M * Kp * sizeof(T), 256);
+  T* wp = reinterpret_cast<T*>(ws);
+  ws += tb_align_up((size_t)N * Kp * sizeof(T), 256);
+  const long bx = dxr ? 0 : (M * (Kp / CE) + 255) / 256, bw = dwr ? 0 : ((long)N * (Kp / CE) + 255) / 256;
+  if (!tb_grid_ok(bx + bw, 256))
     return tb_set_error(TB_ERR_UNSUPPORTED, "linres_fwd: M=%ld K=%d N=%d, off the alignment of 16 bytes, are too many in one call", M, K, N);
-  if (!dxr) {
-    pack_rows<T><<<(unsigned)((M * (Kp / CE) + 255) / 256), 256, 0, s>>>(x, ldx, M, K, reinterpret_cast<T*>(p), (int)Kp);
+  if (bx + bw) {
+    pack_rows<T><<<(unsigned)(bx + bw), 256, 0, s>>>(Rows<T>{x, ldx, M, xp}, Rows<T>{W, ldw, N, wp}, (unsigned)bx, K, (int)Kp);
     TB_LAUNCH_CHECK("linres pack");
-    x = reinterpret_cast<T*>(p);
+  }
+  if (!dxr) {
+    x = xp;
     ldx = Kp;
   }
-  p += tb_align_up((size_t)M * Kp * sizeof(T), 256);
   if (!dwr) {
-    pack_rows<T><<<(unsigned)(((long)N * (Kp / CE) + 255) / 256), 256, 0, s>>>(W, ldw, N, K, reinterpret_cast<T*>(p), (int)Kp);
-    TB_LAUNCH_CHECK("linres pack");
-    W = reinterpret_cast<T*>(p);
+    W = wp;
     ldw = Kp;
   }
-  p += tb_align_up((size_t)N * Kp * sizeof(T), 256);
-  return launch_gemm<T>(x, ldx, W, ldw, M, N, Kp, e, reinterpret_cast<float*>(p), s);
+  return launch_gemm<T>(x, ldx, W, ldw, M, N, Kp, e, reinterpret_cast<float*>(ws), s);
 }
 
 // rows of what the backward pass lays out start on whole lines (a row off them costs its copies another line each)
