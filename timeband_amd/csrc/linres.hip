@@ -231,7 +231,7 @@ __device__ __forceinline__ void whole_rows(const GemmArgs& a, const float* own, 
 
 // 64 x 64 sums of a wave, in LDS as gemm leaves them, through the epilogue to memory
 template <typename T>
-__device__ __forceinline__ void write_block(const GemmArgs& a, const float* own, long m0, int n0, int lane) {
+__device__ __forceinline__ void write_block(const GemmArgs& a, const float* own, long m0, int n0, int lane, int part) {
   const Epi& e = a.e;
   auto piece = [&](int r, int c) { return *reinterpret_cast<const f32x4*>(own + r * 64 + ((c ^ (r & 15)) * 4)); };
   if (e.slab) {
@@ -242,7 +242,7 @@ __device__ __forceinline__ void write_block(const GemmArgs& a, const float* own,
       const long m = m0 + r;
       if (m >= a.M) break;
       const f32x4 v = piece(r, c);
-      float* s = e.slab + ((long)blockIdx.y * a.M + m) * a.N + n;
+      float* s = e.slab + ((long)part * a.M + m) * a.N + n;
       if (n + 4 <= a.N) {
         const float o[4] = {v[0], v[1], v[2], v[3]};
         tb_store_u(s, o);
@@ -269,22 +269,21 @@ __device__ __forceinline__ void write_block(const GemmArgs& a, const float* own,
 // DOWN (fp32, for dW): k runs down the columns of both operands as they are, P[k][m] and Q[k][n], K rows of M and N columns that are
 // whole 16-byte pieces on 16 bytes.  A tile is sixteen rows of BM (BN) columns; a lane takes its k one by one (4 bytes), which the
 // fp32 instructions, a quarter of the 16-bit ones' rate a byte, leave time for.  Saves the transposed copies of dz and x
-// (65536 x 256 x 256: 345 -> 300 us of a training step).
+// (65536 x 256 x 256: 345 -> 306 us of a training step).
 template <typename T, int BM, int BN, int WM, int WN, bool DOWN>
-__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm(GemmArgs a) {
+__device__ __forceinline__ void product(const GemmArgs& a, int tile, int part, char* lds) {
   static_assert(!DOWN || (sizeof(T) == 4 && BM == 128 && BN == 128), "rows of 512 bytes, two a copy");
   constexpr int WAVES = (BM / WM) * (BN / WN), CE = 16 / sizeof(T), BK = 4 * CE;
   constexpr int MF = WM / 16, NF = WN / 16, LP = BM / 16 / WAVES, LQ = BN / 16 / WAVES;
   constexpr int STAGE = (BM + BN) * 64;
   static_assert(LP + LQ == 4, "the counted waits below are for four copies a wave and tile");
-  __shared__ __attribute__((aligned(16))) char lds[4 * STAGE];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int im, in;
-  tile_of(blockIdx.x, a.tm, a.tn, im, in);
+  tile_of(tile, a.tm, a.tn, im, in);
   const long m0 = (long)im * BM;
   const int n0 = in * BN;
   const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
-  const int kt0 = blockIdx.y * a.per, nt = min(a.per, (a.K + BK - 1) / BK - kt0);
+  const int kt0 = part * a.per, nt = min(a.per, (a.K + BK - 1) / BK - kt0);
 
   // What this lane copies: row 16 i + lane / 4 of each of its pieces, and of that row's four 16-byte pieces the one whose place
   // in LDS is lane % 4: piece p of row r lies at p ^ (r / 2 % 4), so that eight neighbouring rows fill all banks.
@@ -438,16 +437,39 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm(GemmArgs a
         *reinterpret_cast<f32x4*>(own + (i * 16 + (lane & 15)) * 64 + (((j * 4 + (lane >> 4)) ^ (lane & 15)) * 4)) = acc[h * 4 + i][j];
     __builtin_amdgcn_s_waitcnt(0xC07F);        // lgkmcnt(0): the block is this wave's own, no barrier
     asm volatile("" ::: "memory");
-    write_block<T>(a, own, m0 + wm + h * 64, n0 + wn, lane);
+    write_block<T>(a, own, m0 + wm + h * 64, n0 + wn, lane, part);
+  }
+}
+
+template <typename T, int BM, int BN, int WM, int WN, bool DOWN>
+__global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm(GemmArgs a) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * (BM + BN) * 64];
+  product<T, BM, BN, WM, WN, DOWN>(a, blockIdx.x, blockIdx.y, lds);
+}
+
+// Two products in one launch, the first's blocks in front (dW, whose k is long, and dx): neither fills the chip to its end alone.
+// With the layouts before them and the finishes behind them in one launch each, a training step of 4099 x 1000 x 1500 fp16 takes 104 us
+// (launch by launch 121), 1024^3 fp32 92 (106), 145 x 560 x 301 fp16 38 (46).
+template <typename T, bool DOWN>
+__global__ void __launch_bounds__(256, 2) gemm_pair(GemmArgs a, GemmArgs b, unsigned first) {
+  __shared__ __attribute__((aligned(16))) char lds[4 * 256 * 64];
+  const bool second = blockIdx.x >= first;
+  const int id = blockIdx.x - (second ? first : 0);
+  if constexpr (DOWN) {
+    const int tiles = second ? b.tm * b.tn : a.tm * a.tn;
+    if (second) product<T, 128, 128, 64, 64, false>(b, id % tiles, id / tiles, lds);
+    else product<T, 128, 128, 64, 64, true>(a, id % tiles, id / tiles, lds);
+  } else {
+    const GemmArgs c = second ? b : a;
+    product<T, 128, 128, 64, 64, false>(c, id % (c.tm * c.tn), id / (c.tm * c.tn), lds);
   }
 }
 
 // the splits' sums and the epilogue: four columns a thread, four threads share a place's splits and are added in their order
 template <typename T>
-__global__ void __launch_bounds__(256) split_finish(Epi e, long M, int N, int splits) {
-  __shared__ float red[4][64][4];
+__device__ __forceinline__ void split_sum(const Epi& e, long M, int N, int splits, unsigned block, float (&red)[4][64][4]) {
   const int nq = (N + 3) / 4, x = threadIdx.x & 63, y = threadIdx.x >> 6;
-  const long id = (long)blockIdx.x * 64 + x;
+  const long id = (long)block * 64 + x;
   const bool on = id < M * nq;
   const long m = on ? id / nq : 0;
   const int n = on ? (int)(id % nq) * 4 : 0;
@@ -476,6 +498,49 @@ __global__ void __launch_bounds__(256) split_finish(Epi e, long M, int N, int sp
 #pragma unroll
   for (int i = 0; i < 4; ++i) s[i] = (red[0][x][i] + red[1][x][i]) + (red[2][x][i] + red[3][x][i]);
   finish4<T>(e, N, m, n, s);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) split_finish(Epi e, long M, int N, int splits) {
+  __shared__ float red[4][64][4];
+  split_sum<T>(e, M, N, splits, blockIdx.x, red);
+}
+
+// What the backward pass leaves for the end, in one launch: the split sums of dW and dx, and db from the sums of each 64 rows
+// (four columns a block, 64 threads a column, added in a fixed order).
+struct EndArgs {
+  Epi w, x;
+  long Mw, Mx;
+  int Nw, Nx, sw, sx;              // rows, columns and parts of each; a part count of one: nothing left to do
+  unsigned bw, bx, bb;             // blocks of each
+  const float* part;
+  long rows;
+  int N;
+  void* db;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) backward_end(EndArgs a) {
+  __shared__ float red[4][64][4];
+  if (blockIdx.x < a.bw) {
+    split_sum<T>(a.w, a.Mw, a.Nw, a.sw, blockIdx.x, red);
+  } else if (blockIdx.x < a.bw + a.bx) {
+    split_sum<T>(a.x, a.Mx, a.Nx, a.sx, blockIdx.x - a.bw, red);
+  } else {
+    const int x = threadIdx.x & 3, y = threadIdx.x >> 2, c = (int)(blockIdx.x - a.bw - a.bx) * 4 + x;
+    float s = 0.f;
+    if (c < a.N) {
+#pragma unroll 8
+      for (long r = y; r < a.rows; r += 64) s += a.part[r * a.N + c];
+    }
+    float(&q)[1024] = reinterpret_cast<float(&)[1024]>(red);
+    q[threadIdx.x] = s;
+#pragma unroll
+    for (int h = 128; h >= 4; h /= 2) {
+      __syncthreads();
+      if ((int)threadIdx.x < h) q[threadIdx.x] += q[threadIdx.x + h];
+    }
+    if (threadIdx.x < 4 && c < a.N) static_cast<T*>(a.db)[c] = (T)q[threadIdx.x];
+  }
 }
 
 struct FewArgs {
@@ -601,97 +666,98 @@ __device__ __forceinline__ void store_column(const float (&t)[64][65], int c, in
 
 // dst[c][r] = src[r][c]; dst's rows are padded by zeros to Rp.  64 x 64 a block, 16 bytes an access on both sides.
 template <typename T>
-__global__ void __launch_bounds__(256) transpose(const T* src, long ld, long R, int C, T* dst, long Rp) {
-  __shared__ float t[64][65];
-  const long r0 = (long)blockIdx.x * 64;
-  const int c0 = blockIdx.y * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
+struct Across {
+  const T* src;
+  long ld, R;
+  int C;
+  T* dst;
+  long Rp;
+  unsigned blocks;
+};
+template <typename T>
+__device__ __forceinline__ void across_block(const Across<T>& a, unsigned block, float (&t)[64][65]) {
+  const unsigned nr = (unsigned)((a.Rp + 63) / 64);
+  const long r0 = (long)(block % nr) * 64;
+  const int c0 = (int)(block / nr) * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
 #pragma unroll
   for (int i = 0; i < 64; i += 32) {
     float v[8];
-    load8(src, ld, R, C, r0 + y + i, c0 + x, v);
+    load8(a.src, a.ld, a.R, a.C, r0 + y + i, c0 + x, v);
 #pragma unroll
     for (int j = 0; j < 8; ++j) t[y + i][x + j] = v[j];
   }
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 64; i += 32)
-    if (c0 + y + i < C) store_column<T>(t, y + i, x, dst + (long)(c0 + y + i) * Rp, Rp, r0);
+    if (c0 + y + i < a.C) store_column<T>(t, y + i, x, a.dst + (long)(c0 + y + i) * a.Rp, a.Rp, r0);
 }
 
 // dz = dy act'(z) in both orders, each nullable, and the column sums of each 64 rows (fp32, before dz is rounded)
 template <typename T>
-__global__ void __launch_bounds__(256) form_dz(const T* dy, long ldy, const float* z, int act, long M, int N, T* dz, int Np, T* dzT, long Mp,
-                                               float* part) {
-  __shared__ float t[64][65];
-  __shared__ float red[4][64];
-  const long r0 = (long)blockIdx.x * 64;
-  const int c0 = blockIdx.y * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
+struct DzArgs {
+  const T* dy;
+  long ldy;
+  const float* z;
+  int act, N, Np;
+  long M, Mp;
+  T *dz, *dzT;
+  float* part;
+  unsigned blocks;
+};
+template <typename T>
+__device__ __forceinline__ void dz_block(const DzArgs<T>& a, unsigned block, float (&t)[64][65], float (&red)[4][64]) {
+  const unsigned nr = (unsigned)((a.M + 63) / 64), br = block % nr;
+  const long r0 = (long)br * 64;
+  const int c0 = (int)(block / nr) * 64, x = (threadIdx.x & 7) * 8, y = threadIdx.x >> 3;
 #pragma unroll
   for (int i = 0; i < 64; i += 32) {
     const long r = r0 + y + i;
     float v[8], p[8];
-    load8(dy, ldy, M, N, r, c0 + x, v);
-    if (z) {
-      load8(z, (long)N, M, N, r, c0 + x, p);
+    load8(a.dy, a.ldy, a.M, a.N, r, c0 + x, v);
+    if (a.z) {
+      load8(a.z, (long)a.N, a.M, a.N, r, c0 + x, p);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[j] *= act_grad(p[j], act);
+      for (int j = 0; j < 8; ++j) v[j] *= act_grad(p[j], a.act);
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) t[y + i][x + j] = v[j];
-    if (dz && r < M) {
+    if (a.dz && r < a.M) {
       constexpr int W = 16 / sizeof(T);
 #pragma unroll
       for (int k = 0; k < 8; k += W)
-        if (c0 + x + k < Np) {
+        if (c0 + x + k < a.Np) {
           float w[W];
 #pragma unroll
           for (int j = 0; j < W; ++j) w[j] = v[k + j];
-          tb_store_n(dz + r * Np + c0 + x + k, w);
+          tb_store_n(a.dz + r * a.Np + c0 + x + k, w);
         }
     }
   }
   __syncthreads();
-  if (dzT) {
+  if (a.dzT) {
 #pragma unroll
     for (int i = 0; i < 64; i += 32)
-      if (c0 + y + i < N) store_column<T>(t, y + i, x, dzT + (long)(c0 + y + i) * Mp, Mp, r0);
+      if (c0 + y + i < a.N) store_column<T>(t, y + i, x, a.dzT + (long)(c0 + y + i) * a.Mp, a.Mp, r0);
   }
-  if (part) {
+  if (a.part) {
     const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
     float s = 0.f;
 #pragma unroll
     for (int i = 0; i < 16; ++i) s += t[q * 16 + i][c];
     red[q][c] = s;
     __syncthreads();
-    if (q == 0 && c0 + c < N) part[(long)blockIdx.x * N + c0 + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
+    if (q == 0 && c0 + c < a.N) a.part[(long)br * a.N + c0 + c] = (red[0][c] + red[1][c]) + (red[2][c] + red[3][c]);
   }
 }
 
-// db from the sums of each 64 rows: sixteen columns a block, 64 threads a column, added in the order of the rows
+// what the backward products read, in one launch: dz, W and x with their axes exchanged (each may have no blocks)
 template <typename T>
-__global__ void __launch_bounds__(1024) colsum_finish(const float* part, long rows, int N, T* db) {
-  __shared__ float red[64][17];
-  const int x = threadIdx.x & 15, y = threadIdx.x >> 4, c = blockIdx.x * 16 + x;
-  float s = 0.f;
-  if (c < N) {
-    const long per = (rows + 63) / 64, r1 = min(rows, (y + 1) * per);
-#pragma unroll 4
-    for (long r = y * per; r < r1; ++r) s += part[r * N + c];
-  }
-  red[y][x] = s;
-  __syncthreads();
-  if (y < 16) {
-    s = (red[y * 4][x] + red[y * 4 + 1][x]) + (red[y * 4 + 2][x] + red[y * 4 + 3][x]);
-  }
-  __syncthreads();
-  if (y < 16) red[y][x] = s;
-  __syncthreads();
-  if (y == 0 && c < N) {
-    s = 0.f;
-#pragma unroll
-    for (int j = 0; j < 16; ++j) s += red[j][x];
-    db[c] = (T)s;
-  }
+__global__ void __launch_bounds__(256) lay_out(DzArgs<T> z, Across<T> w, Across<T> x) {
+  __shared__ float t[64][65];
+  __shared__ float red[4][64];
+  if (blockIdx.x < z.blocks) dz_block<T>(z, blockIdx.x, t, red);
+  else if (blockIdx.x < z.blocks + w.blocks) across_block<T>(w, blockIdx.x - z.blocks, t);
+  else across_block<T>(x, blockIdx.x - z.blocks - w.blocks, t);
 }
 
 constexpr int FEW = 32;     // rows up to which the kernel for few rows is taken
@@ -732,9 +798,8 @@ size_t slab_bytes(long M, int N, long K, int esize, bool down = false) {
   return p.splits > 1 ? tb_align_up((size_t)p.splits * M * N * 4, 256) : 0;
 }
 
-template <typename T, bool DOWN = false>
-int launch_gemm(const T* P, long ldp, const T* Q, long ldq, long M, int N, long K, Epi e, float* slab, hipStream_t s) {
-  const Plan p = plan(M, N, K, sizeof(T), DOWN);
+template <typename T>
+GemmArgs gemm_args(const Plan& p, const T* P, long ldp, const T* Q, long ldq, long M, int N, long K, Epi e, float* slab) {
   GemmArgs a{P, Q, ldp, ldq, M, N, (int)K, p.tm, p.tn, p.splits, p.per, 16 / (int)sizeof(T), e};
   auto whole = [&](int w) {
     const uintptr_t bytes = w * sizeof(T);
@@ -743,15 +808,18 @@ int launch_gemm(const T* P, long ldp, const T* Q, long ldq, long M, int N, long 
   };
   while (a.width > 1 && !whole(a.width)) a.width /= 2;
   a.e.slab = p.splits > 1 ? slab : nullptr;
-  const dim3 grid(p.tm * p.tn, p.splits);
+  return a;
+}
+
+unsigned split_blocks(const GemmArgs& a) { return a.splits > 1 ? (unsigned)((a.M * ((a.N + 3) / 4) + 63) / 64) : 0; }
+
+template <typename T, bool DOWN>
+int launch(const GemmArgs& a, bool big, hipStream_t s) {
+  const dim3 grid(a.tm * a.tn, a.splits);
   if constexpr (DOWN) gemm<T, 128, 128, 64, 64, true><<<grid, 256, 0, s>>>(a);
-  else if (p.big) gemm<T, 256, 256, 128, 64, false><<<grid, 512, 0, s>>>(a);
+  else if (big) gemm<T, 256, 256, 128, 64, false><<<grid, 512, 0, s>>>(a);
   else gemm<T, 128, 128, 64, 64, false><<<grid, 256, 0, s>>>(a);
   TB_LAUNCH_CHECK("linres gemm");
-  if (p.splits > 1) {
-    split_finish<T><<<(unsigned)((M * ((N + 3) / 4) + 63) / 64), 256, 0, s>>>(a.e, M, N, p.splits);
-    TB_LAUNCH_CHECK("linres split_finish");
-  }
   return TB_OK;
 }
 
@@ -794,14 +862,20 @@ int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, in
     W = wp;
     ldw = Kp;
   }
-  return launch_gemm<T>(x, ldx, W, ldw, M, N, Kp, e, reinterpret_cast<float*>(ws), s);
+  const Plan p = plan(M, N, Kp, sizeof(T));
+  const GemmArgs a = gemm_args<T>(p, x, ldx, W, ldw, M, N, Kp, e, reinterpret_cast<float*>(ws));
+  const int rc = launch<T, false>(a, p.big, s);
+  if (rc || a.splits == 1) return rc;
+  split_finish<T><<<split_blocks(a), 256, 0, s>>>(a.e, M, N, a.splits);
+  TB_LAUNCH_CHECK("linres split_finish");
+  return TB_OK;
 }
 
 // rows of what the backward pass lays out start on whole lines (a row off them costs its copies another line each)
 long pitch(long x, int esize) { return (x + 128 / esize - 1) / (128 / esize) * (128 / esize); }
 
 struct BwdSizes {
-  size_t dz, dzT, WT, xT, part, slab, total;
+  size_t dz, dzT, WT, xT, part, slab_x, slab_w, total;
   long Np, Mp;
 };
 BwdSizes bwd_sizes(long M, int K, int N, int es) {
@@ -813,10 +887,10 @@ BwdSizes bwd_sizes(long M, int K, int N, int es) {
   b.WT = tb_align_up((size_t)K * b.Np * es, 256);
   b.xT = tb_align_up((size_t)K * b.Mp * es, 256);
   b.part = tb_align_up((size_t)((M + 63) / 64) * N * 4, 256);
-  const size_t s1 = slab_bytes(M, K, up(N, es), es), s2 = slab_bytes(N, K, up(M, es), es), s3 = slab_bytes(N, K, M, es, true);
-  b.slab = s1 > s2 ? s1 : s2;
-  if (s3 > b.slab) b.slab = s3;
-  b.total = b.dz + b.dzT + b.WT + b.xT + b.part + b.slab + 256;
+  const size_t w = slab_bytes(N, K, up(M, es), es), wd = slab_bytes(N, K, M, es, true);
+  b.slab_x = slab_bytes(M, K, up(N, es), es);
+  b.slab_w = w > wd ? w : wd;
+  b.total = b.dz + b.dzT + b.WT + b.xT + b.part + b.slab_x + b.slab_w + 256;
   return b;
 }
 
@@ -829,42 +903,57 @@ int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, 
   T* WT = reinterpret_cast<T*>(ws + b.dz + b.dzT);
   T* xT = reinterpret_cast<T*>(ws + b.dz + b.dzT + b.WT);
   float* part = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT);
-  float* slab = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT + b.part);
+  float* slab_x = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT + b.part);
+  float* slab_w = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT + b.part + b.slab_x);
   const bool as_is = !z && direct<T>(dy, ldy, N);      // dz = dy, and its rows can be copied as they are
   const T* dzr = as_is ? dy : dz;
   const long ldz = as_is ? ldy : b.Np;
   const bool down = sizeof(T) == 4 && dW && direct<T>(x, ldx, K);      // dW from dz and x as they are
   const bool across = dW && !down;
-  if (!as_is || across || db) {
-    form_dz<T><<<dim3((unsigned)((M + 63) / 64), (unsigned)((b.Np + 63) / 64)), 256, 0, s>>>(
-        dy, ldy, z, act, M, N, as_is || !(dx || down) ? nullptr : dz, (int)b.Np, across ? dzT : nullptr, b.Mp, db ? part : nullptr);
-    TB_LAUNCH_CHECK("linres form_dz");
+
+  auto tiles = [](long rows, long cols) { return ((rows + 63) / 64) * ((cols + 63) / 64); };
+  const long nz = !as_is || across || db ? tiles(M, b.Np) : 0, nw = dx ? tiles(b.Np, K) : 0, nx = across ? tiles(b.Mp, K) : 0;
+  if (!tb_grid_ok(nz + nw + nx, 256)) return tb_set_error(TB_ERR_UNSUPPORTED, "linres_bwd: M=%ld K=%d N=%d are too many in one call", M, K, N);
+  if (nz + nw + nx) {
+    DzArgs<T> az{dy, ldy, z, act, N, (int)b.Np, M, b.Mp, as_is || !(dx || down) ? nullptr : dz, across ? dzT : nullptr, db ? part : nullptr, (unsigned)nz};
+    Across<T> aw{W, ldw, N, K, WT, b.Np, (unsigned)nw}, ax{x, ldx, M, K, xT, b.Mp, (unsigned)nx};
+    lay_out<T><<<(unsigned)(nz + nw + nx), 256, 0, s>>>(az, aw, ax);
+    TB_LAUNCH_CHECK("linres lay_out");
   }
-  if (db) {
-    colsum_finish<T><<<(unsigned)((N + 15) / 16), 1024, 0, s>>>(part, (M + 63) / 64, N, db);
-    TB_LAUNCH_CHECK("linres colsum_finish");
-  }
-  Epi e{};
-  if (dx) {
-    transpose<T><<<dim3((unsigned)((b.Np + 63) / 64), (unsigned)((K + 63) / 64)), 256, 0, s>>>(W, ldw, N, K, WT, b.Np);
-    TB_LAUNCH_CHECK("linres transpose");
-    e.y = dx;
-    const int rc = launch_gemm<T>(dzr, ldz, WT, b.Np, M, K, up(N, sizeof(T)), e, slab, s);
-    if (rc) return rc;
-  }
-  if constexpr (sizeof(T) == 4) {
-    if (down) {
-      e.y = dW;
-      const int rc = launch_gemm<T, true>(dzr, ldz, x, ldx, N, K, M, e, slab, s);
+
+  const long Kw = down ? M : up(M, sizeof(T)), Kx = up(N, sizeof(T));
+  const Plan pw = plan(N, K, Kw, sizeof(T), down), px = plan(M, K, Kx, sizeof(T));
+  Epi ew{}, ex{};
+  ew.y = dW;
+  ex.y = dx;
+  const GemmArgs gw = down ? gemm_args<T>(pw, dzr, ldz, x, ldx, N, K, Kw, ew, slab_w) : gemm_args<T>(pw, dzT, b.Mp, xT, b.Mp, N, K, Kw, ew, slab_w);
+  const GemmArgs gx = gemm_args<T>(px, dzr, ldz, WT, b.Np, M, K, Kx, ex, slab_x);
+  const long bw = (long)pw.tm * pw.tn * pw.splits, bx = (long)px.tm * px.tn * px.splits;
+  if (dx && dW && !pw.big && !px.big && tb_grid_ok(bw + bx, 256)) {
+    if constexpr (sizeof(T) == 4) {
+      if (down) gemm_pair<T, true><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
+      else gemm_pair<T, false><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
+    } else {
+      gemm_pair<T, false><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
+    }
+    TB_LAUNCH_CHECK("linres gemm_pair");
+  } else {
+    if (dW) {
+      int rc = TB_OK;
+      if constexpr (sizeof(T) == 4) rc = down ? launch<T, true>(gw, false, s) : launch<T, false>(gw, pw.big, s);
+      else rc = launch<T, false>(gw, pw.big, s);
+      if (rc) return rc;
+    }
+    if (dx) {
+      const int rc = launch<T, false>(gx, px.big, s);
       if (rc) return rc;
     }
   }
-  if (across) {
-    transpose<T><<<dim3((unsigned)((b.Mp + 63) / 64), (unsigned)((K + 63) / 64)), 256, 0, s>>>(x, ldx, M, K, xT, b.Mp);
-    TB_LAUNCH_CHECK("linres transpose");
-    e.y = dW;
-    const int rc = launch_gemm<T>(dzT, b.Mp, xT, b.Mp, N, K, up(M, sizeof(T)), e, slab, s);
-    if (rc) return rc;
+  EndArgs end{gw.e, gx.e, gw.M, gx.M, gw.N, gx.N, gw.splits, gx.splits, dW ? split_blocks(gw) : 0, dx ? split_blocks(gx) : 0,
+              db ? (unsigned)((N + 3) / 4) : 0, part, (M + 63) / 64, N, db};
+  if (end.bw + end.bx + end.bb) {
+    backward_end<T><<<end.bw + end.bx + end.bb, 256, 0, s>>>(end);
+    TB_LAUNCH_CHECK("linres backward_end");
   }
   return TB_OK;
 }
