@@ -11,9 +11,10 @@
 // would add a second rounding to act'), and dz is rounded to the operands' type because it enters the matrix instructions.
 // Both operands are copied straight to LDS (16 bytes a lane, 64 bytes of a row a tile), tiles ahead of their use; the 16-byte
 // pieces of a row change places by the row's low bits, so that the rows a fragment reads fall on different banks.
-// Measured (bf16, without activation or residual): 16384 x 8192 x 8192 1797 us, 1.22 PFLOP/s (the library's product 1376);
-// 16384 x 2048 x 8192 490 (379), with gelu and residual 574; what bounds the large tiles is LDS (125 of its 128 bytes a
-// clock at the matrix instructions' full rate), and behind it the epilogue, which one block a unit leaves uncovered.  Not kept: 256 x 128 tiles, two blocks a unit (main loop 507 us against 412 a 2048 of k, LDS bound), 128 x 128 a wave
+// Measured (bf16, without activation or residual): 16384 x 8192 x 8192 1790 us, 1.23 PFLOP/s (the library's product 1360);
+// 16384 x 2048 x 8192 497 (376), with gelu and residual 587; what bounds the large tiles is LDS (125 of its 128 bytes a
+// clock at the matrix instructions' full rate), and behind it the epilogue, which one block a unit leaves uncovered.  Not kept:
+// 256 x 128 tiles, two blocks a unit (main loop 507 us against 412 a 2048 of k, LDS bound), 128 x 128 a wave
 // (the compiler moves the 256 sums between register files: 219 TFLOP/s), 256 x 128 one block a unit for middle sizes (same).
 // Few rows (a batch of single tokens) are bound by reading W once: a kernel without LDS staging whose waves split K.
 #include "elem.h"
