@@ -663,3 +663,27 @@ def test_refusals():
     refused("expected shape", ops.linear_residual, x, rnd(2, 6, 8), residual=rnd(3, 2, 1, 6))
     refused("activation", ops.linear_residual, x, rnd(2, 6, 8), act=6)
     refused("throughout", ops.linear_residual, x, rnd(2, 6, 8, type=BF))
+
+
+def test_step_marks_its_state_as_changed():
+    """A state that a recorded call saved and a step then changes: its backward pass is refused, not computed from the new state."""
+    from timeband_amd import ops
+    x, w, state = rnd(3, 2, 5, 8).requires_grad_(True), rnd(4, 8, 4), rnd(5, 2, 3, 8)
+    y = ops.causal_conv(x, w, None, ops.ACT_SILU, state=state)
+    before = state._version
+    with torch.no_grad():
+        ops.causal_conv_step(rnd(6, 2, 8), state, w, None, ops.ACT_SILU)
+    assert state._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    h = rnd(7, 2, 8, 4)
+    before = h._version
+    with torch.no_grad():
+        ops.selective_scan_step(h, rnd(8, 2, 8), rnd(9, 2, 8), -torch.ones(8, 4, device="cuda"), rnd(10, 2, 4), rnd(11, 2, 4))
+    assert h._version > before
+    with torch.inference_mode():                      # tensors without a version are stepped as before
+        s = torch.zeros(2, 3, 8, device="cuda")
+        ops.causal_conv_step(rnd(6, 2, 8), s, w)
+    with torch.no_grad():
+        ops.causal_conv_step(rnd(6, 2, 8), s, w)
+    assert bool((s != 0).any())

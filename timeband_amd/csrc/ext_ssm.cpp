@@ -106,6 +106,12 @@ void inference_only(const char* what, std::initializer_list<const Tensor*> ts) {
   TORCH_CHECK(!wanted(ts), what, " updates its state in place and has no gradient: call it under torch.no_grad()");
 }
 
+// what a step wrote over counts as changed: a recorded call that saved it refuses its backward pass (tensors made for inference only
+// have no count)
+void changed(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // A backward pass ends by making its stream wait for the streams that its leaves' accumulation nodes were made on.  Under
 // capture such a node from outside (an eager graph of the same leaf that somebody still holds) ties the capture to work
 // that is not part of it, and the process ends inside the runtime when the capture does.  Refused here, before anything is
@@ -273,6 +279,7 @@ Tensor causal_conv_step(Tensor x, Tensor state, Tensor w, OptT bias, int64_t act
   ok(tb_conv_step(ptr(x), x.stride(0), out_ptr(state), state.stride(0), ptr(w), ptr(b), w.scalar_type() == at::kFloat, out_ptr(y), fits(what, B),
                   fits(what, D), (int)K, (int)act, code, stream(x)),
      "tb_conv_step");
+  changed(state);
   return y;
 }
 
@@ -434,6 +441,7 @@ Tensor selective_scan_step(Tensor state, Tensor u, Tensor dt, Tensor A, Tensor B
   ok(tb_scan_step(out_fptr(state), state.stride(0), ptr(u), ptr(dt), ptr(z), ptr(Bm), ptr(Cm), st, fptr(A), fptr(D), fptr(bias), softplus, out_ptr(out),
                   fits(what, B), fits(what, Dn), (int)N, (int)G, code, stream(u)),
      "tb_scan_step");
+  changed(state);
   return out;
 }
 
