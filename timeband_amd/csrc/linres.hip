@@ -12,7 +12,7 @@
 // Both operands are copied straight to LDS (16 bytes a lane, 64 bytes of a row a tile), tiles ahead of their use; the 16-byte
 // pieces of a row change places by the row's low bits, so that the rows a fragment reads fall on different banks.
 // Measured (bf16, without activation or residual): 16384 x 8192 x 8192 1790 us, 1.23 PFLOP/s (the library's product 1360);
-// 16384 x 2048 x 8192 497 (376), with gelu and residual 587; what bounds the large tiles is LDS (125 of its 128 bytes a
+// 16384 x 2048 x 8192 493 (376), with gelu and residual 585; what bounds the large tiles is LDS (125 of its 128 bytes a
 // clock at the matrix instructions' full rate), and behind it the epilogue, which one block a unit leaves uncovered.  Not kept:
 // 256 x 128 tiles, two blocks a unit (main loop 507 us against 412 a 2048 of k, LDS bound), 128 x 128 a wave
 // (the compiler moves the 256 sums between register files: 219 TFLOP/s), 256 x 128 one block a unit for middle sizes (same).
@@ -161,7 +161,8 @@ __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& im, int& in
 }
 
 // The epilogue of rows that are whole pieces of V columns: the residual's pieces are fetched two accesses ahead of their use, the
-// activation is chosen once, outside the rows (16384 x 2048 x 8192 with gelu and residual: 685 -> 573 us).
+// activation is chosen once, outside the rows (16384 x 2048 x 8192 with gelu and residual: 685 us, so 585; without both 493, the residual
+// alone adds 58, gelu alone 58; four and eight accesses ahead: 606 and 671).
 template <typename T, int V>
 __device__ __forceinline__ void whole_rows(const GemmArgs& a, const float* own, long m0, int n0, int lane) {
   constexpr int L = 64 / V;      // lanes a row; V rows an access, L accesses
