@@ -15,7 +15,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libtimeband_hip.so")
-SOURCES = ["capi.hip", "gemm.hip", "lstm.hip", "losses.hip", "postproc.hip", "head.hip", "conv.hip", "scan.hip", "linres.hip"]
+SOURCES = ["conv.hip", "scan.hip", "lstm.hip", "linres.hip", "gemm.hip", "postproc.hip", "losses.hip", "head.hip", "capi.hip"]      # slowest first
 # -packed-fp32-ops: no v_pk_{add,mul,fma}_f32 (some of their forms have given wrong results on this part now and then); the
 # host pass does not know the feature and says so, which is harmless.
 FLAGS = ["-O3", "--offload-arch=gfx950", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function",
@@ -37,7 +37,7 @@ def needs_build():
     return any(os.path.getmtime(d) > t for d in deps)
 
 
-def build(force=False, verbose=True, jobs=6, stamps=False):
+def build(force=False, verbose=True, jobs=8, stamps=False):
     """stamps=True: diagnostic build with in-kernel cycle stamps (libtimeband_hip_stamps.so, tools only)."""
     if stamps:
         return _build(os.path.join(HERE, "build_stamps"), os.path.join(HERE, "libtimeband_hip_stamps.so"),
@@ -93,9 +93,19 @@ def build_ext(force=False, verbose=True):
     inc = [f"-I{p}" for p in ce.include_paths()] + [f"-I{sysconfig.get_paths()['include']}", "-I/opt/rocm/include",
                                                     f"-I{os.path.join(os.path.dirname(HERE), 'include')}"]
     cxx = shutil.which("g++") or "g++"
-    cmd = [cxx, "-O2", "-fPIC", "-shared", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-sign-compare",
-           "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_tbext", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc, *EXT_SRC, "-o", EXT,
+    flags = ["-O2", "-fPIC", "-std=c++17", "-Wall", "-Wno-unused-function", "-Wno-sign-compare",
+             "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1", "-DTORCH_EXTENSION_NAME=_tbext", "-DTORCH_API_INCLUDE_EXTENSION_H",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *inc]
+    os.makedirs(os.path.join(HERE, "build"), exist_ok=True)
+    objs = [os.path.join(HERE, "build", os.path.basename(f).replace(".cpp", "_cpp.o")) for f in EXT_SRC]
+    procs = []
+    for src, obj in zip(EXT_SRC, objs):
+        cmd = [cxx, *flags, "-c", src, "-o", obj]
+        if verbose:
+            print(" ".join(cmd), flush=True)
+        procs.append((src, subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)))
+    _drain(procs)
+    cmd = [cxx, "-shared", *objs, "-o", EXT,
            f"-L{tlib}", "-lc10", "-lc10_hip", "-ltorch_cpu", "-ltorch_hip", "-ltorch", "-ltorch_python",
            f"-L{HERE}", "-l:libtimeband_hip.so", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{tlib}"]
     if verbose:
@@ -111,7 +121,7 @@ def _drain(procs):
         if out.strip():
             print(out, flush=True)
         if p.returncode != 0:
-            raise RuntimeError(f"hipcc failed on {src}")
+            raise RuntimeError(f"compilation of {src} failed")
 
 
 if __name__ == "__main__":
