@@ -31,9 +31,10 @@ constexpr int NMAX = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
 // steps a tile of the backward pass.  The states of a tile stay in registers, BWD * S of them, and up to S = 4 as many decays (computed
-// again on the way back, with three waves a SIMD instead of two: 16 x 1024 x 2048 bf16 818 us, so 721; beyond, they would spill:
-// 32 states 250 us, so 512).  A state is kept in memory every BWD steps.
-constexpr int bwd_tile(int S) { return S <= 2 ? 32 : S <= 8 ? 16 : 8; }
+// again on the way back, with three waves a SIMD instead of two: 16 x 1024 x 2048 bf16 818 us, so 721; beyond, they cost more than
+// they save).  A state is kept in memory every BWD steps.  Backward alone, us, 16 x 1024 x 1024: 32 states in tiles of 16 steps
+// bf16 629, fp32 652 (spills), of 8 steps 546, 557, of 8 with the decays kept 597, 671; 8 states fp32 of 32 steps 261, of 16 254.
+constexpr int bwd_tile(int S) { return S <= 1 ? 32 : S <= 4 ? 16 : 8; }
 template <int S>
 struct Tile {
   static constexpr int BWD = bwd_tile(S);
@@ -384,6 +385,10 @@ struct Row {
 template <typename T, int S, bool STATE, bool VEC>
 __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
   constexpr int TT = STATE ? 32 : Tile<S>::BWD, EPT = TT / 4, NP = 4 * S;
+  // The next tile's rows are fetched before the walk, and this one's kept over it, where that spills no registers: 16 x 1024 x 2048
+  // of 16 states fp16 532 us (fetched at the tile's start, and again behind the walk), so 500; 16 x 1000 x 1023 of 8 states bf16 343,
+  // so 295; 16 states fp32 344, with it 354; 64 states fp32 512, with it 570.
+  constexpr bool AHEAD = S < 16 && !(S == 4 && sizeof(T) == 4);
   __shared__ float sD[TT][CB][2], sG[TT][CB];           // delta, delta u; dy
   __shared__ float sB[STATE ? 1 : TT * NP], sC[TT * NP];
   __shared__ float sY[STATE ? 1 : TT][YS], sGB[STATE ? 1 : TT][YS], sGA[STATE ? 1 : TT][YS];
@@ -425,6 +430,19 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
   float sum = 0.f;
   __syncthreads();
 
+  struct {
+    Raw<T, EPT, VEC> u, dt, z, dout;
+    RawRows<T, S, TT> B, C;
+  } next;
+  auto fetch = [&](int t0, auto& r) {
+    const int tc = max(min(t0 + ct, tv - 1), 0);
+    if (!STATE) r.u.fetch(a.u, uo + (long)tc * a.sut, ch, a.Dg);
+    r.dt.fetch(a.dt, dof + (long)tc * a.sdt, ch, a.Dg);
+    r.dout.fetch(a.dout, go + (long)tc * a.sot, ch, a.Dg);
+    if (a.z) r.z.fetch(a.z, zo + (long)tc * a.szt, ch, a.Dg);
+    if (!STATE) r.B.fetch(a.Bm, bo, a.sBt, t0, tv, a.N);
+    r.C.fetch(a.Cm, co, a.sCt, t0, tv, a.N);
+  };
   for (int t0 = ts + (te - ts - 1) / TT * TT; t0 >= ts; t0 -= TT) {
     const int t = t0 + ct, tc = max(min(t, tv - 1), 0);
     const bool on = t < tv;
@@ -432,12 +450,13 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
     Raw<T, EPT, VEC> ru, rdt, rz, ro;
     {
       RawRows<T, S, TT> rB, rC;
-      if (!STATE) ru.fetch(a.u, uo + (long)tc * a.sut, ch, a.Dg);
-      rdt.fetch(a.dt, dof + (long)tc * a.sdt, ch, a.Dg);
-      ro.fetch(a.dout, go + (long)tc * a.sot, ch, a.Dg);
-      if (a.z) rz.fetch(a.z, zo + (long)tc * a.szt, ch, a.Dg);
-      if (!STATE) rB.fetch(a.Bm, bo, a.sBt, t0, tv, a.N);
-      rC.fetch(a.Cm, co, a.sCt, t0, tv, a.N);
+      if (!AHEAD || t0 + TT >= te) fetch(t0, next);
+      ru = next.u;
+      rdt = next.dt;
+      rz = next.z;
+      ro = next.dout;
+      rB = next.B;
+      rC = next.C;
       if (!STATE) ru.mask(on, ch, a.Dg, 0.f);
       rdt.mask(on, ch, a.Dg, a.softplus ? -INFINITY : 0.f);
       ro.mask(on, ch, a.Dg, 0.f);
@@ -454,6 +473,7 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
       if (!STATE) rB.store(sB, t0, tv, a.N);
       rC.store(sC, t0, tv, a.N);
     }
+    if (AHEAD && t0 > ts) fetch(t0 - TT, next);
     __syncthreads();
     if (STATE) {
 #pragma unroll 4
@@ -532,12 +552,14 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
           for (int i = 0; i < H; ++i) p[i] = v[i];
         }
       }
-      // again, from the caches: kept over the walk, they would take the registers of its states
-      ru.fetch(a.u, uo + (long)tc * a.sut, ch, a.Dg);
-      rdt.fetch(a.dt, dof + (long)tc * a.sdt, ch, a.Dg);
-      if (a.dz) {
-        ro.fetch(a.dout, go + (long)tc * a.sot, ch, a.Dg);
-        rz.fetch(a.z, zo + (long)tc * a.szt, ch, a.Dg);
+      // again, from the caches, where they would take the registers of the walk's states
+      if (!AHEAD) {
+        ru.fetch(a.u, uo + (long)tc * a.sut, ch, a.Dg);
+        rdt.fetch(a.dt, dof + (long)tc * a.sdt, ch, a.Dg);
+        if (a.dz) {
+          ro.fetch(a.dout, go + (long)tc * a.sot, ch, a.Dg);
+          rz.fetch(a.z, zo + (long)tc * a.szt, ch, a.Dg);
+        }
       }
     }
     __syncthreads();
