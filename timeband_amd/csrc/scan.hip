@@ -10,8 +10,9 @@
 //
 // Bound by arithmetic: an exponential (a quarter of the vector rate) and four other operations a state and step forward, as many again and
 // nine more backward, against two bytes an element and tensor; where the steps are cut, the first walk comes on top.  Measured, bf16,
-// 16 states, gated: 1 x 16384 x 2048 268 us (537 M state steps; the exponentials and operations of both walks alone are 205 at
-// the vector units' full rate); 4 x 2048 x 2048 with gradients 473 (vector units busy 78 % of the main backward pass, 85 to 93 % of the others).  Layout: a lane owns one channel and S = N/4 of
+// 16 states, gated: 1 x 16384 x 2048 270 us (537 M state steps; the exponentials and operations of both walks alone are 205 at
+// the vector units' full rate); 4 x 2048 x 2048 with gradients 459 (vector units busy 81 % of the main backward pass, 87 to 93 % of the
+// others).  Layout: a lane owns one channel and S = N/4 of
 // its states, four neighbouring lanes a channel, so that the sum over the states is two quad permutes and a block of four
 // waves owns 64 neighbouring channels (whole lines of every tensor).  Steps go in tiles: a tile's rows are fetched into
 // registers one tile ahead, what does not depend on the state (softplus, the gate's derivative) is computed once per element
@@ -31,8 +32,8 @@ constexpr int NMAX = 64;
 constexpr float LOG2E = 1.4426950408889634f;
 
 // steps a tile of the backward pass.  The states of a tile stay in registers, BWD * S of them, and up to S = 4 as many decays (computed
-// again on the way back, with three waves a SIMD instead of two: 16 x 1024 x 2048 bf16 818 us, so 721; beyond, they cost more than
-// they save).  A state is kept in memory every BWD steps.  Backward alone, us, 16 x 1024 x 1024: 32 states in tiles of 16 steps
+// again on the way back, with three waves a SIMD instead of two: 16 x 1024 x 2048 bf16 818 us, so 721, and 690 with the
+// next tile fetched ahead; beyond, they cost more than they save).  A state is kept in memory every BWD steps.  Backward alone, us, 16 x 1024 x 1024: 32 states in tiles of 16 steps
 // bf16 629, fp32 652 (spills), of 8 steps 546, 557, of 8 with the decays kept 597, 671; 8 states fp32 of 32 steps 261, of 16 254.
 constexpr int bwd_tile(int S) { return S <= 1 ? 32 : S <= 4 ? 16 : 8; }
 template <int S>
