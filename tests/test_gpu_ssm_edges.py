@@ -1,0 +1,97 @@
+"""GPU: the state space layer's operators where they went wrong once, or could unseen: gradients through 16-bit products, infinities,
+long and uncut walks, every dispatch branch of the linear layer's backward pass.  Plain forms and `near`: ssm_reference."""
+import pytest
+import torch
+
+import ssm_reference as R
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+INF, NAN = float("inf"), float("nan")
+near = R.near
+
+
+@pytest.fixture(autouse=True)
+def poisoned():
+    """Memory that the allocator hands out again holds NaN: what a kernel does not write, or reads unwritten, shows."""
+    for n in (1 << 24, 1 << 20, 1 << 12, 256):
+        torch.full((n // 4,), NAN, device="cuda")
+    yield
+
+
+def rnd(seed, *shape, type=FP, scale=1.0):
+    g = torch.Generator().manual_seed(seed)
+    return (torch.randn(shape, generator=g) * scale).to(type).cuda()
+
+
+def req(*ts):
+    return [t.requires_grad_(True) for t in ts]
+
+
+def rounded_once(got, want, what):
+    """got is the 64-bit `want` with an error far below its type's step, rounded once: its distance is that of want's own rounding.
+    Over n values that distance's square scatters by 0.9 / sqrt(n) of itself; 25000 values leave 0.3 % on the distance, and 3 % is
+    ten times that.  A second rounding of the same size gives 41 %."""
+    g = got.detach().to("cpu", torch.float64)
+    assert g.numel() >= 25000 and torch.isfinite(g).all(), what
+    ratio = float((g - want).norm() / (want.to(got.dtype).double() - want).norm())
+    assert ratio < 1.03, (what, ratio)
+
+
+# ---- linear: dz of 16-bit types --------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", [BF, HF])
+@pytest.mark.parametrize("kind", [1, 2, 3, 4, 5])
+@pytest.mark.parametrize("M,K,N", [(257, 200, 256), (2049, 132, 200), (300, 90, 1501), (1500, 301, 84)])
+def test_linear_gradients_of_16_bits_are_rounded_once(M, K, N, kind, type):
+    """dz = dy act'(z) must not be rounded to the operands' type before the products: that doubles the gradients' error.  relu:
+    dz is dy or 0, exact; z's sign is clear of its rounding errors (|z| > 0.5 by the bias)."""
+    from timeband_amd import ops
+    x, W, b, dy = rnd(1, M, K, type=type), rnd(2, N, K, type=type, scale=K ** -0.5), rnd(3, N, type=type), rnd(5, M, N, type=type)
+    if kind == 3:
+        W, b = W * 0.05, torch.where(b > 0, b + 1, b - 1)
+    req(x, W, b)
+    got = torch.autograd.grad(ops.linear_residual(x, W, b, kind), (x, W, b), dy)
+    _, dx, dW, _ = R.linear(x, W, b, kind, None, dy)
+    rounded_once(got[0], dx, "dx")
+    rounded_once(got[1], dW, "dW")
+
+
+def test_linear_gradients_at_the_ends_of_fp16():
+    """dy near the largest value where the activation's slope is above 1: dz is past the type, the gradients are not.  dy among the
+    smallest values: dz is below the type's steps, its sums over many rows are not."""
+    from timeband_amd import ops
+    M, K, N = 80, 320, 330
+    x, W, b = rnd(1, M, K, type=HF, scale=1e-3), rnd(2, N, K, type=HF, scale=5e-3), torch.full((N,), 1.4, dtype=HF, device="cuda")
+    dy = (65504 * torch.sign(rnd(3, M, N))).to(HF)
+    req(x, W, b)
+    for kind in (4, 5):
+        got = torch.autograd.grad(ops.linear_residual(x, W, b, kind), (x, W), dy)
+        _, dx, dW, _ = R.linear(x, W, b, kind, None, dy)
+        assert float(dx.abs().max()) < 60000 and float(dW.abs().max()) < 60000
+        rounded_once(got[0], dx, "dx")
+        rounded_once(got[1], dW, "dW")
+    M, K, N = 6000, 200, 200
+    x, W, dy = rnd(4, M, K, type=HF), rnd(5, N, K, type=HF, scale=K ** -0.5), rnd(6, M, N, type=HF, scale=2.0 ** -21)
+    req(x, W)
+    for kind in (1, 2, 4, 5):
+        got = torch.autograd.grad(ops.linear_residual(x, W, None, kind), (x, W), dy)
+        _, dx, dW, _ = R.linear(x, W, None, kind, None, dy)
+        rounded_once(got[1], dW, "dW")
+        rounded_once(got[0], dx, "dx")
+
+
+def test_linear_infinite_gradients_stay_in_their_rows():
+    """An infinite or NaN dy: the infinities and NaN that the formula gives, in its row of dx and its column of dW alone."""
+    from timeband_amd import ops
+    for type in (FP, BF, HF):
+        x, W, dy = rnd(1, 90, 40, type=type), rnd(2, 48, 40, type=type), rnd(3, 90, 48, type=type)
+        req(x, W)
+        y = ops.linear_residual(x, W, None, ops.ACT_SIGMOID)
+        clean = torch.autograd.grad(y, (x, W), dy, retain_graph=True)
+        dy[7, 5], dy[8, 6] = INF, NAN
+        dx, dW = torch.autograd.grad(y, (x, W), dy)
+        rows, cols = [i for i in range(90) if i not in (7, 8)], [i for i in range(48) if i not in (5, 6)]
+        assert torch.equal(dx[rows], clean[0][rows]) and torch.equal(dW[cols], clean[1][cols])
+        assert torch.equal(dx[7].float(), INF * torch.sign(W[5].float())) and torch.isnan(dx[8]).all()
+        assert torch.equal(dW[5].float(), INF * torch.sign(x[7].float())) and torch.isnan(dW[6]).all()

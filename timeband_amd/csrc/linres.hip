@@ -8,7 +8,9 @@
 // the kernel that forms dz = dy act'(z) writes both orders and the column sums of db in its one pass.
 // 16-bit operands go through v_mfma_f32_16x16x32, fp32 ones through v_mfma_f32_16x16x4 (exact fp32 products: no splitting
 // into 16-bit parts, so infinities and the type's whole range pass).  Sums are fp32, z is kept in fp32 for the gradient (kept in 16 bits it
-// would add a second rounding to act'), and dz is rounded to the operands' type because it enters the matrix instructions.
+// would add a second rounding to act').  dz enters the matrix instructions in the operands' type: as it is where that holds it (no
+// activation, relu), else, of 16-bit types, in two parts (Halves below), since one rounding of dz alone puts the gradients off by as
+// much as their own (4099 x 1000 x 1500 fp16 against 64 bits: 2.93e-4 instead of 2.07e-4) and loses fp16 gradients outside its range.
 // Both operands are copied straight to LDS (16 bytes a lane, 64 bytes of a row a tile), tiles ahead of their use; the 16-byte
 // pieces of a row change places by the row's low bits, so that the rows a fragment reads fall on different banks.
 // Measured (bf16, without activation or residual): 16384 x 8192 x 8192 1790 us, 1.23 PFLOP/s (the library's product 1360);
@@ -96,6 +98,21 @@ struct Mfma<float> {
   }
 };
 
+// dz of 16-bit operands in two values of their type: hi, rounded, and lo, what that left out, together good to 2^-16 (bf16) and
+// 2^-21 (fp16).  fp16's range is short at both ends: hi is halved, so that |act'| < 2 cannot push it past the largest value, and lo is
+// enlarged, so that it still counts below the smallest.  A product runs over lo first, turns its sums to hi's scale (LO_TO_HI), runs
+// over hi and undoes the halving (OUT).
+template <typename T>
+struct Halves {
+  static constexpr bool F16 = std::is_same_v<T, _Float16>;
+  static constexpr float HI = F16 ? 0.5f : 1.f, LO = F16 ? 1024.f : 1.f, LO_TO_HI = HI / LO, OUT = 1.f / HI;
+  static __device__ __forceinline__ float hi(float v) { return v * HI; }
+  static __device__ __forceinline__ float lo(float v) {
+    const float h = (float)(T)(v * HI);
+    return fabsf(h) < INFINITY ? (v - h * OUT) * LO : 0.f;      // infinities and NaN are hi's alone
+  }
+};
+
 struct Epi {
   const void *bias, *res;   // element type T, each nullable
   void* y;                  // M x N dense
@@ -142,10 +159,11 @@ __device__ __forceinline__ void finish4(const Epi& e, int N, long m, int n, floa
 
 struct GemmArgs {
   const void *P, *Q;        // P: M rows, Q: N rows; rows start on 16 bytes, K a multiple of 16 bytes
+  const void* lo;           // the second part of P, laid out as P is, nullable (Halves)
   long ldp, ldq;
   long M;
   int N, K;
-  int tm, tn, splits, per;  // tiles; k tiles a split
+  int tm, tn, splits, per;  // tiles; k tiles a split (with two parts of P: of both, lo's first)
   int width;                // columns an access of the epilogue, of which every row is whole: 8 (16-bit types), 4, 2 or 1
   Epi e;
 };
@@ -272,9 +290,13 @@ __device__ __forceinline__ void write_block(const GemmArgs& a, const float* own,
 // whole 16-byte pieces on 16 bytes.  A tile is sixteen rows of BM (BN) columns; a lane takes its k one by one (4 bytes), which the
 // fp32 instructions, a quarter of the 16-bit ones' rate a byte, leave time for.  Saves the transposed copies of dz and x
 // (65536 x 256 x 256: 345 -> 306 us of a training step).
-template <typename T, int BM, int BN, int WM, int WN, bool DOWN>
+//
+// TWO: P comes in two parts, and k runs over all of lo and then over all of P (twice the products; 4099 x 1000 x 1500 fp16 with SiLU and
+// gradients: 145 us, with dz rounded once 102).
+template <typename T, int BM, int BN, int WM, int WN, bool DOWN, bool TWO>
 __device__ __forceinline__ void product(const GemmArgs& a, int tile, int part, char* lds) {
   static_assert(!DOWN || (sizeof(T) == 4 && BM == 128 && BN == 128), "rows of 512 bytes, two a copy");
+  static_assert(!TWO || sizeof(T) == 2, "fp32 holds dz as it is");
   constexpr int WAVES = (BM / WM) * (BN / WN), CE = 16 / sizeof(T), BK = 4 * CE;
   constexpr int MF = WM / 16, NF = WN / 16, LP = BM / 16 / WAVES, LQ = BN / 16 / WAVES;
   constexpr int STAGE = (BM + BN) * 64;
@@ -285,7 +307,8 @@ __device__ __forceinline__ void product(const GemmArgs& a, int tile, int part, c
   const long m0 = (long)im * BM;
   const int n0 = in * BN;
   const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
-  const int kt0 = part * a.per, nt = min(a.per, (a.K + BK - 1) / BK - kt0);
+  const int kt = (a.K + BK - 1) / BK;                    // k tiles of a part of P
+  int kt0 = part * a.per, nt = min(a.per, kt - kt0);      // TWO: set for each part below
 
   // What this lane copies: row 16 i + lane / 4 of each of its pieces, and of that row's four 16-byte pieces the one whose place
   // in LDS is lane % 4: piece p of row r lies at p ^ (r / 2 % 4), so that eight neighbouring rows fill all banks.
@@ -293,6 +316,7 @@ __device__ __forceinline__ void product(const GemmArgs& a, int tile, int part, c
   // of a read fall on different banks.
   const int lr = DOWN ? lane >> 5 : lane >> 2;
   const int piece = (DOWN ? (lane & 31) : (lane & 3) ^ ((lr >> 1) & 3)) * CE;
+  const T* const P = static_cast<const T*>(TWO ? a.lo : a.P);
   const T* pp[LP];
   const T* qp[LQ];
   int pr[LP], qr[LQ];              // DOWN: the row within a tile, or past every K where the columns are behind the last
@@ -301,12 +325,12 @@ __device__ __forceinline__ void product(const GemmArgs& a, int tile, int part, c
     if constexpr (DOWN) {
       const int row = (wave * LP + i) * 2 + lr;
       const long c = m0 + (piece ^ (row & 3) * 16);
-      pp[i] = static_cast<const T*>(a.P) + (c < a.M ? c : 0) + row * a.ldp;
+      pp[i] = P + (c < a.M ? c : 0) + row * a.ldp;
       pr[i] = c < a.M ? row : 1 << 30;
     } else {
       long r = m0 + (wave * LP + i) * 16 + lr;
       r = r < a.M ? r : a.M - 1;                // rows behind the last: any row, never stored
-      pp[i] = static_cast<const T*>(a.P) + r * a.ldp + piece;
+      pp[i] = P + r * a.ldp + piece;
     }
   }
 #pragma unroll
@@ -393,7 +417,8 @@ __device__ __forceinline__ void product(const GemmArgs& a, int tile, int part, c
   };
   constexpr std::true_type yes{};
   constexpr std::false_type no{};
-  if (nt > 0) {
+  auto all_tiles = [&] {
+    if (nt <= 0) return;
     for (int t = 0; t < 4 && t < nt; ++t) copy(t, yes);
     meet(yes);
     read(0, fp[0], fq[0]);
@@ -420,6 +445,32 @@ __device__ __forceinline__ void product(const GemmArgs& a, int tile, int part, c
         multiply(fp[1], fq[1]);
       }
     }
+  };
+  if constexpr (TWO) {
+    const int k0 = part * a.per, k1 = min(k0 + a.per, 2 * kt);
+#pragma unroll 1
+    for (int i = 0; i < 2; ++i) {
+      kt0 = max(k0 - i * kt, 0);
+      nt = min(k1 - i * kt, kt) - kt0;
+      if (i) {
+        __syncthreads();                  // every wave has read lo's last tile: its place is free
+#pragma unroll
+        for (int j = 0; j < LP; ++j) pp[j] += static_cast<const T*>(a.P) - P;
+        if constexpr (Halves<T>::LO_TO_HI != 1.f)
+#pragma unroll
+          for (int m = 0; m < MF; ++m)
+#pragma unroll
+            for (int n = 0; n < NF; ++n) acc[m][n] *= Halves<T>::LO_TO_HI;
+      }
+      all_tiles();
+    }
+    if constexpr (Halves<T>::OUT != 1.f)
+#pragma unroll
+      for (int m = 0; m < MF; ++m)
+#pragma unroll
+        for (int n = 0; n < NF; ++n) acc[m][n] *= Halves<T>::OUT;
+  } else {
+    all_tiles();
   }
   // A lane holds row lane & 15 and four neighbouring columns of each 16 x 16 piece (Q is the left operand).  They change
   // places through LDS, 64 rows at a time in each wave's own 16 KB, so that every access to memory is of whole rows of
@@ -443,27 +494,27 @@ __device__ __forceinline__ void product(const GemmArgs& a, int tile, int part, c
   }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, bool DOWN>
+template <typename T, int BM, int BN, int WM, int WN, bool DOWN, bool TWO>
 __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm(GemmArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[4 * (BM + BN) * 64];
-  product<T, BM, BN, WM, WN, DOWN>(a, blockIdx.x, blockIdx.y, lds);
+  product<T, BM, BN, WM, WN, DOWN, TWO>(a, blockIdx.x, blockIdx.y, lds);
 }
 
 // Two products in one launch, the first's blocks in front (dW, whose k is long, and dx): neither fills the chip to its end alone.
 // With the layouts before them and the finishes behind them in one launch each, a training step of 4099 x 1000 x 1500 fp16 takes 104 us
 // (launch by launch 121), 1024^3 fp32 92 (106), 145 x 560 x 301 fp16 38 (46).
-template <typename T, bool DOWN>
+template <typename T, bool DOWN, bool TWO>
 __global__ void __launch_bounds__(256, 2) gemm_pair(GemmArgs a, GemmArgs b, unsigned first) {
   __shared__ __attribute__((aligned(16))) char lds[4 * 256 * 64];
   const bool second = blockIdx.x >= first;
   const int id = blockIdx.x - (second ? first : 0);
   if constexpr (DOWN) {
     const int tiles = second ? b.tm * b.tn : a.tm * a.tn;
-    if (second) product<T, 128, 128, 64, 64, false>(b, id % tiles, id / tiles, lds);
-    else product<T, 128, 128, 64, 64, true>(a, id % tiles, id / tiles, lds);
+    if (second) product<T, 128, 128, 64, 64, false, TWO>(b, id % tiles, id / tiles, lds);
+    else product<T, 128, 128, 64, 64, true, TWO>(a, id % tiles, id / tiles, lds);
   } else {
     const GemmArgs c = second ? b : a;
-    product<T, 128, 128, 64, 64, false>(c, id % (c.tm * c.tn), id / (c.tm * c.tn), lds);
+    product<T, 128, 128, 64, 64, false, TWO>(c, id % (c.tm * c.tn), id / (c.tm * c.tn), lds);
   }
 }
 
@@ -648,12 +699,12 @@ __device__ __forceinline__ void load8(const T* src, long ld, long R, int C, long
     for (int i = 0; i < 8; ++i) v[i] = r < R && c + i < C ? (float)src[r * ld + c + i] : 0.f;
   }
 }
-// row c of the tile's columns r0 + x0 .. + 8 to dst[c][r], whose rows are Rp long (a multiple of 16 bytes)
-template <typename T>
-__device__ __forceinline__ void store_column(const float (&t)[64][65], int c, int x0, T* dst, long Rp, long r0) {
+// row c of the tile's columns r0 + x0 .. + 8, each through f, to dst[c][r], whose rows are Rp long (a multiple of 16 bytes)
+template <typename T, typename F>
+__device__ __forceinline__ void store_column(const float (&t)[64][65], int c, int x0, T* dst, long Rp, long r0, F&& f) {
   float v[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = t[x0 + i][c];
+  for (int i = 0; i < 8; ++i) v[i] = f(t[x0 + i][c]);
   constexpr int W = 16 / sizeof(T);
 #pragma unroll
   for (int i = 0; i < 8; i += W) {
@@ -691,10 +742,10 @@ __device__ __forceinline__ void across_block(const Across<T>& a, unsigned block,
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 64; i += 32)
-    if (c0 + y + i < a.C) store_column<T>(t, y + i, x, a.dst + (long)(c0 + y + i) * a.Rp, a.Rp, r0);
+    if (c0 + y + i < a.C) store_column<T>(t, y + i, x, a.dst + (long)(c0 + y + i) * a.Rp, a.Rp, r0, [](float v) { return v; });
 }
 
-// dz = dy act'(z) in both orders, each nullable, and the column sums of each 64 rows (fp32, before dz is rounded)
+// dz = dy act'(z) in both orders, each nullable, in one part or two, and the column sums of each 64 rows (fp32, before dz is rounded)
 template <typename T>
 struct DzArgs {
   const T* dy;
@@ -703,6 +754,8 @@ struct DzArgs {
   int act, N, Np;
   long M, Mp;
   T *dz, *dzT;
+  T *lo, *loT;         // two parts: the second ones, where the first are
+  bool two;
   float* part;
   unsigned blocks;
 };
@@ -725,21 +778,37 @@ __device__ __forceinline__ void dz_block(const DzArgs<T>& a, unsigned block, flo
     for (int j = 0; j < 8; ++j) t[y + i][x + j] = v[j];
     if (a.dz && r < a.M) {
       constexpr int W = 16 / sizeof(T);
+      auto put = [&](T* dst, auto&& f) {
 #pragma unroll
-      for (int k = 0; k < 8; k += W)
-        if (c0 + x + k < a.Np) {
-          float w[W];
+        for (int k = 0; k < 8; k += W)
+          if (c0 + x + k < a.Np) {
+            float w[W];
 #pragma unroll
-          for (int j = 0; j < W; ++j) w[j] = v[k + j];
-          tb_store_n(a.dz + r * a.Np + c0 + x + k, w);
-        }
+            for (int j = 0; j < W; ++j) w[j] = f(v[k + j]);
+            tb_store_n(dst + r * a.Np + c0 + x + k, w);
+          }
+      };
+      if (a.two) {
+        put(a.dz, [](float q) { return Halves<T>::hi(q); });
+        put(a.lo, [](float q) { return Halves<T>::lo(q); });
+      } else {
+        put(a.dz, [](float q) { return q; });
+      }
     }
   }
   __syncthreads();
   if (a.dzT) {
 #pragma unroll
     for (int i = 0; i < 64; i += 32)
-      if (c0 + y + i < a.N) store_column<T>(t, y + i, x, a.dzT + (long)(c0 + y + i) * a.Mp, a.Mp, r0);
+      if (c0 + y + i < a.N) {
+        const long at = (long)(c0 + y + i) * a.Mp;
+        if (a.two) {
+          store_column<T>(t, y + i, x, a.dzT + at, a.Mp, r0, [](float q) { return Halves<T>::hi(q); });
+          store_column<T>(t, y + i, x, a.loT + at, a.Mp, r0, [](float q) { return Halves<T>::lo(q); });
+        } else {
+          store_column<T>(t, y + i, x, a.dzT + at, a.Mp, r0, [](float q) { return q; });
+        }
+      }
   }
   if (a.part) {
     const int c = threadIdx.x & 63, q = threadIdx.x >> 6;
@@ -774,9 +843,9 @@ struct Plan {
 // idle, into parts of sixteen k tiles (1 KB of a row) at least, of fp32, whose products take longer a byte, of four: 1000 x 1000 x 1000
 // fp32 in parts of 16, 8, 4, 2 tiles 33.5, 29.9, 29.6, 29.7 us, 241 x 2048 x 272 24.5, 18.2, 16.4, 16.4; 1024 x 1024 x 1024 bf16
 // 16.7, 20.4, 20.4, 20.5.
-Plan plan(long M, int N, long K, int esize, bool down = false) {
+Plan plan(long M, int N, long K, int esize, bool down = false, int parts = 1) {
   Plan p;
-  const long cus = tb_num_cus(), kt = (K * esize + 63) / 64;
+  const long cus = tb_num_cus(), kt = (K * esize + 63) / 64 * parts;
   const long big = ((M + 255) / 256) * ((N + 255) / 256);
   p.big = big >= cus && !down;
   const int b = p.big ? 256 : 128;
@@ -795,14 +864,14 @@ Plan plan(long M, int N, long K, int esize, bool down = false) {
   p.splits = (int)((kt + p.per - 1) / p.per);
   return p;
 }
-size_t slab_bytes(long M, int N, long K, int esize, bool down = false) {
-  const Plan p = plan(M, N, K, esize, down);
+size_t slab_bytes(long M, int N, long K, int esize, bool down = false, int parts = 1) {
+  const Plan p = plan(M, N, K, esize, down, parts);
   return p.splits > 1 ? tb_align_up((size_t)p.splits * M * N * 4, 256) : 0;
 }
 
 template <typename T>
-GemmArgs gemm_args(const Plan& p, const T* P, long ldp, const T* Q, long ldq, long M, int N, long K, Epi e, float* slab) {
-  GemmArgs a{P, Q, ldp, ldq, M, N, (int)K, p.tm, p.tn, p.splits, p.per, 16 / (int)sizeof(T), e};
+GemmArgs gemm_args(const Plan& p, const T* P, long ldp, const T* Q, long ldq, long M, int N, long K, Epi e, float* slab, const T* lo = nullptr) {
+  GemmArgs a{P, Q, lo, ldp, ldq, M, N, (int)K, p.tm, p.tn, p.splits, p.per, 16 / (int)sizeof(T), e};
   auto whole = [&](int w) {
     const uintptr_t bytes = w * sizeof(T);
     return N % w == 0 && (!e.res || e.ldr % w == 0) && reinterpret_cast<uintptr_t>(e.y) % bytes == 0 && reinterpret_cast<uintptr_t>(e.res) % bytes == 0 &&
@@ -818,9 +887,17 @@ unsigned split_blocks(const GemmArgs& a) { return a.splits > 1 ? (unsigned)((a.M
 template <typename T, bool DOWN>
 int launch(const GemmArgs& a, bool big, hipStream_t s) {
   const dim3 grid(a.tm * a.tn, a.splits);
-  if constexpr (DOWN) gemm<T, 128, 128, 64, 64, true><<<grid, 256, 0, s>>>(a);
-  else if (big) gemm<T, 256, 256, 128, 64, false><<<grid, 512, 0, s>>>(a);
-  else gemm<T, 128, 128, 64, 64, false><<<grid, 256, 0, s>>>(a);
+  auto one = [&](auto two) {
+    if constexpr (DOWN) gemm<T, 128, 128, 64, 64, true, two><<<grid, 256, 0, s>>>(a);
+    else if (big) gemm<T, 256, 256, 128, 64, false, two><<<grid, 512, 0, s>>>(a);
+    else gemm<T, 128, 128, 64, 64, false, two><<<grid, 256, 0, s>>>(a);
+  };
+  if constexpr (sizeof(T) == 2) {
+    if (a.lo) one(std::true_type{});
+    else one(std::false_type{});
+  } else {
+    one(std::false_type{});
+  }
   TB_LAUNCH_CHECK("linres gemm");
   return TB_OK;
 }
@@ -880,17 +957,18 @@ struct BwdSizes {
   size_t dz, dzT, WT, xT, part, slab_x, slab_w, total;
   long Np, Mp;
 };
-BwdSizes bwd_sizes(long M, int K, int N, int es) {
+// dz and dzT in up to two parts, one behind the other
+BwdSizes bwd_sizes(long M, int K, int N, int es, int parts) {
   BwdSizes b;
   b.Np = pitch(N, es);
   b.Mp = pitch(M, es);
-  b.dz = tb_align_up((size_t)M * b.Np * es, 256);
-  b.dzT = tb_align_up((size_t)N * b.Mp * es, 256);
+  b.dz = tb_align_up((size_t)M * b.Np * es, 256) * parts;
+  b.dzT = tb_align_up((size_t)N * b.Mp * es, 256) * parts;
   b.WT = tb_align_up((size_t)K * b.Np * es, 256);
   b.xT = tb_align_up((size_t)K * b.Mp * es, 256);
   b.part = tb_align_up((size_t)((M + 63) / 64) * N * 4, 256);
-  const size_t w = slab_bytes(N, K, up(M, es), es), wd = slab_bytes(N, K, M, es, true);
-  b.slab_x = slab_bytes(M, K, up(N, es), es);
+  const size_t w = slab_bytes(N, K, up(M, es), es, false, parts), wd = slab_bytes(N, K, M, es, true);
+  b.slab_x = slab_bytes(M, K, up(N, es), es, false, parts);
   b.slab_w = w > wd ? w : wd;
   b.total = b.dz + b.dzT + b.WT + b.xT + b.part + b.slab_x + b.slab_w + 256;
   return b;
@@ -899,9 +977,12 @@ BwdSizes bwd_sizes(long M, int K, int N, int es) {
 template <typename T>
 int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, const float* z, int act, T* dx, T* dW, T* db, long M, int K,
              int N, char* ws, hipStream_t s) {
-  const BwdSizes b = bwd_sizes(M, K, N, sizeof(T));
+  const bool two = sizeof(T) == 2 && z && act != 3;     // dy act'(z) of relu is dy or 0: one value holds it
+  const BwdSizes b = bwd_sizes(M, K, N, sizeof(T), two ? 2 : 1);
   T* dz = reinterpret_cast<T*>(ws);
   T* dzT = reinterpret_cast<T*>(ws + b.dz);
+  T* const lo = two ? reinterpret_cast<T*>(ws + b.dz / 2) : nullptr;
+  T* const loT = two ? reinterpret_cast<T*>(ws + b.dz + b.dzT / 2) : nullptr;
   T* WT = reinterpret_cast<T*>(ws + b.dz + b.dzT);
   T* xT = reinterpret_cast<T*>(ws + b.dz + b.dzT + b.WT);
   float* part = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT);
@@ -917,26 +998,27 @@ int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, 
   const long nz = !as_is || across || db ? tiles(M, b.Np) : 0, nw = dx ? tiles(b.Np, K) : 0, nx = across ? tiles(b.Mp, K) : 0;
   if (!tb_grid_ok(nz + nw + nx, 256)) return tb_set_error(TB_ERR_UNSUPPORTED, "linres_bwd: M=%ld K=%d N=%d are too many in one call", M, K, N);
   if (nz + nw + nx) {
-    DzArgs<T> az{dy, ldy, z, act, N, (int)b.Np, M, b.Mp, as_is || !(dx || down) ? nullptr : dz, across ? dzT : nullptr, db ? part : nullptr, (unsigned)nz};
+    DzArgs<T> az{dy, ldy, z, act, N, (int)b.Np, M, b.Mp, as_is || !(dx || down) ? nullptr : dz, across ? dzT : nullptr, lo, loT, two, db ? part : nullptr, (unsigned)nz};
     Across<T> aw{W, ldw, N, K, WT, b.Np, (unsigned)nw}, ax{x, ldx, M, K, xT, b.Mp, (unsigned)nx};
     lay_out<T><<<(unsigned)(nz + nw + nx), 256, 0, s>>>(az, aw, ax);
     TB_LAUNCH_CHECK("linres lay_out");
   }
 
   const long Kw = down ? M : up(M, sizeof(T)), Kx = up(N, sizeof(T));
-  const Plan pw = plan(N, K, Kw, sizeof(T), down), px = plan(M, K, Kx, sizeof(T));
+  const Plan pw = plan(N, K, Kw, sizeof(T), down, two ? 2 : 1), px = plan(M, K, Kx, sizeof(T), false, two ? 2 : 1);
   Epi ew{}, ex{};
   ew.y = dW;
   ex.y = dx;
-  const GemmArgs gw = down ? gemm_args<T>(pw, dzr, ldz, x, ldx, N, K, Kw, ew, slab_w) : gemm_args<T>(pw, dzT, b.Mp, xT, b.Mp, N, K, Kw, ew, slab_w);
-  const GemmArgs gx = gemm_args<T>(px, dzr, ldz, WT, b.Np, M, K, Kx, ex, slab_x);
+  const GemmArgs gw = down ? gemm_args<T>(pw, dzr, ldz, x, ldx, N, K, Kw, ew, slab_w) : gemm_args<T>(pw, dzT, b.Mp, xT, b.Mp, N, K, Kw, ew, slab_w, loT);
+  const GemmArgs gx = gemm_args<T>(px, dzr, ldz, WT, b.Np, M, K, Kx, ex, slab_x, lo);
   const long bw = (long)pw.tm * pw.tn * pw.splits, bx = (long)px.tm * px.tn * px.splits;
   if (dx && dW && !pw.big && !px.big && tb_grid_ok(bw + bx, 256)) {
     if constexpr (sizeof(T) == 4) {
-      if (down) gemm_pair<T, true><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
-      else gemm_pair<T, false><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
+      if (down) gemm_pair<T, true, false><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
+      else gemm_pair<T, false, false><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
     } else {
-      gemm_pair<T, false><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
+      if (two) gemm_pair<T, false, true><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
+      else gemm_pair<T, false, false><<<(unsigned)(bw + bx), 256, 0, s>>>(gw, gx, (unsigned)bw);
     }
     TB_LAUNCH_CHECK("linres gemm_pair");
   } else {
@@ -977,7 +1059,10 @@ extern "C" {
 size_t tb_linres_workspace_bytes(long M, int K, int N, int dtype, int backward) {
   if (M < 1 || K < 1 || N < 1 || !tb_dtype_ok(dtype)) return 256;
   const int es = (int)tb_dtype_size(dtype);
-  if (backward) return bwd_sizes(M, K, N, es).total;
+  if (backward) {                                // whatever the activation: of 16-bit types in one part or two
+    const size_t one = bwd_sizes(M, K, N, es, 1).total, two = es == 2 ? bwd_sizes(M, K, N, es, 2).total : 0;
+    return one > two ? one : two;
+  }
   if (M <= FEW) return 256;
   const long Kp = up(K, es);
   return tb_align_up((size_t)M * Kp * es, 256) + tb_align_up((size_t)N * Kp * es, 256) + slab_bytes(M, N, Kp, es) + 256;
