@@ -95,3 +95,9 @@ def test_linear_infinite_gradients_stay_in_their_rows():
         assert torch.equal(dx[rows], clean[0][rows]) and torch.equal(dW[cols], clean[1][cols])
         assert torch.equal(dx[7].float(), INF * torch.sign(W[5].float())) and torch.isnan(dx[8]).all()
         assert torch.equal(dW[5].float(), INF * torch.sign(x[7].float())) and torch.isnan(dW[6]).all()
+
+
+# ---- modes of differentiation ------------------------------------------------------------------------------------------------
+def test_forward_mode_is_refused():
+    from test_ssm_edges_host import check_forward_mode_is_refused
+    check_forward_mode_is_refused("cuda")

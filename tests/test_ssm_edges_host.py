@@ -1,0 +1,34 @@
+"""CPU: what the state space layer's operators refuse before they look at a tensor's device."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+
+def forward_mode_calls(device):
+    """(name, call of one dual tensor, that tensor's primal) for every tensor of every operator."""
+    from timeband_amd import ops
+    z = lambda *s: torch.zeros(s, device=device)
+    calls = {
+        "causal_conv": (ops.causal_conv, dict(x=z(2, 5, 8), weight=z(8, 4), bias=z(8), state=z(2, 3, 8))),
+        "causal_conv_step": (ops.causal_conv_step, dict(x=z(2, 8), state=z(2, 3, 8), weight=z(8, 4), bias=z(8))),
+        "selective_scan": (ops.selective_scan, dict(u=z(2, 5, 8), dt=z(2, 5, 8), A=z(8, 4), B=z(2, 5, 4), C=z(2, 5, 4), D=z(8), z=z(2, 5, 8),
+                                                    dt_bias=z(8), h0=z(2, 8, 4))),
+        "selective_scan_step": (ops.selective_scan_step, dict(state=z(2, 8, 4), u=z(2, 8), dt=z(2, 8), A=z(8, 4), B=z(2, 4), C=z(2, 4), D=z(8),
+                                                              z=z(2, 8), dt_bias=z(8))),
+        "linear_residual": (ops.linear_residual, dict(x=z(40, 8), W=z(6, 8), b=z(6), residual=z(40, 6))),
+    }
+    for name, (f, args) in calls.items():
+        for k in args:
+            yield name, (lambda t, f=f, args=args, k=k: f(**{**args, k: t})), args[k]
+
+
+def check_forward_mode_is_refused(device):
+    for name, call, primal in forward_mode_calls(device):
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match=name + ": forward-mode"):
+                call(forward_ad.make_dual(primal, torch.ones_like(primal)))
+
+
+def test_forward_mode_is_refused():
+    """Without the refusal the result has no tangent, and x + f(x) would have that of x alone."""
+    check_forward_mode_is_refused("cpu")

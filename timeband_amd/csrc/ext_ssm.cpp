@@ -5,6 +5,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPException.h>
 #include <c10/hip/HIPStream.h>
@@ -100,6 +101,13 @@ bool wanted(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// Dual tensors (torch.autograd.forward_ad): without requires_grad a call passes its autograd Function by, and its result would have no
+// tangent, which counts as a zero one.
+void no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : ts) TORCH_CHECK(!t->defined() || !t->_fw_grad(0).defined(), what, ": forward-mode derivatives are not supported");
 }
 
 void inference_only(const char* what, std::initializer_list<const Tensor*> ts) {
@@ -232,6 +240,7 @@ void conv_params(const char* what, Tensor& w, Tensor& b, int64_t D, const Tensor
 py::object causal_conv(Tensor x, Tensor w, OptT bias, int64_t act, OptT state_, OptT lengths_, bool return_state) {
   const char* what = "causal_conv";
   Tensor b = opt(bias), state = opt(state_);
+  no_tangents(what, {&x, &w, &b, &state});
   check(what, x, {&state});
   TORCH_CHECK(x.dim() == 3, "causal_conv: x must be (B, T, D)");
   const int64_t B = x.size(0), D = x.size(2);
@@ -262,6 +271,7 @@ py::object causal_conv(Tensor x, Tensor w, OptT bias, int64_t act, OptT state_, 
 Tensor causal_conv_step(Tensor x, Tensor state, Tensor w, OptT bias, int64_t act) {
   const char* what = "causal_conv_step";
   Tensor b = opt(bias);
+  no_tangents(what, {&x, &w, &b, &state});
   const int code = check(what, x, {&state});
   TORCH_CHECK(x.dim() == 2, "causal_conv_step: x must be (B, D)");
   const int64_t B = x.size(0), D = x.size(1);
@@ -371,7 +381,8 @@ struct ScanFn : public torch::autograd::Function<ScanFn> {
 py::object selective_scan(Tensor u, Tensor dt, Tensor A, Tensor Bm, Tensor Cm, OptT D_, OptT z_, OptT bias_, bool softplus, OptT h0_, OptT lengths_,
                           bool return_state) {
   const char* what = "selective_scan";
-  Tensor z = opt(z_);
+  Tensor z = opt(z_), D = opt(D_), bias = opt(bias_), h0 = opt(h0_);
+  no_tangents(what, {&u, &dt, &A, &Bm, &Cm, &D, &z, &bias, &h0});
   check(what, u, {&dt, &Bm, &Cm, &z});
   TORCH_CHECK(u.dim() == 3, "selective_scan: u must be (B, T, D)");
   const int64_t B = u.size(0), T = u.size(1), Dn = u.size(2);
@@ -384,7 +395,9 @@ py::object selective_scan(Tensor u, Tensor dt, Tensor A, Tensor Bm, Tensor Cm, O
   const int64_t G = Bm.size(2), N = Bm.size(3);
   TORCH_CHECK(G > 0 && Dn % G == 0, "selective_scan: ", Dn, " channels do not divide into ", G, " groups");
   A = par32(what, "A", A, {Dn, N}, u);
-  Tensor D = par32(what, "D", opt(D_), {Dn}, u), bias = par32(what, "dt_bias", opt(bias_), {Dn}, u), h0 = par32(what, "h0", opt(h0_), {B, Dn, N}, u);
+  D = par32(what, "D", D, {Dn}, u);
+  bias = par32(what, "dt_bias", bias, {Dn}, u);
+  h0 = par32(what, "h0", h0, {B, Dn, N}, u);
   Tensor lengths = lengths_of(what, opt(lengths_), B, u);
   u = last_dense(u);
   dt = last_dense(dt);
@@ -411,7 +424,8 @@ py::object selective_scan(Tensor u, Tensor dt, Tensor A, Tensor Bm, Tensor Cm, O
 
 Tensor selective_scan_step(Tensor state, Tensor u, Tensor dt, Tensor A, Tensor Bm, Tensor Cm, OptT D_, OptT z_, OptT bias_, bool softplus) {
   const char* what = "selective_scan_step";
-  Tensor z = opt(z_);
+  Tensor z = opt(z_), D = opt(D_), bias = opt(bias_);
+  no_tangents(what, {&state, &u, &dt, &A, &Bm, &Cm, &D, &z, &bias});
   const int code = check(what, u, {&dt, &Bm, &Cm, &z});
   TORCH_CHECK(u.dim() == 2, "selective_scan_step: u must be (B, D)");
   const int64_t B = u.size(0), Dn = u.size(1);
@@ -423,7 +437,8 @@ Tensor selective_scan_step(Tensor state, Tensor u, Tensor dt, Tensor A, Tensor B
   const int64_t G = Bm.size(1), N = Bm.size(2);
   TORCH_CHECK(G > 0 && Dn % G == 0, "selective_scan_step: ", Dn, " channels do not divide into ", G, " groups");
   A = par32(what, "A", A, {Dn, N}, u);
-  Tensor D = par32(what, "D", opt(D_), {Dn}, u), bias = par32(what, "dt_bias", opt(bias_), {Dn}, u);
+  D = par32(what, "D", D, {Dn}, u);
+  bias = par32(what, "dt_bias", bias, {Dn}, u);
   TORCH_CHECK(state.scalar_type() == at::kFloat && state.sizes() == at::IntArrayRef({B, Dn, N}) && state.device() == u.device(),
               "selective_scan_step: state must be float32 (", B, ", ", Dn, ", ", N, ") on ", u.device());
   inference_only(what, {&state, &u, &dt, &A, &Bm, &Cm, &D, &z, &bias});
@@ -499,6 +514,7 @@ struct LinResFn : public torch::autograd::Function<LinResFn> {
 Tensor linear_residual(Tensor x, Tensor W, OptT b_, int64_t act, OptT res_) {
   const char* what = "linear_residual";
   Tensor b = opt(b_), res = opt(res_);
+  no_tangents(what, {&x, &W, &b, &res});
   check(what, x, {&W, &b, &res});
   TORCH_CHECK(x.dim() >= 1 && W.dim() == 2 && W.size(1) == x.size(-1) && W.size(0) >= 1 && W.size(1) >= 1, "linear_residual: weight ", W.sizes(),
               " does not match the input ", x.sizes());

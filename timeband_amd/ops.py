@@ -538,7 +538,8 @@ def linear_act(x2d, W, b, act=ACT_NONE, pre=None):
 # ----------------------------------------------------------------------------------------------
 # State space layer: causal convolution, selective scan, linear with residual.  fp32, bf16 or fp16 tensors (one type a call),
 # parameters of the scan fp32.  Checks, workspaces and autograd Functions are the extension's (csrc/ext_ssm.cpp), whatever
-# TB_EXT says: that variable chooses between two forms of the operators above, and these have one.
+# TB_EXT says: that variable chooses between two forms of the operators above, and these have one.  Dual tensors of
+# torch.autograd.forward_ad are refused.
 # ----------------------------------------------------------------------------------------------
 _SSM = None
 
