@@ -101,3 +101,80 @@ def test_linear_infinite_gradients_stay_in_their_rows():
 def test_forward_mode_is_refused():
     from test_ssm_edges_host import check_forward_mode_is_refused
     check_forward_mode_is_refused("cuda")
+
+
+# ---- scan: infinities ------------------------------------------------------------------------------------------------------------
+def scan_case(B, T, D, N, G=1, type=FP, seed=10, positive=False):
+    t = dict(u=rnd(seed, B, T, D, type=type), dt=rnd(seed + 1, B, T, D, type=type, scale=0.7),
+             A=-(torch.rand(D, N, generator=torch.Generator().manual_seed(seed)) * 2 + 0.05).cuda(),
+             Bm=rnd(seed + 2, B, T, G, N, type=type), Cm=rnd(seed + 3, B, T, G, N, type=type), D=rnd(seed + 4, D), bias=rnd(seed + 5, D) - 2,
+             z=rnd(seed + 6, B, T, D, type=type), h0=rnd(seed + 7, B, D, N))
+    if positive:
+        for k in ("Bm", "Cm", "D", "h0"):
+            t[k] = t[k].abs()
+    return t
+
+
+def call_scan(t, **k):
+    from timeband_amd import ops
+    return ops.selective_scan(t["u"], t["dt"], t["A"], t["Bm"], t["Cm"], D=t.get("D"), z=t.get("z"), dt_bias=t.get("bias"), h0=t.get("h0"), **k)
+
+
+def grads(t, out, hT, dout, dhT):
+    return dict(zip(["d" + (k[0] if k in ("Bm", "Cm") else k) for k in t], torch.autograd.grad((out, hT), list(t.values()), (dout, dhT))))
+
+
+def like(got, want, size, steps, what):
+    """Infinities and NaN where the 64-bit form has them, of the same sign; what is finite, and of finite parts, is near."""
+    g, w = got.detach().to("cpu", torch.float64), want
+    assert torch.equal(torch.isnan(g), torch.isnan(w)), (what, "NaN", int(torch.isnan(g).sum()), int(torch.isnan(w).sum()))
+    assert torch.equal(torch.where(torch.isinf(g), g, 0), torch.where(torch.isinf(w), w, 0)), (what, "infinities")
+    fine = torch.isfinite(w) & torch.isfinite(size)
+    near(got.detach().cpu()[fine], w[fine], size[fine], steps, what)
+
+
+def scan_like(t, dout, dhT, lengths=None, names=None, **k):
+    """A call forward and backward like the 64-bit form.  Counts of 32-bit roundings: 40 T for a decay over T steps, 64 + N for the
+    functions and the sum over states, D and B T for the sums over channels and steps."""
+    plain = {n: v.detach().clone() for n, v in t.items()}
+    req(*t.values())
+    out, hT = call_scan(t, lengths=lengths, return_state=True, **k)
+    got = dict(grads(t, out, hT, dout, dhT), out=out, hT=hT)
+    want = R.scan(**plain, lengths=lengths, dout=dout, dhT=dhT, **k)
+    size = R.scan(**plain, lengths=lengths, dout=dout, dhT=dhT, mag=True, **k)
+    B, T, D = t["u"].shape
+    for n in names or got:
+        like(got[n], want[n], size[n], 2 * (40 * T + 64 + t["A"].shape[1]) + D + B * T, n)
+
+
+@pytest.mark.parametrize("type", [FP, BF])
+@pytest.mark.parametrize("N", [1, 3, 6, 11, 16, 17, 33, 40])
+def test_scan_infinities_with_any_number_of_states(N, type):
+    """An infinite u, delta or dy: the infinities of the definition, also where N does not fill the lanes' states."""
+    B, T, D = 2, 64, 6
+    dhT = rnd(31, B, D, N)
+    for where in ("u", "dt", "dout"):
+        t, dout = scan_case(B, T, D, N, type=type, positive=True), rnd(30, B, T, D, type=type)
+        if where == "dout":
+            dout[0, 40, 1], dout[1, 9, 2] = INF, -INF
+        else:
+            t[where][0, 37, 1] = INF
+            t[where][1, 5, 2] = INF if where == "dt" else -INF
+        scan_like(t, dout, dhT)
+    t = scan_case(B, T, D, N, type=type, positive=True)
+    t["u"][0, 37, 1] = INF
+    t["z"] = None
+    y, h = call_scan(t, return_state=True)
+    assert (y[0, 37:, 1] == INF).all() and (h[0, 1] == INF).all()
+
+
+@pytest.mark.parametrize("N", [1, 3, 6, 11, 16, 17, 33])
+def test_scan_step_infinities_with_any_number_of_states(N):
+    from timeband_amd import ops
+    t = scan_case(3, 1, 10, N, positive=True)
+    t["u"][0, 0, 4], t["dt"][1, 0, 7] = INF, INF
+    want, state = R.scan(**t), t["h0"].clone()
+    out = ops.selective_scan_step(state, *(t[k][:, 0] if k != "A" else t[k] for k in ("u", "dt", "A", "Bm", "Cm")), D=t["D"], z=t["z"][:, 0], dt_bias=t["bias"])
+    size = R.scan(**t, mag=True)
+    like(out, want["out"][:, 0], size["out"][:, 0], 104 + N, "out")
+    like(state, want["hT"], size["hT"], 104, "state")

@@ -227,7 +227,9 @@ __device__ __forceinline__ void chain(const ScanArgs& a, int b, int chunk, long 
 }
 
 // forward.  STATE: only the chunk's end state from zero and its sum of delta (first pass over chunks).
-template <typename T, int S, bool STATE, bool VEC>
+// PART: N is not 4 S, and the states behind it are kept at 0: their products are 0 times what may be infinite.  Kernels of their own, so that
+// whole states take no selects (4 x 2048 x 2048 x 11 fp32: forward 144 us without them, 150 with; gradients too 491, 506).
+template <typename T, int S, bool STATE, bool VEC, bool PART>
 __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
   constexpr int TT = 32, EPT = 8, NP = 4 * S;
   __shared__ float sD[TT][CB][2];            // delta, delta u
@@ -319,6 +321,7 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
         for (int s = 0; s < S; ++s) {
           const float e = __builtin_amdgcn_exp2f(d * A2[s]);
           h[s] = fmaf(e, h[s], x * bv[s]);
+          if (PART) h[s] = n0 + s < a.N ? h[s] : 0.f;
           if (!STATE) y[j] = fmaf(h[s], cv[s], y[j]);
         }
         if (STATE) sum += d;
@@ -383,7 +386,7 @@ struct Row {
 };
 
 // backward.  STATE: only g in front of the chunk's first step from zero behind its last, and its sum of delta.
-template <typename T, int S, bool STATE, bool VEC>
+template <typename T, int S, bool STATE, bool VEC, bool PART>
 __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
   constexpr int TT = STATE ? 32 : Tile<S>::BWD, EPT = TT / 4, NP = 4 * S;
   // The next tile's rows are fetched before the walk, and this one's kept over it, where that spills no registers: 16 x 1024 x 2048
@@ -412,7 +415,7 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
   load_state<S>(a.A, rd, n0, a.N, ron, A2);
 #pragma unroll
   for (int s = 0; s < S; ++s) {
-    A2[s] *= LOG2E;
+    A2[s] = PART && n0 + s >= a.N ? -1.f : A2[s] * LOG2E;      // behind N: an infinite delta decays to 0 (0 times it is NaN)
     dA[s] = 0.f;
     g[s] = 0.f;
   }
@@ -494,6 +497,9 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
       else
 #pragma unroll
         for (int s = 0; s < S; ++s) h[0][s] = 0.f;
+      if constexpr (PART)
+#pragma unroll
+        for (int s = 0; s < S; ++s) h[0][s] = n0 + s < a.N ? h[0][s] : 0.f;
       // one step ahead of the arithmetic, and no further: left alone, the compiler keeps all of a tile's rows in registers
       Row<S> r;
       r.load(sD[0][rc], sG[0][rc], sB + n0, sC + n0);
@@ -510,6 +516,10 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
           const float e = __builtin_amdgcn_exp2f(c.d * A2[s]);
           if constexpr (KEEP) ea[k][s] = e;
           h[k + 1][s] = fmaf(e, h[k][s], c.x * c.b[s]);
+          if constexpr (PART) {
+            h[k + 1][s] = n0 + s < a.N ? h[k + 1][s] : 0.f;
+            asm volatile("" : "+v"(h[k + 1][s]));          // one value: left alone, the one before the select is kept beside it
+          }
           y = fmaf(h[k + 1][s], c.c[s], y);
         }
         asm volatile("" : "+v"(y));
@@ -526,12 +536,14 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           g[s] = fmaf(c.c[s], c.y, g[s]);
+          if constexpr (PART) g[s] = n0 + s < a.N ? g[s] : 0.f;
           v[s] = g[s] * c.x;                       // dB
           v[S + s] = h[k + 1][s] * c.y;            // dC
           gB = fmaf(g[s], c.b[s], gB);
           if constexpr (KEEP) g[s] *= ea[k][s];
           else g[s] *= __builtin_amdgcn_exp2f(c.d * A2[s]);
-          const float q = g[s] * h[k][s];
+          float q = g[s] * h[k][s];          // behind N 0: neither factor is infinite there
+          if constexpr (PART && S == 16) q = n0 + s < a.N ? q : 0.f;      // for the registers alone (4 x 2048 x 1024 x 40 bf16 1331 us, without 1500)
           gA = fmaf(q, A2[s], gA);                 // of A log2 e: divided out of the sum
           dA[s] = fmaf(q, c.d, dA[s]);
           asm volatile("" : "+v"(g[s]), "+v"(dA[s]));      // here and now: put off, their operands stay in registers
@@ -731,6 +743,7 @@ __global__ void __launch_bounds__(256) scan_step(StepArgs a) {
 #pragma unroll
   for (int s = 0; s < S; ++s) {
     h[s] = fmaf(__builtin_amdgcn_exp2f(dl * (A[s] * LOG2E)), h[s], dl * u * bv[s]);
+    h[s] = n0 + s < a.N ? h[s] : 0.f;          // behind N: 0 times what may be infinite
     y = fmaf(h[s], cv[s], y);
   }
   y = quad_sum(y);
@@ -775,12 +788,15 @@ struct FwdLaunch {
   hipStream_t s;
   template <typename T, int S>
   int operator()() {
-    return a.vec ? run<T, S, true>() : run<T, S, false>();
+    // accesses off their alignment serve aligned rows too, but cost time (4 x 2048 x 2048 x 11 fp32 forward 162 us, aligned ones 150);
+    // not for 33 to 64 states, whose backward pass they take more registers from
+    if (a.N < 4 * S) return a.vec && S < 16 ? run<T, S, S < 16, true>() : run<T, S, false, true>();
+    return a.vec ? run<T, S, true, false>() : run<T, S, false, false>();
   }
-  template <typename T, int S, bool VEC>
+  template <typename T, int S, bool VEC, bool PART>
   int run() {
-    if (a.chunks > 1) scan_fwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
-    scan_fwd<T, S, false, VEC><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
+    if (a.chunks > 1) scan_fwd<T, S, true, VEC, false><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
+    scan_fwd<T, S, false, VEC, PART><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
     return 0;
   }
 };
@@ -792,12 +808,13 @@ struct BwdLaunch {
   hipStream_t s;
   template <typename T, int S>
   int operator()() {
-    return a.vec ? run<T, S, true>() : run<T, S, false>();
+    if (a.N < 4 * S) return a.vec && S < 16 ? run<T, S, S < 16, true>() : run<T, S, false, true>();
+    return a.vec ? run<T, S, true, false>() : run<T, S, false, false>();
   }
-  template <typename T, int S, bool VEC>
+  template <typename T, int S, bool VEC, bool PART>
   int run() {
-    if (a.chunks > 1) scan_bwd<T, S, true, VEC><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
-    scan_bwd<T, S, false, VEC><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
+    if (a.chunks > 1) scan_bwd<T, S, true, VEC, false><<<(unsigned)(blocks * (a.chunks - 1)), 256, 0, s>>>(a);
+    scan_bwd<T, S, false, VEC, PART><<<(unsigned)(blocks * a.chunks), 256, 0, s>>>(a);
     FinishArgs f{a.par, a.bc, dA, dD, dbias, dB, dC, a.B * a.chunks, a.B, a.T, a.D, a.N, a.G, 4 * S, a.cblk, 0};
     f.first = dA || dD || dbias ? (unsigned)finish_blocks_par(a, S) : 0;
     const unsigned rest = dB || dC ? (unsigned)finish_blocks_bc(a, S) : 0;
