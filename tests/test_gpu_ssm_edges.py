@@ -178,3 +178,22 @@ def test_scan_step_infinities_with_any_number_of_states(N):
     size = R.scan(**t, mag=True)
     like(out, want["out"][:, 0], size["out"][:, 0], 104 + N, "out")
     like(state, want["hT"], size["hT"], 104, "state")
+
+
+@pytest.mark.parametrize("N", [4, 11])
+def test_scan_infinities_without_the_skip_term(N):
+    """No D: neither u nor dy is multiplied by a 0 in its place, and with positive B and C an infinite u gives infinite outputs, an
+    infinite dy infinite du, not NaN."""
+    B, T, D = 1, 40, 5
+    t = scan_case(B, T, D, N, positive=True)
+    del t["D"]
+    t["u"][0, 20, 1] = INF
+    t["z"] = t["z"].abs() + 0.1
+    req(*t.values())
+    out, hT = call_scan(t, return_state=True)
+    dout = rnd(30, B, T, D)
+    clean = torch.autograd.grad(out, t["u"], dout, retain_graph=True)[0]
+    assert (out[0, 20:, 1] == INF).all() and torch.isfinite(out[0, :20]).all() and torch.isfinite(out[0, :, [0, 2, 3, 4]]).all()
+    du, dz = torch.autograd.grad(out, (t["u"], t["z"]), dout.index_put((torch.tensor(0), torch.tensor(30), torch.tensor(2)), torch.tensor(INF, device="cuda")))
+    assert (du[0, :31, 2] == INF).all() and torch.equal(du[0, 31:, 2], clean[0, 31:, 2]) and torch.equal(du[..., [0, 1, 3, 4]], clean[..., [0, 1, 3, 4]])
+    assert torch.equal(dz[0, 20:, 1], INF * torch.sign(dout[0, 20:, 1]))

@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
       float o[EPT];
 #pragma unroll
       for (int i = 0; i < EPT; ++i) {
-        float y = fmaf(Dp[i], u[i], sY[ct][cc + i]);
+        float y = a.Dp ? fmaf(Dp[i], u[i], sY[ct][cc + i]) : sY[ct][cc + i];      // no skip term: not 0 times u
         if (a.z) y *= tb_silu(z[i]);
         o[i] = on ? y : 0.f;
       }
@@ -600,7 +600,7 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
           const float dy = sG[ct][cc + i];
-          o[i] = on ? fmaf(sD[ct][cc + i][0], sGB[ct][cc + i], sPar[1][cc + i] * dy) : 0.f;
+          o[i] = on ? fmaf(sD[ct][cc + i][0], sGB[ct][cc + i], a.Dp ? sPar[1][cc + i] * dy : 0.f) : 0.f;
           dD[i] = fmaf(dy, u[i], dD[i]);
         }
         if (a.du) put<T, EPT, VEC>(a.du, oo + (long)t * a.D, ch, a.Dg, o);
@@ -609,7 +609,7 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
           rz.mask(on, ch, a.Dg, 0.f);
 #pragma unroll
           for (int i = 0; i < EPT; ++i) {
-            const float z = rz.get(i), q = tb_sig(z), y = fmaf(sPar[1][cc + i], u[i], sY[ct][cc + i]);
+            const float z = rz.get(i), q = tb_sig(z), y = a.Dp ? fmaf(sPar[1][cc + i], u[i], sY[ct][cc + i]) : sY[ct][cc + i];
             o[i] = on ? ro.get(i) * y * (q * (1.f + z * (1.f - q))) : 0.f;
           }
           put<T, EPT, VEC>(a.dz, oo + (long)t * a.D, ch, a.Dg, o);
