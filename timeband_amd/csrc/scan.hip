@@ -297,6 +297,7 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
       else d = on ? d : 0.f;
       sD[ct][cc + i][0] = d;
       sD[ct][cc + i][1] = d * u[i];
+      if (!STATE) u[i] = a.Dp ? u[i] : 0.f;      // no skip term: 0 times u is none where u is infinite
     }
     rB.store(sB, t0, tv, a.N);
     if (!STATE) rC.store(sC, t0, tv, a.N);
@@ -333,7 +334,7 @@ __global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
       float o[EPT];
 #pragma unroll
       for (int i = 0; i < EPT; ++i) {
-        float y = a.Dp ? fmaf(Dp[i], u[i], sY[ct][cc + i]) : sY[ct][cc + i];      // no skip term: not 0 times u
+        float y = fmaf(Dp[i], u[i], sY[ct][cc + i]);
         if (a.z) y *= tb_silu(z[i]);
         o[i] = on ? y : 0.f;
       }
