@@ -197,3 +197,27 @@ def test_scan_infinities_without_the_skip_term(N):
     du, dz = torch.autograd.grad(out, (t["u"], t["z"]), dout.index_put((torch.tensor(0), torch.tensor(30), torch.tensor(2)), torch.tensor(INF, device="cuda")))
     assert (du[0, :31, 2] == INF).all() and torch.equal(du[0, 31:, 2], clean[0, 31:, 2]) and torch.equal(du[..., [0, 1, 3, 4]], clean[..., [0, 1, 3, 4]])
     assert torch.equal(dz[0, 20:, 1], INF * torch.sign(dout[0, 20:, 1]))
+
+
+@pytest.mark.parametrize("type", [FP, BF])
+@pytest.mark.parametrize("N,T,lengths", [(4, 50, None), (16, 40, [40, 33]), (11, 300, [258, 300]), (40, 9, [1, 9]), (16, 70, [0, 70])])
+def test_scan_infinite_last_state_leaves_dA_alone(N, T, lengths, type):
+    """An infinite u at a sequence's last step makes its end state infinite.  dA has no part of that state, and the steps that fill the
+    walk's last tile, or lie behind `lengths`, must not add 0 times it."""
+    B, D = 2, 6
+    t, dout, dhT = scan_case(B, T, D, N, type=type, positive=True), rnd(30, B, T, D, type=type), rnd(31, B, D, N)
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    ends = lengths or [T] * B
+    for b, n in enumerate(ends):
+        if n:
+            t["u"][b, n - 1, 1 + b] = INF
+        else:
+            t["h0"][b, 3, :] = INF
+    scan_like(t, dout, dhT, lengths=ln)
+    t = scan_case(B, T, D, N, type=type, positive=True)
+    for b, n in enumerate(ends):
+        if n:
+            t["u"][b, n - 1, 1 + b] = INF
+    req(*t.values())
+    out, hT = call_scan(t, lengths=ln, return_state=True)
+    assert torch.isfinite(torch.autograd.grad(out, t["A"], dout)[0]).all()

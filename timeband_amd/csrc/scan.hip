@@ -492,6 +492,7 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
       }
     } else {
       constexpr bool KEEP = S <= 4;      // each step's decay, too, where registers allow
+      const int last = tv - 1 - t0;
       float ea[KEEP ? TT : 1][S];
       float h[TT + 1][S];      // h[k]: the state in front of step k
       if (ron) load_row<S>(a.ck + (((long)w.b * a.cktiles + t0 / TT) * a.D + rd) * NP + n0, h[0]);
@@ -534,6 +535,14 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
         __builtin_amdgcn_sched_barrier(0);
         if (k > 0) r.load(sD[k - 1][rc], sG[k - 1][rc], sB + (k - 1) * NP + n0, sC + (k - 1) * NP + n0);
         float v[2 * S], gB = 0.f, gA = 0.f;
+        // the sequence's last step: what the steps behind it added is 0 times the state that they kept, NaN where that is infinite
+        if (__builtin_expect(k == last, 0)) {
+#pragma unroll
+          for (int s = 0; s < S; ++s) {
+            dA[s] = 0.f;
+            asm volatile("" : "+v"(dA[s]));          // a branch, not a select a step
+          }
+        }
 #pragma unroll
         for (int s = 0; s < S; ++s) {
           g[s] = fmaf(c.c[s], c.y, g[s]);
@@ -627,7 +636,7 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
   }
   if (ron) {
 #pragma unroll
-    for (int s = 0; s < S; ++s) a.par[row * (NP + 2) + n0 + s] = dA[s];
+    for (int s = 0; s < S; ++s) a.par[row * (NP + 2) + n0 + s] = tv > ts ? dA[s] : 0.f;
   }
   if (a.dh0 && w.chunk == 0) store_state<S>(a.dh0, (long)w.b * a.D + rd, n0, a.N, ron, g);
   // dD and dbias: over the block's steps, in their order
