@@ -221,3 +221,31 @@ def test_scan_infinite_last_state_leaves_dA_alone(N, T, lengths, type):
     req(*t.values())
     out, hT = call_scan(t, lengths=ln, return_state=True)
     assert torch.isfinite(torch.autograd.grad(out, t["A"], dout)[0]).all()
+
+
+@pytest.mark.parametrize("N", [4, 11, 16])
+def test_scan_states_past_the_range_of_a_chunk_s_decay(N):
+    """Walks that are cut: states that grow by more than fp32's range over a chunk but start small enough, or at 0; and an infinite
+    state that decays by more than its range.  Step by step none of them leaves the range (or infinity)."""
+    B, D = 1, 4
+    big = 3.4e38
+    for T, step, A0, h0 in ((36, 2.9, 1.0, 1e-30), (300, 2.9, 1.0, 0.0), (36, 2.9, 1.0, -1e-32), (300, 3.0, -1.0, INF), (300, 0.01, -1.0, INF)):
+        t = dict(u=torch.zeros(B, T, D, device="cuda"), dt=torch.full((B, T, D), step, device="cuda"), A=torch.full((D, N), A0, device="cuda"),
+                 Bm=rnd(1, B, T, 1, N).abs(), Cm=rnd(2, B, T, 1, N).abs() + 0.1, h0=torch.full((B, D, N), h0, device="cuda"))
+        out, hT = call_scan(t, softplus=False, return_state=True)
+        want = R.scan(**t, softplus=False)
+        assert h0 == INF or (float(want["hT"].abs().max()) < big and float(want["out"].abs().max()) < big)
+        n = 40 * T + 64 + N
+        like(out, want["out"], want["out"].abs(), n, "out")
+        like(hT, want["hT"], want["hT"].abs(), n, "hT")
+        # backward: the state's gradient runs the same way from the end
+        t = {k: v.detach().clone() for k, v in t.items()}
+        t["u"] = rnd(3, B, T, D) * 1e-30
+        t["h0"] = torch.zeros_like(t["h0"])
+        dhT = torch.full((B, D, N), h0, device="cuda")
+        plain = {k: v.clone() for k, v in t.items()}
+        req(*t.values())
+        out, hT = call_scan(t, softplus=False, return_state=True)
+        dh0, = torch.autograd.grad((out, hT), t["h0"], (torch.zeros_like(out), dhT))
+        want = R.scan(**plain, softplus=False, dout=torch.zeros(B, T, D), dhT=dhT)["dh0"]
+        like(dh0, want, want.abs(), 2 * n, "dh0")

@@ -205,10 +205,15 @@ __device__ __forceinline__ float quad_sum4(const float (&y)[4], int lane) {
 
 // The state that a chunk starts from: the chunks before it (REV: behind it), each with its own end state from zero and the sum of
 // its delta, chained from the first (REV: last) one on.  Eight are fetched together: only the products wait for each other.
+// A chunk's decay can pass fp32's range where no step's does (a state that grows, or decays from infinity): what does not come out finite
+// is chained again with the decay in two factors, and with 0 and infinity kept, as the steps would keep them.
 template <int S, bool REV>
 __device__ __forceinline__ void chain(const ScanArgs& a, int b, int chunk, long rd, int n0, const float (&A2)[S], float (&h)[S]) {
   constexpr int NP = 4 * S;
   const int count = REV ? a.chunks - 1 - chunk : chunk;
+  float first[S];
+#pragma unroll
+  for (int s = 0; s < S; ++s) first[s] = h[s];
   for (int i = 0; i < count; i += 8) {
     float own[8][S], sum[8];
 #pragma unroll
@@ -224,13 +229,31 @@ __device__ __forceinline__ void chain(const ScanArgs& a, int b, int chunk, long 
 #pragma unroll
         for (int s = 0; s < S; ++s) h[s] = fmaf(__builtin_amdgcn_exp2f(A2[s] * sum[j]), h[s], own[j][s]);
   }
+  bool fine = true;
+#pragma unroll
+  for (int s = 0; s < S; ++s) fine = fine && fabsf(h[s]) < INFINITY;
+  if (__builtin_expect(fine, 1)) return;
+#pragma unroll
+  for (int s = 0; s < S; ++s) h[s] = first[s];
+  for (int k = 0; k < count; ++k) {
+    float own[S];
+    const long row = ((long)b * a.chunks + (REV ? a.chunks - 1 - k : k)) * a.D + rd;
+    load_row<S>(a.cstate + row * NP + n0, own);
+    const float sum = a.csum[row];
+#pragma unroll
+    for (int s = 0; s < S; ++s) {
+      const float x = A2[s] * sum, e = __builtin_amdgcn_exp2f(x * 0.5f);
+      const bool kept = (h[s] == 0.f || fabsf(h[s]) == INFINITY) && fabsf(x) < INFINITY;
+      h[s] = (kept ? h[s] : h[s] * e * e) + own[s];
+    }
+  }
 }
 
 // forward.  STATE: only the chunk's end state from zero and its sum of delta (first pass over chunks).
 // PART: N is not 4 S, and the states behind it are kept at 0: their products are 0 times what may be infinite.  Kernels of their own, so that
 // whole states take no selects (4 x 2048 x 2048 x 11 fp32: forward 144 us without them, 150 with; gradients too 491, 506).
 template <typename T, int S, bool STATE, bool VEC, bool PART>
-__global__ void __launch_bounds__(256) scan_fwd(ScanArgs a) {
+__global__ void __launch_bounds__(256, VEC && S <= 4 ? 4 : 1) scan_fwd(ScanArgs a) {      // four waves a SIMD (4 x 2048 x 2048 x 16 fp32 145 us, three 158)
   constexpr int TT = 32, EPT = 8, NP = 4 * S;
   __shared__ float sD[TT][CB][2];            // delta, delta u
   __shared__ float sB[TT * NP], sC[STATE ? 1 : TT * NP];
