@@ -249,3 +249,24 @@ def test_scan_states_past_the_range_of_a_chunk_s_decay(N):
         dh0, = torch.autograd.grad((out, hT), t["h0"], (torch.zeros_like(out), dhT))
         want = R.scan(**plain, softplus=False, dout=torch.zeros(B, T, D), dhT=dhT)["dh0"]
         like(dh0, want, want.abs(), 2 * n, "dh0")
+
+
+# ---- convolution -----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("type", [FP, BF])
+@pytest.mark.parametrize("T,lengths,at", [(40, None, 6), (40, None, 39), (23, [23, 17], 16), (5, [4, 5], 3)])
+def test_conv_infinite_x_in_dw(T, lengths, at, type):
+    """An infinite x makes the taps' gradients infinite, by the signs of dy, not NaN: steps that do not count, or that belong to
+    another run of steps, must not add 0 times it."""
+    from timeband_amd import ops
+    B, D, K = 2, 16, 4
+    x, w, dy = rnd(1, B, T, D, type=type), rnd(2, D, K, type=type), rnd(3, B, T, D, type=type).abs() + 0.1
+    x[:, at, 3], x[:, at, 5] = INF, -INF
+    ln = None if lengths is None else torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    req(x, w)
+    y = ops.causal_conv(x, w, None, ops.ACT_NONE, lengths=ln)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    want, size = R.conv(x, w, None, 0, lengths=ln, dy=dy), R.conv(x, w, None, 0, lengths=ln, dy=dy, mag=True)
+    assert torch.isinf(want[3]).any()
+    like(y, want[0], size[0], K + 32, "y")
+    like(dx, want[2], size[2], K + 48, "dx")
+    like(dw, want[3], size[3], B * T + 48, "dw")

@@ -197,7 +197,7 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < GRP; ++j) {
-        const bool own = s + j < t1;          // the run's own steps: their share of dw and db
+        const bool own = s + j < t1 && s + j < len;      // the run's own steps, of those that count: their share of dw and db
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
           float d = g[j][i];
@@ -210,10 +210,14 @@ __global__ void __launch_bounds__(256) conv_bwd(ConvArgs a) {
             d = s + j < len ? d : 0.f;
           }
           dp[K - 1 + j][i] = d;
-          const float m = own ? d : 0.f;
+        }
+        if (own) {                            // not 0 times the x of steps before, which may be infinite
 #pragma unroll
-          for (int k = 0; k < K; ++k) dw[k][i] = fmaf(m, win[j + k][i], dw[k][i]);
-          dw[K][i] += m;
+          for (int i = 0; i < VEC; ++i) {
+#pragma unroll
+            for (int k = 0; k < K; ++k) dw[k][i] = fmaf(dp[K - 1 + j][i], win[j + k][i], dw[k][i]);
+            dw[K][i] += dp[K - 1 + j][i];
+          }
         }
         const int t = s + j - (K - 1);        // dx[t] needs dpre[t .. t+K-1] = dp[j .. j+K-1]
         if (t >= t0 && t < t1) {
