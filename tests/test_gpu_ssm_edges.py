@@ -145,6 +145,7 @@ def scan_like(t, dout, dhT, lengths=None, names=None, **k):
     B, T, D = t["u"].shape
     for n in names or got:
         like(got[n], want[n], size[n], 2 * (40 * T + 64 + t["A"].shape[1]) + D + B * T, n)
+    return got, want
 
 
 @pytest.mark.parametrize("type", [FP, BF])
@@ -270,3 +271,112 @@ def test_conv_infinite_x_in_dw(T, lengths, at, type):
     like(y, want[0], size[0], K + 32, "y")
     like(dx, want[2], size[2], K + 48, "dx")
     like(dw, want[3], size[3], B * T + 48, "dw")
+
+
+@pytest.mark.parametrize("type", [FP, BF])
+@pytest.mark.parametrize("B,T,D,K,run", [(6, 4100, 512, 4, 12), (2, 9001, 2063, 3, 32), (4, 8200, 2064, 4, 64)])
+def test_conv_in_long_runs(B, T, D, K, run, type):
+    """Enough steps and channels for runs of more than eight steps, which do not divide T: some channels against the formula."""
+    from timeband_amd import ops
+    assert T % run and min(64, (B * T * ((D + 3) // 4)) >> 18) // 4 * 4 == run
+    g = torch.Generator(device="cuda").manual_seed(1)
+    x, dy = (torch.randn(B, T, D, device="cuda", generator=g).to(type) for _ in range(2))
+    w, b = rnd(2, D, K, type=type, scale=0.5), rnd(3, D, type=type, scale=0.3)
+    ln = torch.tensor([T, T - run - 1, 5, T - 1][:B], dtype=torch.int32, device="cuda")
+    if B > 4:
+        ln = torch.tensor([T, T - run - 1, 5, T - 1, 0, T // 2], dtype=torch.int32, device="cuda")
+    req(x, w, b)
+    y = ops.causal_conv(x, w, b, ops.ACT_SILU, lengths=ln)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    c = [0, 1, 3, 4, 7, D // 2, D - 5, D - 4, D - 1]
+    part = [v.detach()[..., c] for v in (x, dy)] + [w.detach()[c], b.detach()[c]]
+    want, size = (R.conv(part[0], part[2], part[3], 4, None, ln, part[1], mag=m) for m in (False, True))
+    # |pre| < 8 puts K + 32 roundings on y and K + 48 on dx, as for short ones; a thread sums its run, a block 4 to 64 runs, and
+    # sixteen threads the blocks: fewer than B T additions in a row
+    near(y[..., c], want[0], size[0], K + 32, "y")
+    near(dx[..., c], want[2], size[2], K + 48, "dx")
+    near(dw[c], want[3], size[3], B * T + 48, "dw")
+    near(db[c], want[4], size[4], B * T + 48, "db")
+
+
+# ---- scan: walks of many tiles ---------------------------------------------------------------------------------------------------
+LONG = [  # B, T, G, channels a group, N, lengths: by the number of channel blocks B G the steps are cut into
+    (32, 70, 12, 2, 16, False),      # 384 blocks: one walk of several tiles
+    (32, 200, 12, 8, 4, True),       # the same, aligned, states of 32 steps a tile
+    (32, 333, 12, 1, 32, False),     # tiles of eight steps
+    (33, 130, 12, 2, 64, True),
+    (10, 300, 8, 3, 16, True),       # 80 blocks: chunks of 128 steps, the last of 44
+    (10, 300, 8, 8, 11, False),
+    (16, 1000, 10, 2, 8, True),      # 160 blocks: six chunks of 192 and less
+    (16, 1000, 10, 1, 16, False),
+    (12, 385, 8, 70, 16, False),     # two channel blocks a group, the second of six channels
+]
+
+
+@pytest.mark.parametrize("type", [FP, BF, HF])
+@pytest.mark.parametrize("B,T,G,C,N,ragged", LONG)
+def test_scan_gradients_over_many_tiles(B, T, G, C, N, ragged, type):
+    t, dout, dhT = scan_case(B, T, G * C, N, G=G, type=type), rnd(30, B, T, G * C, type=type), rnd(31, B, G * C, N)
+    ln = None
+    if ragged:
+        ln = torch.randint(0, T + 1, (B,), generator=torch.Generator().manual_seed(3), dtype=torch.int32)
+        ln[0], ln[1], ln[2] = T, 0, 129
+        ln = ln.cuda()
+    got, want = scan_like(t, dout, dhT, lengths=ln)
+    if type != FP:      # the counts allow 40 T roundings of sums that mostly decay; their norm is far below the type's own step
+        for k in ("out", "du", "ddt", "dz", "dB", "dC"):
+            if want[k].numel() >= 25000:
+                rounded_once(got[k], want[k], k)
+
+
+# ---- linear: every branch of the backward pass ---------------------------------------------------------------------------------
+def linear_like(M, K, N, kind, type, need="xWbr", seed=1):
+    from timeband_amd import ops
+    x, W, b, res = rnd(seed, M, K, type=type), rnd(seed + 1, N, K, type=type, scale=K ** -0.5), rnd(seed + 2, N, type=type), rnd(seed + 3, M, N, type=type)
+    dy = rnd(seed + 4, M, N, type=type)
+    if kind == 3:                      # where z is within its rounding errors of 0, dy is 0: relu's derivative does not count there
+        z, size = R.linear(x, W, b, 0), R.linear(x, W, b, 0, mag=True)
+        close = z.abs() <= (K + 4) * R.U * size
+        assert close.float().mean() < 0.01
+        dy[close.cuda()] = 0
+    leaves = dict(zip("xWbr", (x, W, b, res)))
+    req(*(leaves[k] for k in need))
+    y = ops.linear_residual(x, W, b, kind, residual=res)
+    got = dict(zip(need, torch.autograd.grad(y, [leaves[k] for k in need], dy)))
+    want, size = R.linear(x, W, b, kind, res, dy), R.linear(x, W, b, kind, res, dy, mag=True)
+    near(y, want[0], size[0], K + 64, "y")
+    # dz in two parts of 16 bits: within 2^-16 (bf16) of itself, 2^8 roundings of 32 bits, and twice the sums
+    two = 0 if type == FP or kind in (0, 3) else 256
+    for k, steps, name in (("x", 2 * N + K, "dx"), ("W", 2 * M + K, "dW"), ("b", M + K, "db")):
+        if k in need:
+            near(got[k], want["xWb".index(k) + 1], size["xWb".index(k) + 1], steps + 64 + two, name)
+    if "r" in need:
+        assert torch.equal(got["r"], dy)
+
+
+@pytest.mark.parametrize("type", [FP, BF, HF])
+@pytest.mark.parametrize("M,K,N", [(2049, 24, 132), (129, 72, 127), (33, 16, 16), (7, 40, 30), (300, 88, 1100)])
+def test_linear_relu_gradients(M, K, N, type):
+    linear_like(M, K, N, 3, type)
+
+
+@pytest.mark.parametrize("type", [FP, BF, HF])
+@pytest.mark.parametrize("kind", [0, 4])
+@pytest.mark.parametrize("M,K,N", [
+    (65500, 200, 40),        # dx in 256 x 256 tiles, dW in a launch of its own (fp32: from x as it lies)
+    (65500, 201, 36),        # the same with rows off 16 bytes
+    (100, 4099, 4000),       # dW in 256 x 256 tiles
+    (100, 72, 2056),         # dx split over k
+    (100, 72, 2051),
+    (5000, 72, 90),          # dW split over k
+])
+def test_linear_backward_branches(M, K, N, kind, type):
+    linear_like(M, K, N, kind, type)
+
+
+@pytest.mark.parametrize("type", [FP, BF, HF])
+@pytest.mark.parametrize("kind", [0, 5])
+@pytest.mark.parametrize("need", ["x", "W", "b", "r", "xb", "Wb", "xr", "xW"])
+def test_linear_some_gradients(need, kind, type):
+    for M, K, N in ((150, 72, 136), (150, 75, 131), (20, 72, 1100)):
+        linear_like(M, K, N, kind, type, need)
