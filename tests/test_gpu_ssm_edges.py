@@ -380,3 +380,20 @@ def test_linear_backward_branches(M, K, N, kind, type):
 def test_linear_some_gradients(need, kind, type):
     for M, K, N in ((150, 72, 136), (150, 75, 131), (20, 72, 1100)):
         linear_like(M, K, N, kind, type, need)
+
+
+def test_linear_activations_to_their_stated_precision():
+    """One input and a weight of 1: z is x itself.  fp32, relative: tanh 2^-20, sigmoid and SiLU |z| + 4 roundings (the exponent's, the
+    exponential's, the sum's and the reciprocal's), GELU 2^-20 + 2.5 z^2 2^-24 below 0 and 2^-20 above."""
+    from timeband_amd import ops
+    one = torch.ones(1, 1, device="cuda")
+    for lo, hi in ((1e-6, 0.3), (0.3, 3), (3, 13)):
+        for sign in (1, -1):
+            z = (torch.linspace(lo, hi, 500009) * sign).cuda()[:, None]
+            z64 = z.double().cpu()
+            allowed = {1: 2.0 ** -20 + 0 * z64, 2: (z64.abs() + 4) * 2 * R.U, 4: (z64.abs() + 5) * 2 * R.U,
+                       5: 2.0 ** -20 + 2.5 * R.U * z64.clamp(max=0) ** 2}
+            for kind, tol in allowed.items():
+                got, want = ops.linear_residual(z, one, None, kind).double().cpu(), R.act(z64, kind)[0]
+                off = ((got - want) / want).abs() / tol
+                assert float(off.max()) <= 1, (kind, float(z[int(off.argmax())]), float(off.max()))
