@@ -32,3 +32,14 @@ def check_forward_mode_is_refused(device):
 def test_forward_mode_is_refused():
     """Without the refusal the result has no tangent, and x + f(x) would have that of x alone."""
     check_forward_mode_is_refused("cpu")
+
+
+def test_linear_refuses_more_tiles_than_a_launch():
+    """Tiles of a product that one launch cannot hold (their count would wrap): refused (3) before anything is launched."""
+    from timeband_amd import _lib
+    lib = _lib.load()
+    p, wide = 4096, 1 << 62
+    lin = lambda M, K, N: lib.tb_linres_fwd(p, K, p, K, 0, 0, 0, p, 0, M, K, N, 0, 1, p, wide, 0)
+    back = lambda M, K, N: lib.tb_linres_bwd(p, N, p, K, p, K, 0, 0, p, p, p, M, K, N, 1, p, wide, 0)
+    assert lin(10 ** 9, 8, 4 * 10 ** 6) == 3 and back(10 ** 9, 8, 4 * 10 ** 6) == 3 and back(10 ** 9, 4 * 10 ** 6, 8) == 3
+    assert back(100, 4 * 10 ** 6, 4 * 10 ** 6) == 3

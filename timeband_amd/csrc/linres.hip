@@ -1046,8 +1046,10 @@ int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, 
 
 int check_common(const char* what, long M, int K, int N, int act, int dtype) {
   if (M < 0 || K < 1 || N < 1) return tb_set_error(TB_ERR_ARG, "%s: bad sizes M=%ld K=%d N=%d", what, M, K, N);
-  // The transposes' grids are 16 bits wide across; a block of them takes 64 rows, and DOWN puts columns that are not there 2^30 rows away.
-  if (K > 4000000 || N > 4000000 || M > 1000000000L)
+  // Rows below 2^30, because DOWN puts columns that are not there 2^30 rows away; columns and k are 32-bit indexes up to a tile behind their
+  // last one, which 4 million leave room for; and the tiles of each product are one launch.
+  auto tiles = [](long a, long b) { return ((a + 127) / 128) * ((b + 127) / 128); };
+  if (K > 4000000 || N > 4000000 || M > 1000000000L || !tb_grid_ok(tiles(M, N), 256) || !tb_grid_ok(tiles(M, K), 256) || !tb_grid_ok(tiles(N, K), 256))
     return tb_set_error(TB_ERR_UNSUPPORTED, "%s: M=%ld K=%d N=%d are too many in one call", what, M, K, N);
   if (act < 0 || act > TB_ACT_LAST) return tb_set_error(TB_ERR_UNSUPPORTED, "%s: activation %d is not supported", what, act);
   if (!tb_dtype_ok(dtype)) return tb_set_error(TB_ERR_ARG, "%s: bad element type %d", what, dtype);
