@@ -176,8 +176,13 @@ int tb_scan_step(float* state, long state_batch_stride, const void* u, const voi
 /* Linear with bias, activation and residual: y[M,N] = act(x[M,K].W[N,K]^T + b[N]) + residual[M,N]  (tb_linear_act_fwd beside it
  * is fp32 through split bf16 products, without residual).  b, residual nullable.  z (M,N) fp32 nullable: the pre-activation,
  * which the backward pass needs when act != 0.  M up to 10^9, N and K up to 4 * 10^6.  backward: dz = dy act'(z), dx = dz.W,
- * dW = dz^T.x, db = colsum(dz), each nullable and dense; the residual's gradient is dy itself. */
+ * dW = dz^T.x, db = colsum(dz), each nullable and dense; the residual's gradient is dy itself.
+ * Workspaces: tb_linres_workspace_bytes is enough for any operands of these sizes; the other two are what a call with these pointers,
+ * strides and wishes needs (operands on 16 bytes are read in place, only what is wanted is laid out), and what it checks. */
 size_t tb_linres_workspace_bytes(long M, int K, int N, int dtype, int backward);
+size_t tb_linres_fwd_workspace_bytes(const void* x, long x_row_stride, const void* W, long w_row_stride, long M, int K, int N, int dtype);
+size_t tb_linres_bwd_workspace_bytes(const void* dy, long dy_row_stride, const void* x, long x_row_stride, int act, int want_dx, int want_dW,
+                                     int want_db, long M, int K, int N, int dtype);
 int tb_linres_fwd(const void* x, long x_row_stride, const void* W, long w_row_stride, const void* b, const void* residual,
                   long residual_row_stride, void* y, float* z, long M, int K, int N, int act, int dtype, void* ws, size_t ws_bytes,
                   void* stream);

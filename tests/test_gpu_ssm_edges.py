@@ -397,3 +397,26 @@ def test_linear_activations_to_their_stated_precision():
                 got, want = ops.linear_residual(z, one, None, kind).double().cpu(), R.act(z64, kind)[0]
                 off = ((got - want) / want).abs() / tol
                 assert float(off.max()) <= 1, (kind, float(z[int(off.argmax())]), float(off.max()))
+
+
+def test_linear_takes_the_memory_that_it_uses():
+    """Aligned operands are read in place: a call's peak is its outputs and what it lays out."""
+    from timeband_amd import ops
+    MB = 1 << 20
+
+    def peak(f):
+        f()
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        torch.cuda.reset_peak_memory_stats()
+        r = f()
+        torch.cuda.synchronize()
+        return torch.cuda.max_memory_allocated() - before
+
+    x, W = rnd(1, 8192, 1024, type=BF), rnd(2, 2048, 1024, type=BF)
+    assert peak(lambda: ops.linear_residual(x, W)) <= 32 * MB + MB
+    x, W, dy = rnd(1, 32768, 256), rnd(2, 256, 256), rnd(3, 32768, 256)
+    req(x, W)
+    y = ops.linear_residual(x, W)
+    # dx (32 MB), dW, W across, dW's split sums (up to 64 of 1/4 MB); dy and x as they lie
+    assert peak(lambda: torch.autograd.grad(y, (x, W), dy, retain_graph=True)) <= 50 * MB

@@ -43,3 +43,27 @@ def test_linear_refuses_more_tiles_than_a_launch():
     back = lambda M, K, N: lib.tb_linres_bwd(p, N, p, K, p, K, 0, 0, p, p, p, M, K, N, 1, p, wide, 0)
     assert lin(10 ** 9, 8, 4 * 10 ** 6) == 3 and back(10 ** 9, 8, 4 * 10 ** 6) == 3 and back(10 ** 9, 4 * 10 ** 6, 8) == 3
     assert back(100, 4 * 10 ** 6, 4 * 10 ** 6) == 3
+
+
+def test_linear_workspaces_hold_what_a_call_lays_out():
+    """The size for given operands: never above the size for any operands, next to nothing where all are read in place, and checked."""
+    import itertools
+    from timeband_amd import _lib
+    lib = _lib.load()
+    fwd, bwd, any_ = lib.tb_linres_fwd_workspace_bytes, lib.tb_linres_bwd_workspace_bytes, lib.tb_linres_workspace_bytes
+    sizes = [(1, 8, 16), (32, 8, 16), (33, 16, 16), (100, 72, 2056), (100, 75, 2051), (4099, 1000, 1500), (65536, 256, 256), (300, 4096, 40), (70000, 1030, 3)]
+    for (M, K, N), dtype, at in itertools.product(sizes, (0, 1, 2), (4096, 4098)):
+        assert fwd(at, K, at, K, M, K, N, dtype) <= any_(M, K, N, dtype, 0)
+        for act, dx, dW, db in itertools.product((0, 3, 4), (0, 1), (0, 1), (0, 1)):
+            assert bwd(at, N, at, K, act, dx, dW, db, M, K, N, dtype) <= any_(M, K, N, dtype, 1)
+    p, slack = 4096, 4096
+    assert fwd(p, 2048, p, 2048, 16384, 2048, 8192, 1) <= slack                                 # 16384 x 2048 x 8192 bf16, nothing copied
+    assert bwd(p, 256, p, 256, 0, 1, 0, 0, 65536, 256, 256, 0) <= 256 * 256 * 4 + slack          # fp32 dx: W across
+    assert bwd(p, 256, p, 256, 0, 0, 1, 0, 65536, 256, 256, 0) <= 65 * 256 * 256 * 4 + slack     # fp32 dW: its split sums
+    one = bwd(p, 1024, p, 1024, 0, 1, 0, 0, 8192, 1024, 1024, 2)
+    assert bwd(p, 1024, p, 1024, 3, 1, 0, 0, 8192, 1024, 1024, 2) == one + 8192 * 1024 * 2          # relu: dz in one part
+    assert bwd(p, 1024, p, 1024, 4, 1, 0, 0, 8192, 1024, 1024, 2) == one + 2 * 8192 * 1024 * 2      # SiLU: in two
+    need = fwd(4098, 75, p, 75, 100, 75, 2051, 1)
+    assert lib.tb_linres_fwd(4098, 75, p, 75, 0, 0, 0, p, 0, 100, 75, 2051, 0, 1, p, need - 1, 0) == 4
+    need = bwd(p, 2051, p, 75, 4, 1, 1, 1, 100, 75, 2051, 1)
+    assert lib.tb_linres_bwd(p, 2051, p, 75, p, 75, p, 4, p, p, p, 100, 75, 2051, 1, p, need - 1, 0) == 4

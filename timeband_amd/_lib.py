@@ -60,6 +60,8 @@ SIGNATURES = {
     "tb_scan_bwd": (I, [P, P, P, P, P, P, P, P, P, P, I, P, P, P, P, P, P, P, P, P, P, P, P, I, I, I, I, I, I, P, Z, P]),
     "tb_scan_step": (I, [P, L, P, P, P, P, P, P, P, P, P, I, P, I, I, I, I, I, P]),
     "tb_linres_workspace_bytes": (Z, [L, I, I, I, I]),
+    "tb_linres_fwd_workspace_bytes": (Z, [P, L, P, L, L, I, I, I]),
+    "tb_linres_bwd_workspace_bytes": (Z, [P, L, P, L, I, I, I, I, L, I, I, I]),
     "tb_linres_fwd": (I, [P, L, P, L, P, P, L, P, P, L, I, I, I, I, P, Z, P]),
     "tb_linres_bwd": (I, [P, L, P, L, P, L, P, I, P, P, P, L, I, I, I, P, Z, P]),
     "tb_loss_workspace_bytes": (Z, []),

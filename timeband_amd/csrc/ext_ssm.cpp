@@ -467,8 +467,7 @@ Tensor linres_forward(const Tensor& x, const Tensor& W, const Tensor& b, int act
   const int K = fits("linear_residual", x.size(1)), N = fits("linear_residual", W.size(0)), code = code_of(x);
   Tensor y = at::empty({M, N}, x.options());
   if (z && act) *z = at::empty({M, N}, x.options().dtype(at::kFloat));
-  const size_t need = tb_linres_workspace_bytes(M, K, N, code, 0);
-  Tensor ws = bytes(need, x);
+  Tensor ws = bytes(tb_linres_fwd_workspace_bytes(ptr(x), x.stride(0), ptr(W), W.stride(0), M, K, N, code), x);
   ok(tb_linres_fwd(ptr(x), x.stride(0), ptr(W), W.stride(0), ptr(b), ptr(res), res.defined() ? res.stride(0) : 0, out_ptr(y),
                    z ? out_fptr(*z) : nullptr, M, K, N, act, code, out_ptr(ws), ws.numel(), stream(x)),
      "tb_linres_fwd");
@@ -502,9 +501,9 @@ struct LinResFn : public torch::autograd::Function<LinResFn> {
     if (need[2]) g[2] = make({N});
     if (M) {
       Tensor dy = last_dense(grads[0]);
-      Tensor ws = bytes(tb_linres_workspace_bytes(M, K, N, code, 1), x);
-      ok(tb_linres_bwd(ptr(dy), dy.stride(0), ptr(x), x.stride(0), ptr(W), W.stride(0), fptr(z), (int)ctx->saved_data["act"].toInt(), out_ptr(g[0]),
-                       out_ptr(g[1]), out_ptr(g[2]), M, K, N, code, out_ptr(ws), ws.numel(), stream(x)),
+      const int act = (int)ctx->saved_data["act"].toInt();
+      Tensor ws = bytes(tb_linres_bwd_workspace_bytes(ptr(dy), dy.stride(0), ptr(x), x.stride(0), act, need[0], need[1], need[2], M, K, N, code), x);
+      ok(tb_linres_bwd(ptr(dy), dy.stride(0), ptr(x), x.stride(0), ptr(W), W.stride(0), fptr(z), act, out_ptr(g[0]), out_ptr(g[1]), out_ptr(g[2]), M, K, N, code, out_ptr(ws), ws.numel(), stream(x)),
          "tb_linres_bwd");
     }
     return once(std::move(g));

@@ -910,10 +910,37 @@ bool direct(const void* p, long ld, long K) { return aligned(p) && ld % (16 / (l
 
 long up(long x, int esize) { return (x + 16 / esize - 1) / (16 / esize) * (16 / esize); }
 
+// What a forward call does with its operands and workspace: asked by who sizes the workspace and by the call itself.
+struct FwdLayout {
+  bool few, pack_x, pack_w;
+  long Kp;
+  Plan p;
+  size_t x, w, slab, total;        // bytes of the copies of x and W, and of the split sums
+};
 template <typename T>
-int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, int N, char* ws, hipStream_t s) {
+FwdLayout fwd_layout(const void* x, long ldx, const void* W, long ldw, long M, int K, int N) {
+  constexpr int es = sizeof(T);
+  FwdLayout l{};
+  l.few = M <= FEW;
+  l.Kp = up(K, es);
+  if (!l.few) {
+    l.pack_x = !direct<T>(x, ldx, K);
+    l.pack_w = !direct<T>(W, ldw, K);
+    l.p = plan(M, N, l.Kp, es);
+    l.x = l.pack_x ? tb_align_up((size_t)M * l.Kp * es, 256) : 0;
+    l.w = l.pack_w ? tb_align_up((size_t)N * l.Kp * es, 256) : 0;
+    l.slab = slab_bytes(M, N, l.Kp, es);
+  }
+  l.total = l.x + l.w + l.slab + 256;
+  return l;
+}
+
+template <typename T>
+int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, int N, char* ws, size_t ws_bytes, hipStream_t s) {
   constexpr int CE = 16 / sizeof(T);
-  if (M <= FEW) {
+  const FwdLayout l = fwd_layout<T>(x, ldx, W, ldw, M, K, N);
+  if (ws_bytes < l.total) return tb_set_error(TB_ERR_WORKSPACE, "linres_fwd: workspace too small");
+  if (l.few) {
     FewArgs a{x, W, ldx, ldw, M, N, K, 0, e};
     a.vec = direct<T>(x, ldx, K) && direct<T>(W, ldw, K);
     const unsigned grid = (N + 15) / 16;
@@ -922,30 +949,26 @@ int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, in
     TB_LAUNCH_CHECK("linres gemm_few");
     return TB_OK;
   }
-  const long Kp = up(K, sizeof(T));
-  const bool dxr = direct<T>(x, ldx, K), dwr = direct<T>(W, ldw, K);
+  const long Kp = l.Kp;
   T* xp = reinterpret_cast<T*>(ws);
-  ws += tb_align_up((size_t)M * Kp * sizeof(T), 256);
-  T* wp = reinterpret_cast<T*>(ws);
-  ws += tb_align_up((size_t)N * Kp * sizeof(T), 256);
-  const long bx = dxr ? 0 : (M * (Kp / CE) + 255) / 256, bw = dwr ? 0 : ((long)N * (Kp / CE) + 255) / 256;
+  T* wp = reinterpret_cast<T*>(ws + l.x);
+  const long bx = l.pack_x ? (M * (Kp / CE) + 255) / 256 : 0, bw = l.pack_w ? ((long)N * (Kp / CE) + 255) / 256 : 0;
   if (!tb_grid_ok(bx + bw, 256))
     return tb_set_error(TB_ERR_UNSUPPORTED, "linres_fwd: M=%ld K=%d N=%d, off the alignment of 16 bytes, are too many in one call", M, K, N);
   if (bx + bw) {
     pack_rows<T><<<(unsigned)(bx + bw), 256, 0, s>>>(Rows<T>{x, ldx, M, xp}, Rows<T>{W, ldw, N, wp}, (unsigned)bx, K, (int)Kp);
     TB_LAUNCH_CHECK("linres pack");
   }
-  if (!dxr) {
+  if (l.pack_x) {
     x = xp;
     ldx = Kp;
   }
-  if (!dwr) {
+  if (l.pack_w) {
     W = wp;
     ldw = Kp;
   }
-  const Plan p = plan(M, N, Kp, sizeof(T));
-  const GemmArgs a = gemm_args<T>(p, x, ldx, W, ldw, M, N, Kp, e, reinterpret_cast<float*>(ws));
-  const int rc = launch<T, false>(a, p.big, s);
+  const GemmArgs a = gemm_args<T>(l.p, x, ldx, W, ldw, M, N, Kp, e, reinterpret_cast<float*>(ws + l.x + l.w));
+  const int rc = launch<T, false>(a, l.p.big, s);
   if (rc || a.splits == 1) return rc;
   split_finish<T><<<split_blocks(a), 256, 0, s>>>(a.e, M, N, a.splits);
   TB_LAUNCH_CHECK("linres split_finish");
@@ -955,59 +978,75 @@ int forward(const T* x, long ldx, const T* W, long ldw, Epi e, long M, int K, in
 // rows of what the backward pass lays out start on whole lines (a row off them costs its copies another line each)
 long pitch(long x, int esize) { return (x + 128 / esize - 1) / (128 / esize) * (128 / esize); }
 
-struct BwdSizes {
-  size_t dz, dzT, WT, xT, part, slab_x, slab_w, total;
-  long Np, Mp;
+// The same of a backward call: which of dx, dW and db are wanted, and whether there is an activation, decide too.
+struct BwdLayout {
+  bool as_is, down, across, two;   // dz is dy and can be copied as it lies; dW from dz and x as they are, or from both across; dz in two parts
+  long Np, Mp, Kw, Kx;
+  Plan pw, px;
+  size_t dz, dzT, WT, xT, part, slab_x, slab_w, total;      // bytes; dz and dzT with both parts, one behind the other
 };
-// dz and dzT in up to two parts, one behind the other
-BwdSizes bwd_sizes(long M, int K, int N, int es, int parts) {
-  BwdSizes b;
-  b.Np = pitch(N, es);
-  b.Mp = pitch(M, es);
-  b.dz = tb_align_up((size_t)M * b.Np * es, 256) * parts;
-  b.dzT = tb_align_up((size_t)N * b.Mp * es, 256) * parts;
-  b.WT = tb_align_up((size_t)K * b.Np * es, 256);
-  b.xT = tb_align_up((size_t)K * b.Mp * es, 256);
-  b.part = tb_align_up((size_t)((M + 63) / 64) * N * 4, 256);
-  const size_t w = slab_bytes(N, K, up(M, es), es, false, parts), wd = slab_bytes(N, K, M, es, true);
-  b.slab_x = slab_bytes(M, K, up(N, es), es, false, parts);
-  b.slab_w = w > wd ? w : wd;
-  b.total = b.dz + b.dzT + b.WT + b.xT + b.part + b.slab_x + b.slab_w + 256;
-  return b;
+template <typename T>
+BwdLayout bwd_layout(const void* dy, long ldy, const void* x, long ldx, int act, bool dx, bool dW, bool db, long M, int K, int N) {
+  constexpr int es = sizeof(T);
+  BwdLayout l{};
+  l.two = es == 2 && act && act != 3;                   // dy act'(z) of relu is dy or 0: one value holds it
+  l.as_is = !act && direct<T>(dy, ldy, N);
+  l.down = es == 4 && dW && direct<T>(x, ldx, K);
+  l.across = dW && !l.down;
+  l.Np = pitch(N, es);
+  l.Mp = pitch(M, es);
+  l.Kw = l.down ? M : up(M, es);
+  l.Kx = up(N, es);
+  const int parts = l.two ? 2 : 1;
+  l.pw = plan(N, K, l.Kw, es, l.down, parts);
+  l.px = plan(M, K, l.Kx, es, false, parts);
+  l.dz = !l.as_is && (dx || l.down) ? tb_align_up((size_t)M * l.Np * es, 256) * parts : 0;
+  l.dzT = l.across ? tb_align_up((size_t)N * l.Mp * es, 256) * parts : 0;
+  l.WT = dx ? tb_align_up((size_t)K * l.Np * es, 256) : 0;
+  l.xT = l.across ? tb_align_up((size_t)K * l.Mp * es, 256) : 0;
+  l.part = db ? tb_align_up((size_t)((M + 63) / 64) * N * 4, 256) : 0;
+  l.slab_x = dx ? slab_bytes(M, K, l.Kx, es, false, parts) : 0;
+  l.slab_w = dW ? slab_bytes(N, K, l.Kw, es, l.down, parts) : 0;
+  l.total = l.dz + l.dzT + l.WT + l.xT + l.part + l.slab_x + l.slab_w + 256;
+  return l;
 }
 
 template <typename T>
 int backward(const T* dy, long ldy, const T* x, long ldx, const T* W, long ldw, const float* z, int act, T* dx, T* dW, T* db, long M, int K,
-             int N, char* ws, hipStream_t s) {
-  const bool two = sizeof(T) == 2 && z && act != 3;     // dy act'(z) of relu is dy or 0: one value holds it
-  const BwdSizes b = bwd_sizes(M, K, N, sizeof(T), two ? 2 : 1);
-  T* dz = reinterpret_cast<T*>(ws);
-  T* dzT = reinterpret_cast<T*>(ws + b.dz);
-  T* const lo = two ? reinterpret_cast<T*>(ws + b.dz / 2) : nullptr;
-  T* const loT = two ? reinterpret_cast<T*>(ws + b.dz + b.dzT / 2) : nullptr;
-  T* WT = reinterpret_cast<T*>(ws + b.dz + b.dzT);
-  T* xT = reinterpret_cast<T*>(ws + b.dz + b.dzT + b.WT);
-  float* part = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT);
-  float* slab_x = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT + b.part);
-  float* slab_w = reinterpret_cast<float*>(ws + b.dz + b.dzT + b.WT + b.xT + b.part + b.slab_x);
-  const bool as_is = !z && direct<T>(dy, ldy, N);      // dz = dy, and its rows can be copied as they are
+             int N, char* ws, size_t ws_bytes, hipStream_t s) {
+  const BwdLayout b = bwd_layout<T>(dy, ldy, x, ldx, act, dx, dW, db, M, K, N);
+  if (ws_bytes < b.total) return tb_set_error(TB_ERR_WORKSPACE, "linres_bwd: workspace too small");
+  const bool two = b.two, as_is = b.as_is, down = b.down, across = b.across;
+  size_t used = 0;
+  auto take = [&](size_t n) {
+    char* p = n ? ws + used : nullptr;
+    used += n;
+    return p;
+  };
+  T* const dz = reinterpret_cast<T*>(take(b.dz));
+  T* const dzT = reinterpret_cast<T*>(take(b.dzT));
+  T* const WT = reinterpret_cast<T*>(take(b.WT));
+  T* const xT = reinterpret_cast<T*>(take(b.xT));
+  float* const part = reinterpret_cast<float*>(take(b.part));
+  float* const slab_x = reinterpret_cast<float*>(take(b.slab_x));
+  float* const slab_w = reinterpret_cast<float*>(take(b.slab_w));
+  T* const lo = two && dz ? dz + b.dz / 2 / sizeof(T) : nullptr;
+  T* const loT = two && dzT ? dzT + b.dzT / 2 / sizeof(T) : nullptr;
   const T* dzr = as_is ? dy : dz;
   const long ldz = as_is ? ldy : b.Np;
-  const bool down = sizeof(T) == 4 && dW && direct<T>(x, ldx, K);      // dW from dz and x as they are
-  const bool across = dW && !down;
 
   auto tiles = [](long rows, long cols) { return ((rows + 63) / 64) * ((cols + 63) / 64); };
   const long nz = !as_is || across || db ? tiles(M, b.Np) : 0, nw = dx ? tiles(b.Np, K) : 0, nx = across ? tiles(b.Mp, K) : 0;
   if (!tb_grid_ok(nz + nw + nx, 256)) return tb_set_error(TB_ERR_UNSUPPORTED, "linres_bwd: M=%ld K=%d N=%d are too many in one call", M, K, N);
   if (nz + nw + nx) {
-    DzArgs<T> az{dy, ldy, z, act, N, (int)b.Np, M, b.Mp, as_is || !(dx || down) ? nullptr : dz, across ? dzT : nullptr, lo, loT, two, db ? part : nullptr, (unsigned)nz};
+    DzArgs<T> az{dy, ldy, z, act, N, (int)b.Np, M, b.Mp, dz, dzT, lo, loT, two, part, (unsigned)nz};
     Across<T> aw{W, ldw, N, K, WT, b.Np, (unsigned)nw}, ax{x, ldx, M, K, xT, b.Mp, (unsigned)nx};
     lay_out<T><<<(unsigned)(nz + nw + nx), 256, 0, s>>>(az, aw, ax);
     TB_LAUNCH_CHECK("linres lay_out");
   }
 
-  const long Kw = down ? M : up(M, sizeof(T)), Kx = up(N, sizeof(T));
-  const Plan pw = plan(N, K, Kw, sizeof(T), down, two ? 2 : 1), px = plan(M, K, Kx, sizeof(T), false, two ? 2 : 1);
+  const long Kw = b.Kw, Kx = b.Kx;
+  const Plan &pw = b.pw, &px = b.px;
   Epi ew{}, ex{};
   ew.y = dW;
   ex.y = dx;
@@ -1060,16 +1099,41 @@ int check_common(const char* what, long M, int K, int N, int act, int dtype) {
 
 extern "C" {
 
+// enough for any operands of these sizes: none on 16 bytes, every gradient, an activation
 size_t tb_linres_workspace_bytes(long M, int K, int N, int dtype, int backward) {
   if (M < 1 || K < 1 || N < 1 || !tb_dtype_ok(dtype)) return 256;
   const int es = (int)tb_dtype_size(dtype);
-  if (backward) {                                // whatever the activation: of 16-bit types in one part or two
-    const size_t one = bwd_sizes(M, K, N, es, 1).total, two = es == 2 ? bwd_sizes(M, K, N, es, 2).total : 0;
-    return one > two ? one : two;
+  if (!backward) {
+    if (M <= FEW) return 256;
+    const long Kp = up(K, es);
+    return tb_align_up((size_t)M * Kp * es, 256) + tb_align_up((size_t)N * Kp * es, 256) + slab_bytes(M, N, Kp, es) + 256;
   }
-  if (M <= FEW) return 256;
-  const long Kp = up(K, es);
-  return tb_align_up((size_t)M * Kp * es, 256) + tb_align_up((size_t)N * Kp * es, 256) + slab_bytes(M, N, Kp, es) + 256;
+  auto most = [&](auto of) {
+    size_t m = 0;
+    for (int parts = 1; parts <= (es == 2 ? 2 : 1); ++parts) {
+      const size_t n = of(parts);
+      if (n > m) m = n;
+    }
+    return m;
+  };
+  const long Np = pitch(N, es), Mp = pitch(M, es);
+  const size_t across = most([&](int q) { return slab_bytes(N, K, up(M, es), es, false, q); }), down = es == 4 ? slab_bytes(N, K, M, es, true) : 0;
+  return most([&](int q) { return (tb_align_up((size_t)M * Np * es, 256) + tb_align_up((size_t)N * Mp * es, 256)) * q; }) +
+         tb_align_up((size_t)K * Np * es, 256) + tb_align_up((size_t)K * Mp * es, 256) + tb_align_up((size_t)((M + 63) / 64) * N * 4, 256) +
+         most([&](int q) { return slab_bytes(M, K, up(N, es), es, false, q); }) + (across > down ? across : down) + 256;
+}
+
+size_t tb_linres_fwd_workspace_bytes(const void* x, long x_row_stride, const void* W, long w_row_stride, long M, int K, int N, int dtype) {
+  if (M < 1 || K < 1 || N < 1 || !tb_dtype_ok(dtype)) return 256;
+  if (dtype == TB_F32) return fwd_layout<float>(x, x_row_stride, W, w_row_stride, M, K, N).total;
+  return fwd_layout<_Float16>(x, x_row_stride, W, w_row_stride, M, K, N).total;      // of bf16 too: layouts go by the element's size
+}
+
+size_t tb_linres_bwd_workspace_bytes(const void* dy, long dy_row_stride, const void* x, long x_row_stride, int act, int want_dx, int want_dW,
+                                     int want_db, long M, int K, int N, int dtype) {
+  if (M < 1 || K < 1 || N < 1 || !tb_dtype_ok(dtype)) return 256;
+  if (dtype == TB_F32) return bwd_layout<float>(dy, dy_row_stride, x, x_row_stride, act, want_dx, want_dW, want_db, M, K, N).total;
+  return bwd_layout<_Float16>(dy, dy_row_stride, x, x_row_stride, act, want_dx, want_dW, want_db, M, K, N).total;
 }
 
 int tb_linres_fwd(const void* x, long x_row_stride, const void* W, long w_row_stride, const void* b, const void* residual,
@@ -1079,13 +1143,12 @@ int tb_linres_fwd(const void* x, long x_row_stride, const void* W, long w_row_st
   if (rc) return rc;
   if (M == 0) return TB_OK;
   if (!x || !W || !y || !ws) return tb_set_error(TB_ERR_ARG, "linres_fwd: null pointer");
-  if (ws_bytes < tb_linres_workspace_bytes(M, K, N, dtype, 0)) return tb_set_error(TB_ERR_WORKSPACE, "linres_fwd: workspace too small");
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* w = static_cast<char*>(ws);
   Epi e{b, residual, y, z, nullptr, residual_row_stride, act};
-  if (dtype == TB_F32) return forward<float>((const float*)x, x_row_stride, (const float*)W, w_row_stride, e, M, K, N, w, s);
-  if (dtype == TB_BF16) return forward<__bf16>((const __bf16*)x, x_row_stride, (const __bf16*)W, w_row_stride, e, M, K, N, w, s);
-  return forward<_Float16>((const _Float16*)x, x_row_stride, (const _Float16*)W, w_row_stride, e, M, K, N, w, s);
+  if (dtype == TB_F32) return forward<float>((const float*)x, x_row_stride, (const float*)W, w_row_stride, e, M, K, N, w, ws_bytes, s);
+  if (dtype == TB_BF16) return forward<__bf16>((const __bf16*)x, x_row_stride, (const __bf16*)W, w_row_stride, e, M, K, N, w, ws_bytes, s);
+  return forward<_Float16>((const _Float16*)x, x_row_stride, (const _Float16*)W, w_row_stride, e, M, K, N, w, ws_bytes, s);
 }
 
 int tb_linres_bwd(const void* dy, long dy_row_stride, const void* x, long x_row_stride, const void* W, long w_row_stride, const float* z,
@@ -1094,12 +1157,11 @@ int tb_linres_bwd(const void* dy, long dy_row_stride, const void* x, long x_row_
   if (rc) return rc;
   if (M < 1) return tb_set_error(TB_ERR_ARG, "linres_bwd: no rows have no gradients to form here");
   if (!dy || (dx && !W) || (dW && !x) || (act && !z) || !ws) return tb_set_error(TB_ERR_ARG, "linres_bwd: null pointer");
-  if (ws_bytes < tb_linres_workspace_bytes(M, K, N, dtype, 1)) return tb_set_error(TB_ERR_WORKSPACE, "linres_bwd: workspace too small");
   hipStream_t s = static_cast<hipStream_t>(stream);
   char* w = static_cast<char*>(ws);
   const float* zz = act ? z : nullptr;
 #define TB_BWD(T) \
-  return backward<T>((const T*)dy, dy_row_stride, (const T*)x, x_row_stride, (const T*)W, w_row_stride, zz, act, (T*)dx, (T*)dW, (T*)db, M, K, N, w, s)
+  return backward<T>((const T*)dy, dy_row_stride, (const T*)x, x_row_stride, (const T*)W, w_row_stride, zz, act, (T*)dx, (T*)dW, (T*)db, M, K, N, w, ws_bytes, s)
   if (dtype == TB_F32) TB_BWD(float);
   if (dtype == TB_BF16) TB_BWD(__bf16);
   TB_BWD(_Float16);
