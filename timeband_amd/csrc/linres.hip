@@ -841,7 +841,10 @@ struct Plan {
   bool big;
   int tm, tn, splits, per;
 };
-// 256 x 256 tiles where they fill the chip, 128 x 128 otherwise (two blocks a unit).  k is split where even those leave units
+// 256 x 256 tiles where they fill the chip, whatever K: 128 x 128 ones (two blocks a unit) move twice the operands and win nothing even
+// where prologue and epilogue are most of the time.  K = 64, 128, 256, 512, 1024, 2048, us with 256 (128): 65536 x K x 256 bf16 14 (14), 17 (17), 20 (23),
+// 27 (33), 41 (53), 86 (112), fp32 35 (35), 51 (53), 83 (86), 145 (156), 265 (284), 484 (523); 16384 x K x 4096 bf16 45 (45), 53 (53), 66 (70), 93 (98),
+// 142 (165), 241 (308).  128 x 128 otherwise; k is split where even those leave units
 // idle, into parts of sixteen k tiles (1 KB of a row) at least, of fp32, whose products take longer a byte, of four: 1000 x 1000 x 1000
 // fp32 in parts of 16, 8, 4, 2 tiles 33.5, 29.9, 29.6, 29.7 us, 241 x 2048 x 272 24.5, 18.2, 16.4, 16.4; 1024 x 1024 x 1024 bf16
 // 16.7, 20.4, 20.4, 20.5.
