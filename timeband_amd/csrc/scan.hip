@@ -68,6 +68,9 @@ __device__ __forceinline__ float softplus(float x) {
   return x > 20.f ? x : m > 0.f ? l : e;
 }
 
+// v or 0, by a mask of all its bits: no branch around what makes v
+__device__ __forceinline__ float only(float v, unsigned mask) { return __uint_as_float(__float_as_uint(v) & mask); }
+
 template <int CTRL>
 __device__ __forceinline__ float dpp(float v) {
   return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
@@ -250,10 +253,12 @@ __device__ __forceinline__ void chain(const ScanArgs& a, int b, int chunk, long 
 }
 
 // forward.  STATE: only the chunk's end state from zero and its sum of delta (first pass over chunks).
+// fp32 is held to four waves a SIMD (4 x 2048 x 2048 x 16 146 us, with three 158); 16-bit types reach them, and are slower held to it
+// (1 x 16384 x 2048 x 16 bf16 277 us, 271).
 // PART: N is not 4 S, and the states behind it are kept at 0: their products are 0 times what may be infinite.  Kernels of their own, so that
 // whole states take no selects (4 x 2048 x 2048 x 11 fp32: forward 144 us without them, 150 with; gradients too 491, 506).
 template <typename T, int S, bool STATE, bool VEC, bool PART>
-__global__ void __launch_bounds__(256, VEC && S <= 4 ? 4 : 1) scan_fwd(ScanArgs a) {      // four waves a SIMD (4 x 2048 x 2048 x 16 fp32 145 us, three 158)
+__global__ void __launch_bounds__(256, sizeof(T) == 4 && VEC && S <= 4 ? 4 : 1) scan_fwd(ScanArgs a) {
   constexpr int TT = 32, EPT = 8, NP = 4 * S;
   __shared__ float sD[TT][CB][2];            // delta, delta u
   __shared__ float sB[TT * NP], sC[STATE ? 1 : TT * NP];
@@ -302,6 +307,7 @@ __global__ void __launch_bounds__(256, VEC && S <= 4 ? 4 : 1) scan_fwd(ScanArgs 
     rB.fetch(a.Bm, bo, a.sBt, t0, tv, a.N);
     if (!STATE) rC.fetch(a.Cm, co, a.sCt, t0, tv, a.N);
   };
+  const unsigned skip = a.Dp ? ~0u : 0u;
   load(ts);
   for (int t0 = ts; t0 < te; t0 += TT) {
     const int t = t0 + ct;
@@ -320,7 +326,7 @@ __global__ void __launch_bounds__(256, VEC && S <= 4 ? 4 : 1) scan_fwd(ScanArgs 
       else d = on ? d : 0.f;
       sD[ct][cc + i][0] = d;
       sD[ct][cc + i][1] = d * u[i];
-      if (!STATE) u[i] = a.Dp ? u[i] : 0.f;      // no skip term: 0 times u is none where u is infinite
+      if (!STATE) u[i] = only(u[i], skip);       // no skip term: 0 times u is none where u is infinite
     }
     rB.store(sB, t0, tv, a.N);
     if (!STATE) rC.store(sC, t0, tv, a.N);
@@ -455,6 +461,7 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
              go = (long)w.b * a.sob + gof, oo = (long)w.b * a.T * a.D + gof;
   const long bo = (long)w.b * a.sBb + (long)w.g * a.sBg, co = (long)w.b * a.sCb + (long)w.g * a.sCg;
   const int ch = w.c0 + cc;
+  const unsigned skip = a.Dp ? ~0u : 0u;        // no skip term: 0 times u or dy is none where they are infinite
   float sum = 0.f;
   __syncthreads();
 
@@ -633,7 +640,7 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
           const float dy = sG[ct][cc + i];
-          o[i] = on ? fmaf(sD[ct][cc + i][0], sGB[ct][cc + i], a.Dp ? sPar[1][cc + i] * dy : 0.f) : 0.f;
+          o[i] = on ? fmaf(sD[ct][cc + i][0], sGB[ct][cc + i], only(sPar[1][cc + i] * dy, skip)) : 0.f;
           dD[i] = fmaf(dy, u[i], dD[i]);
         }
         if (a.du) put<T, EPT, VEC>(a.du, oo + (long)t * a.D, ch, a.Dg, o);
@@ -642,7 +649,7 @@ __global__ void __launch_bounds__(256, STATE ? 4 : 2) scan_bwd(ScanArgs a) {
           rz.mask(on, ch, a.Dg, 0.f);
 #pragma unroll
           for (int i = 0; i < EPT; ++i) {
-            const float z = rz.get(i), q = tb_sig(z), y = a.Dp ? fmaf(sPar[1][cc + i], u[i], sY[ct][cc + i]) : sY[ct][cc + i];
+            const float z = rz.get(i), q = tb_sig(z), y = fmaf(sPar[1][cc + i], only(u[i], skip), sY[ct][cc + i]);
             o[i] = on ? ro.get(i) * y * (q * (1.f + z * (1.f - q))) : 0.f;
           }
           put<T, EPT, VEC>(a.dz, oo + (long)t * a.D, ch, a.Dg, o);
