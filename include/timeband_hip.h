@@ -137,7 +137,7 @@ int tb_head_bwd(const float* dy, const float* out, const float* x, const float* 
  * Convolution: y[b,t,d] = act(bias[d] + sum_k w[d,k] x[b,t-K+1+k,d]), act none or silu, K = 1 .. 8.
  *   x (B,T,D), w (D,K), bias (D) nullable; w_f32 != 0: w and bias (and dw, db) are fp32 whatever dtype.
  *   state (B,K-1,D) nullable: the inputs before step 0 (zero without).  lengths (B) int32 nullable: steps at or behind a
- *   sequence's length are not read, their outputs and gradients are zero.  state_out (B,K-1,D) nullable: the last K-1 inputs of each
+ *   sequence's length may hold anything, their outputs and gradients are zero.  state_out (B,K-1,D) nullable: the last K-1 inputs of each
  *   sequence; it must not be `state`.
  *   backward: dx (B,T,D) dense, dw / db nullable; dy dense.
  *   step: x (B,D) with rows x_batch_stride apart, state rows (K-1,D) dense and state_batch_stride apart, shifted IN PLACE. */

@@ -13,8 +13,8 @@
 // much as their own (4099 x 1000 x 1500 fp16 against 64 bits: 2.93e-4 instead of 2.07e-4) and loses fp16 gradients outside its range.
 // Both operands are copied straight to LDS (16 bytes a lane, 64 bytes of a row a tile), tiles ahead of their use; the 16-byte
 // pieces of a row change places by the row's low bits, so that the rows a fragment reads fall on different banks.
-// Measured (bf16, without activation or residual): 16384 x 8192 x 8192 1790 us, 1.23 PFLOP/s (the library's product 1360);
-// 16384 x 2048 x 8192 493 (376), with gelu and residual 585; what bounds the large tiles is LDS (125 of its 128 bytes a
+// Measured (bf16, without activation or residual): 16384 x 8192 x 8192 1948 us, 1.13 PFLOP/s (the library's product 1505 us in turn with it);
+// 16384 x 2048 x 8192 491 us (374), with gelu and residual 571 to 590; what bounds the large tiles is LDS (125 of its 128 bytes a
 // clock at the matrix instructions' full rate), and behind it the epilogue, which one block a unit leaves uncovered.  Not kept:
 // 256 x 128 tiles, two blocks a unit (main loop 507 us against 412 a 2048 of k, LDS bound), 128 x 128 a wave
 // (the compiler moves the 256 sums between register files: 219 TFLOP/s), 256 x 128 one block a unit for middle sizes (same).
@@ -181,8 +181,8 @@ __device__ __forceinline__ void tile_of(int id, int tm, int tn, int& im, int& in
 }
 
 // The epilogue of rows that are whole pieces of V columns: the residual's pieces are fetched two accesses ahead of their use, the
-// activation is chosen once, outside the rows (16384 x 2048 x 8192 with gelu and residual: 685 us, so 585; without both 493, the residual
-// alone adds 58, gelu alone 58; four and eight accesses ahead: 606 and 671).
+// activation is chosen once, outside the rows (16384 x 2048 x 8192 with gelu and residual: 685 us, so 585; without both 491, the residual
+// alone adds 51, gelu alone 49; four and eight accesses ahead: 606 and 671).
 template <typename T, int V>
 __device__ __forceinline__ void whole_rows(const GemmArgs& a, const float* own, long m0, int n0, int lane) {
   constexpr int L = 64 / V;      // lanes a row; V rows an access, L accesses
@@ -291,10 +291,10 @@ __device__ __forceinline__ void write_block(const GemmArgs& a, const float* own,
 // DOWN (fp32, for dW): k runs down the columns of both operands as they are, P[k][m] and Q[k][n], K rows of M and N columns that are
 // whole 16-byte pieces on 16 bytes.  A tile is sixteen rows of BM (BN) columns; a lane takes its k one by one (4 bytes), which the
 // fp32 instructions, a quarter of the 16-bit ones' rate a byte, leave time for.  Saves the transposed copies of dz and x
-// (65536 x 256 x 256: 345 -> 306 us of a training step).
+// (65536 x 256 x 256: 345 us of a training step, so 302).
 //
 // TWO: P comes in two parts, and k runs over all of lo and then over all of P (twice the products; 4099 x 1000 x 1500 fp16 with SiLU and
-// gradients: 145 us, with dz rounded once 102).
+// gradients: 142 us, with dz rounded once 102).
 template <typename T, int BM, int BN, int WM, int WN, bool DOWN, bool TWO>
 __device__ __forceinline__ void product(const GemmArgs& a, int tile, int part, char* lds) {
   static_assert(!DOWN || (sizeof(T) == 4 && BM == 128 && BN == 128), "rows of 512 bytes, two a copy");
@@ -503,8 +503,8 @@ __global__ void __launch_bounds__((BM / WM) * (BN / WN) * 64, 2) gemm(GemmArgs a
 }
 
 // Two products in one launch, the first's blocks in front (dW, whose k is long, and dx): neither fills the chip to its end alone.
-// With the layouts before them and the finishes behind them in one launch each, a training step of 4099 x 1000 x 1500 fp16 takes 104 us
-// (launch by launch 121), 1024^3 fp32 92 (106), 145 x 560 x 301 fp16 38 (46).
+// With the layouts before them and the finishes behind them in one launch each, a training step of 4099 x 1000 x 1500 fp16, dz in one part, took
+// 104 us (launch by launch 121), 1024^3 fp32 92 (106), 145 x 560 x 301 fp16 38 (46).
 template <typename T, bool DOWN, bool TWO>
 __global__ void __launch_bounds__(256, 2) gemm_pair(GemmArgs a, GemmArgs b, unsigned first) {
   __shared__ __attribute__((aligned(16))) char lds[4 * 256 * 64];

@@ -10,8 +10,8 @@
 //
 // Bound by arithmetic: an exponential (a quarter of the vector rate) and four other operations a state and step forward, as many again and
 // nine more backward, against two bytes an element and tensor; where the steps are cut, the first walk comes on top.  Measured, bf16,
-// 16 states, gated: 1 x 16384 x 2048 270 us (537 M state steps; the exponentials and operations of both walks alone are 205 at
-// the vector units' full rate); 4 x 2048 x 2048 with gradients 459 (vector units busy 81 % of the main backward pass, 87 to 93 % of the
+// 16 states, gated: 1 x 16384 x 2048 271 us (537 M state steps; the exponentials and operations of both walks alone are 205 at
+// the vector units' full rate); 4 x 2048 x 2048 with gradients 468 (vector units busy 80 % of the main backward pass, 88 to 92 % of the
 // others).  Layout: a lane owns one channel and S = N/4 of
 // its states, four neighbouring lanes a channel, so that the sum over the states is two quad permutes and a block of four
 // waves owns 64 neighbouring channels (whole lines of every tensor).  Steps go in tiles: a tile's rows are fetched into

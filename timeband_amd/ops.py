@@ -559,8 +559,8 @@ def _ssm():
 def causal_conv(x, weight, bias=None, act=ACT_NONE, state=None, lengths=None, return_state=False):
     """Depthwise causal convolution of x (B,T,D) along its steps: act(bias + sum_k weight[:,k] x[t-K+1+k]), weight (D,K) with
     1 to 8 taps, act ACT_NONE or ACT_SILU; weight and bias of x's type or float32.  state (B,K-1,D): the inputs before step 0
-    (zero without); lengths (B,) int32, taken as between 0 and T: steps at or behind a sequence's length are not read and give
-    zero.  return_state: also the last K-1 inputs of each sequence, for the next call or causal_conv_step (no gradient runs
+    (zero without); lengths (B,) int32, taken as between 0 and T: steps at or behind a sequence's length may hold anything and
+    give zero.  return_state: also the last K-1 inputs of each sequence, for the next call or causal_conv_step (no gradient runs
     through either state)."""
     return (_SSM or _ssm()).causal_conv(x, weight, bias, act, state, lengths, return_state)
 
